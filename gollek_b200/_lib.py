@@ -51,9 +51,20 @@ SIGNATURES = {
                                                    _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                                    _c_ll, _c_int, _c_int, _c_ll, _c_ll, _c_ll,
                                                    _c_float, _c_float, _c_int, _vp]),
+    "gollek_paged_attention_varlen": (_c_int, [_vp] * 12 + [_c_int] * 8 +
+                                      [_c_ll, _c_int, _c_int, _c_ll, _c_ll, _c_ll, _c_float,
+                                       _c_float, _c_int, _c_int, _vp, _c_size, _vp]),
+    "gollek_paged_attention_varlen_workspace_size": (_c_size, [_c_int] * 5),
+    "gollek_paged_attention_shared_prefix": (_c_int, [_vp] * 11 + [_c_int] * 9 +
+                                             [_c_ll, _c_int, _c_int, _c_ll, _c_ll, _c_ll,
+                                              _c_float, _c_float, _vp, _c_size, _vp]),
+    "gollek_paged_attention_shared_prefix_workspace_size": (_c_size, [_c_int] * 5),
     "gollek_kv_append": (_c_int, [_vp, _vp, _c_int, _vp, _vp, _vp, _c_int, _c_int, _vp, _vp, _vp,
                                   _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ll, _c_ll, _c_ll,
                                   _c_ll, _vp]),
+    "gollek_kv_gather": (_c_int, [_vp, _vp, _c_int, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp,
+                                  _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ll, _c_ll,
+                                  _c_ll, _c_ll, _vp]),
     "gollek_kv_migrate": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_ll,
                                    _c_ll, _c_ll, _c_int, _vp]),
     "gollek_kv_block_checksum": (_c_int, [_vp, _vp, _c_int, _c_int, _c_ll, _c_ll, _vp, _vp]),

@@ -13,6 +13,7 @@ import shutil
 import subprocess
 import sys
 import time
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -58,31 +59,43 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
 def _build_locked(verbose: bool) -> str:
     tmp = f"{LIB_PATH}.{os.getpid()}.tmp"
+    units = sorted(glob.glob(os.path.join(CSRC, "*.cu")))
+    objs = [os.path.join(LIB_DIR, f"{os.path.basename(u)}.{os.getpid()}.o") for u in units]
     # The output carries the build's start time, so a source edited while nvcc runs still
     # reads as newer than the library.
     start = time.time()
-    cmd = [
-        nvcc_path(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-shared",
-        "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
-        "--expt-relaxed-constexpr",
-        "-I", os.path.join(ROOT, "include"),
-        "-o", tmp, os.path.join(CSRC, "gollek_kernels.cu"),
-    ]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-    env = dict(os.environ)
+    nvcc = [nvcc_path()]
     # nvcc's host compiler: prefer the system g++ (the environment's CXX may lack libgomp
     # or differ from what libstdc++ on the GPU box expects).
     if os.path.exists("/usr/bin/g++"):
-        cmd[1:1] = ["-ccbin", "/usr/bin/g++"]
-    r = subprocess.run(cmd, env=env, capture_output=True, text=True)
-    if r.returncode != 0:
+        nvcc += ["-ccbin", "/usr/bin/g++"]
+    flags = [*ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
+             "-Xcompiler", "-fvisibility=hidden", "--expt-relaxed-constexpr",
+             "-I", os.path.join(ROOT, "include")]
+    if verbose:
+        flags.append("-Xptxas=-v")
+
+    def run(cmd):
+        return subprocess.run(cmd, env=dict(os.environ), capture_output=True, text=True)
+
+    try:
+        # the translation units compile side by side, then link
+        with ThreadPoolExecutor(len(units)) as pool:
+            done = list(pool.map(lambda uo: run([*nvcc, *flags, "-c", "-o", uo[1], uo[0]]),
+                                 zip(units, objs)))
+        if all(r.returncode == 0 for r in done):
+            done.append(run([*nvcc, *ARCH_FLAGS, "-shared", "-o", tmp, *objs]))
+    finally:
+        for o in objs:
+            if os.path.exists(o):
+                os.remove(o)
+    if any(r.returncode != 0 for r in done):
         if os.path.exists(tmp):
             os.remove(tmp)
-        sys.stderr.write(r.stdout + r.stderr)
+        sys.stderr.write("".join(r.stdout + r.stderr for r in done))
         raise RuntimeError("nvcc failed building libgollek_kernels.so")
     if verbose:
-        sys.stderr.write(r.stderr)
+        sys.stderr.write("".join(r.stderr for r in done))
     os.utime(tmp, (start, start))
     os.replace(tmp, LIB_PATH)
     return LIB_PATH

@@ -53,6 +53,25 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
         return make_float2(bf16_lo(w), bf16_hi(w));
 }
 
+// Element e of a pool (nibble e for int4), before its scale.
+__device__ __forceinline__ float load_kv(const void *base, int dtype, long long e) {
+    switch (dtype) {
+        case GOLLEK_DTYPE_F32:
+            return reinterpret_cast<const float *>(base)[e];
+        case GOLLEK_DTYPE_BF16:
+            return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(base)[e]);
+        case GOLLEK_DTYPE_F16:
+            return __half2float(reinterpret_cast<const __half *>(base)[e]);
+        case GOLLEK_DTYPE_I8:
+            return static_cast<float>(reinterpret_cast<const int8_t *>(base)[e]);
+        default: {  // I4: nibble e of the byte stream, stored as value + 8
+            const int b = reinterpret_cast<const uint8_t *>(base)[e >> 1];
+            const int nib = (e & 1) ? ((b >> 4) & 0xF) : (b & 0xF);
+            return static_cast<float>(nib - 8);
+        }
+    }
+}
+
 // ----------------------------------------------------------------- mbarrier
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {

@@ -33,24 +33,6 @@ struct GenericArgs {
     float q_scale, soft_cap, post_scale, norm_eps;
 };
 
-__device__ __forceinline__ float load_kv(const void *base, int dtype, long long e) {
-    switch (dtype) {
-        case GOLLEK_DTYPE_F32:
-            return reinterpret_cast<const float *>(base)[e];
-        case GOLLEK_DTYPE_BF16:
-            return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(base)[e]);
-        case GOLLEK_DTYPE_F16:
-            return __half2float(reinterpret_cast<const __half *>(base)[e]);
-        case GOLLEK_DTYPE_I8:
-            return static_cast<float>(reinterpret_cast<const int8_t *>(base)[e]);
-        default: {  // I4: nibble e of the byte stream, stored as value + 8
-            const int b = reinterpret_cast<const uint8_t *>(base)[e >> 1];
-            const int nib = (e & 1) ? ((b >> 4) & 0xF) : (b & 0xF);
-            return static_cast<float>(nib - 8);
-        }
-    }
-}
-
 __global__ void __launch_bounds__(kGenWarps * 32) decode_generic_kernel(const GenericArgs a) {
     const int s = blockIdx.x;
     const int h = blockIdx.y;

@@ -19,12 +19,12 @@
 #include "decode_generic.cuh"
 #include "decode_tc.cuh"
 #include "decode_tma.cuh"
+#include "host.cuh"
 #include "kv_append.cuh"
 #include "kv_migrate.cuh"
 #include "prefill_tc.cuh"
 
 namespace gk {
-namespace {
 
 thread_local std::string t_last_error;
 
@@ -42,25 +42,6 @@ int cuda_fail(cudaError_t e, const char *what) {
     cudaGetLastError();  // clear a non-sticky error so the next call starts clean
     return fail(static_cast<int>(e), "%s: %s", what, cudaGetErrorString(e));
 }
-
-#define GK_CUDA(call, what)                        \
-    do {                                           \
-        cudaError_t e_ = (call);                   \
-        if (e_ != cudaSuccess) return cuda_fail(e_, what); \
-    } while (0)
-
-// Restores the caller's current device on scope exit.
-struct DeviceGuard {
-    int prev = -1;
-    explicit DeviceGuard(int dev) {
-        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-        if (dev >= 0 && dev != prev) cudaSetDevice(dev);
-    }
-    ~DeviceGuard() {
-        int cur = -1;
-        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
-    }
-};
 
 // ----------------------------------------------------------- driver entry points
 
@@ -116,7 +97,7 @@ int sm_count(int dev) {
 
 // Library-owned split-K scratch for (device, stream), zero-filled when (re)allocated;
 // *cap_out receives its size.
-int library_workspace(int dev, void *stream, size_t bytes, void **out, size_t *cap_out = nullptr) {
+int library_workspace(int dev, void *stream, size_t bytes, void **out, size_t *cap_out) {
     const size_t tkey = stream == static_cast<void *>(cudaStreamPerThread)
                             ? std::hash<std::thread::id>()(std::this_thread::get_id())
                             : 0;
@@ -152,6 +133,8 @@ int dtype_bytes(int dt) {
             return 0;
     }
 }
+
+namespace {
 
 // Split-K scratch of W bytes: the arrival counters (int per (sequence, kv-head), zero
 // between calls) fill the first W/128 bytes, the partial states follow.  The counter
@@ -291,8 +274,6 @@ CUtensorMapDataType tma_type(int kv) {
         default: return CU_TENSOR_MAP_DATA_TYPE_UINT8;
     }
 }
-
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 struct V2 {
     void *out;
@@ -1413,17 +1394,18 @@ int gollek_device_status(int device, int clear, unsigned int *status_out) {
     if (gollek_cuda_device_count() == 0) return fail(GOLLEK_ERR_NO_DEVICE, "no CUDA device");
     DeviceGuard guard(device);
     GK_CUDA(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
-    unsigned v = 0;
+    unsigned v = 0, w = 0;
     GK_CUDA(cudaMemcpyFromSymbol(&v, g_status, sizeof(v)), "read status");
     if (clear) {
         const unsigned zero = 0;
         GK_CUDA(cudaMemcpyToSymbol(g_status, &zero, sizeof(zero)), "clear status");
     }
+    GK_CUDA(varlen_status(clear != 0, &w), "read status");  // the word of gollek_varlen.cu's kernels
     if (v & GOLLEK_STATUS_TIMEOUT) {
         const int rc = rezero_library_counters(device);
         if (rc) return rc;
     }
-    *status_out = v;
+    *status_out = v | w;
     return GOLLEK_OK;
 }
 

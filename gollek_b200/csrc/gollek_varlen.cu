@@ -1,0 +1,258 @@
+// gollek_varlen.cu -- host side of ragged and shared-prefix paged attention and of the
+// cache read-back: argument checks, kernel selection and their C ABI (gollek_kernels.h).
+#include <algorithm>
+
+#include "host.cuh"
+#include "kv_gather.cuh"
+#include "varlen.cuh"
+
+namespace gk {
+
+cudaError_t varlen_status(bool clear, unsigned *out) {
+    cudaError_t e = cudaMemcpyFromSymbol(out, g_status, sizeof(*out));
+    if (e == cudaSuccess && clear) {
+        const unsigned zero = 0;
+        e = cudaMemcpyToSymbol(g_status, &zero, sizeof(zero));
+    }
+    return e;
+}
+
+namespace {
+
+constexpr long long kMaxTokens = 1LL << 30;  // positions a table may name (32-bit arithmetic on them)
+
+bool float_dtype(int dt) {
+    return dt == GOLLEK_DTYPE_F32 || dt == GOLLEK_DTYPE_BF16 || dt == GOLLEK_DTYPE_F16;
+}
+bool quantised(int dt) { return dt == GOLLEK_DTYPE_I8 || dt == GOLLEK_DTYPE_I4; }
+
+// What every entry point here checks of a pool; *stride receives the page stride in use.
+int check_pool(int kv_dtype, const float *ks, const float *vs, int num_kv_heads, int head_dim, int block_size,
+               int max_blocks, int num_blocks, long long page_stride, long long *stride) {
+    if (num_kv_heads <= 0 || head_dim <= 0 || block_size <= 0 || max_blocks <= 0 || num_blocks < 0)
+        return fail(GOLLEK_ERR_INVALID_ARGUMENT, "non-positive size");
+    if (kv_dtype < GOLLEK_DTYPE_F32 || kv_dtype > GOLLEK_DTYPE_I4)
+        return fail(GOLLEK_ERR_UNSUPPORTED, "kv dtype %d", kv_dtype);
+    if (quantised(kv_dtype) && (!ks || !vs))
+        return fail(GOLLEK_ERR_INVALID_ARGUMENT, "quantised KV needs k_scales and v_scales");
+    const long long minimal = static_cast<long long>(num_kv_heads) * block_size * head_dim;
+    if (page_stride != 0 && page_stride < minimal)
+        return fail(GOLLEK_ERR_INVALID_ARGUMENT, "page_stride %lld < num_kv_heads*block_size*head_dim", page_stride);
+    *stride = page_stride ? page_stride : minimal;
+    if (kv_dtype == GOLLEK_DTYPE_I4 && ((head_dim & 1) || (*stride & 1)))
+        return fail(GOLLEK_ERR_UNSUPPORTED, "int4 pools need an even head_dim and page stride");
+    if (static_cast<long long>(max_blocks) * block_size > kMaxTokens)
+        return fail(GOLLEK_ERR_INVALID_ARGUMENT, "max_blocks_per_seq * block_size too large");
+    return GOLLEK_OK;
+}
+
+int check_attn(const AttnArgs &a) {
+    if (a.num_q_heads <= 0 || a.num_q_heads % a.num_kv_heads != 0)
+        return fail(GOLLEK_ERR_INVALID_ARGUMENT, "num_q_heads %d not a multiple of num_kv_heads %d", a.num_q_heads,
+                    a.num_kv_heads);
+    if (!float_dtype(a.q_dtype)) return fail(GOLLEK_ERR_UNSUPPORTED, "q dtype %d (F32, BF16 or F16 only)", a.q_dtype);
+    if (a.head_dim > 256) return fail(GOLLEK_ERR_UNSUPPORTED, "head_dim %d above 256", a.head_dim);
+    if (a.num_kv_heads > 65535 || a.num_q_heads / a.num_kv_heads > 65535)
+        return fail(GOLLEK_ERR_UNSUPPORTED, "more than 65535 heads");
+    return GOLLEK_OK;
+}
+
+template <int J>
+const void *generic_fn(int G) {
+    if (G == 1) return reinterpret_cast<const void *>(&attn_generic_kernel<J, 1>);
+    if (G == 2) return reinterpret_cast<const void *>(&attn_generic_kernel<J, 2>);
+    if constexpr (J < 8)
+        if (G > 4) return reinterpret_cast<const void *>(&attn_generic_kernel<J, 8>);
+    return reinterpret_cast<const void *>(&attn_generic_kernel<J, 4>);
+}
+
+int launch_generic(AttnArgs &a, cudaStream_t st) {
+    const int G = a.num_q_heads / a.num_kv_heads;
+    const int J = a.head_dim <= 64 ? 2 : a.head_dim <= 128 ? 4 : 8;
+    const void *fn = J == 2 ? generic_fn<2>(G) : J == 4 ? generic_fn<4>(G) : generic_fn<8>(G);
+    const int GC = G == 1 ? 1 : G == 2 ? 2 : (G <= 4 || J == 8) ? 4 : 8;
+    void *args[] = {&a};
+    GK_CUDA(cudaLaunchKernel(fn, dim3(a.total_q, a.num_kv_heads, (G + GC - 1) / GC), dim3(kAgWarps * 32), args, 0, st),
+            "attn_generic_kernel launch");
+    return GOLLEK_OK;
+}
+
+}  // namespace
+}  // namespace gk
+
+using namespace gk;
+
+extern "C" {
+
+int gollek_paged_attention_varlen(void *out, const void *q, const void *k_cache, const void *v_cache,
+                                  const float *k_scales, const float *v_scales, const int *block_tables,
+                                  const int *cu_seqlens_q, const int *context_lens, const float *alibi_slopes,
+                                  const int *prefix_lens, const int *token_starts, int num_seqs, int total_queries,
+                                  int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                                  int max_blocks_per_seq, int num_blocks, long long page_stride, int q_dtype,
+                                  int kv_dtype, long long scale_page_stride, long long scale_head_stride,
+                                  long long scale_token_stride, float scale, float soft_cap, int sliding_window,
+                                  int causal, void *workspace, size_t workspace_bytes, void *stream) {
+    t_last_error.clear();
+    AttnArgs a{};
+    int rc = check_pool(kv_dtype, k_scales, v_scales, num_kv_heads, head_dim, block_size, max_blocks_per_seq, num_blocks,
+                        page_stride, &a.page_stride);
+    if (rc) return rc;
+    if (num_seqs < 0 || total_queries < 0 || total_queries > kMaxTokens)
+        return fail(GOLLEK_ERR_INVALID_ARGUMENT, "num_seqs or total_queries out of range");
+    if (num_seqs == 0 || total_queries == 0) return GOLLEK_OK;
+    if (!out || !q || !k_cache || !v_cache || !block_tables || !cu_seqlens_q || !context_lens)
+        return fail(GOLLEK_ERR_INVALID_ARGUMENT, "null tensor pointer");
+    if (!causal && sliding_window > 0)
+        return fail(GOLLEK_ERR_UNSUPPORTED, "a sliding window without causal masking");
+    a.out = out;
+    a.q = q;
+    a.k = k_cache;
+    a.v = v_cache;
+    a.k_scales = quantised(kv_dtype) ? k_scales : nullptr;
+    a.v_scales = quantised(kv_dtype) ? v_scales : nullptr;
+    a.block_tables = block_tables;
+    a.context_lens = context_lens;
+    a.cu = cu_seqlens_q;
+    a.slopes = alibi_slopes;
+    a.prefix_lens = prefix_lens;
+    a.token_starts = token_starts;
+    a.scale_page_stride = scale_page_stride;
+    a.scale_head_stride = scale_head_stride;
+    a.scale_token_stride = scale_token_stride;
+    a.num_seqs = num_seqs;
+    a.total_q = total_queries;
+    a.num_q_heads = num_q_heads;
+    a.num_kv_heads = num_kv_heads;
+    a.head_dim = head_dim;
+    a.block_size = block_size;
+    a.max_blocks = max_blocks_per_seq;
+    a.num_blocks = num_blocks;
+    a.causal = causal != 0;
+    a.window = sliding_window > 0 ? std::min<int>(sliding_window, 1 << 30) : 0;
+    a.q_dtype = q_dtype;
+    a.kv_dtype = kv_dtype;
+    a.soft_cap = soft_cap > 0.f ? soft_cap : 0.f;
+    a.q_scale = a.soft_cap > 0.f ? scale : scale * kLog2e;
+    rc = check_attn(a);
+    if (rc) return rc;
+    (void)workspace;
+    (void)workspace_bytes;
+    return launch_generic(a, static_cast<cudaStream_t>(stream));
+}
+
+size_t gollek_paged_attention_varlen_workspace_size(int num_seqs, int total_queries, int num_q_heads, int num_kv_heads,
+                                                    int head_dim) {
+    (void)num_seqs, (void)total_queries, (void)num_q_heads, (void)num_kv_heads, (void)head_dim;
+    return 0;
+}
+
+int gollek_paged_attention_shared_prefix(void *out, const void *q, const void *k_cache, const void *v_cache,
+                                         const float *k_scales, const float *v_scales, const int *prefix_tables,
+                                         const int *prefix_lens, const int *group_starts, const int *block_tables,
+                                         const int *context_lens, int num_groups, int max_prefix_blocks, int num_seqs,
+                                         int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+                                         int max_blocks_per_seq, int num_blocks, long long page_stride, int q_dtype,
+                                         int kv_dtype, long long scale_page_stride, long long scale_head_stride,
+                                         long long scale_token_stride, float scale, float soft_cap, void *workspace,
+                                         size_t workspace_bytes, void *stream) {
+    t_last_error.clear();
+    AttnArgs a{};
+    int rc = check_pool(kv_dtype, k_scales, v_scales, num_kv_heads, head_dim, block_size, max_blocks_per_seq, num_blocks,
+                        page_stride, &a.page_stride);
+    if (rc) return rc;
+    if (num_seqs < 0 || num_groups <= 0 || max_prefix_blocks <= 0 ||
+        static_cast<long long>(max_prefix_blocks) * block_size > kMaxTokens)
+        return fail(GOLLEK_ERR_INVALID_ARGUMENT, "num_seqs, num_groups or max_prefix_blocks out of range");
+    if (num_seqs == 0) return GOLLEK_OK;
+    if (!out || !q || !k_cache || !v_cache || !prefix_tables || !prefix_lens || !group_starts || !block_tables ||
+        !context_lens)
+        return fail(GOLLEK_ERR_INVALID_ARGUMENT, "null tensor pointer");
+    a.out = out;
+    a.q = q;
+    a.k = k_cache;
+    a.v = v_cache;
+    a.k_scales = quantised(kv_dtype) ? k_scales : nullptr;
+    a.v_scales = quantised(kv_dtype) ? v_scales : nullptr;
+    a.block_tables = block_tables;
+    a.context_lens = context_lens;
+    a.prefix_tables = prefix_tables;
+    a.group_plens = prefix_lens;
+    a.group_starts = group_starts;
+    a.scale_page_stride = scale_page_stride;
+    a.scale_head_stride = scale_head_stride;
+    a.scale_token_stride = scale_token_stride;
+    a.num_seqs = num_seqs;
+    a.total_q = num_seqs;
+    a.num_groups = num_groups;
+    a.max_pblocks = max_prefix_blocks;
+    a.num_q_heads = num_q_heads;
+    a.num_kv_heads = num_kv_heads;
+    a.head_dim = head_dim;
+    a.block_size = block_size;
+    a.max_blocks = max_blocks_per_seq;
+    a.num_blocks = num_blocks;
+    a.q_dtype = q_dtype;
+    a.kv_dtype = kv_dtype;
+    a.soft_cap = soft_cap > 0.f ? soft_cap : 0.f;
+    a.q_scale = a.soft_cap > 0.f ? scale : scale * kLog2e;
+    rc = check_attn(a);
+    if (rc) return rc;
+    (void)workspace;
+    (void)workspace_bytes;
+    return launch_generic(a, static_cast<cudaStream_t>(stream));
+}
+
+size_t gollek_paged_attention_shared_prefix_workspace_size(int num_groups, int num_seqs, int num_q_heads,
+                                                           int num_kv_heads, int head_dim) {
+    (void)num_groups, (void)num_seqs, (void)num_q_heads, (void)num_kv_heads, (void)head_dim;
+    return 0;
+}
+
+int gollek_kv_gather(void *key, void *value, int out_dtype, const int *token_seq, const int *token_pos,
+                     const int *block_tables, int num_seqs, int max_blocks_per_seq, int num_blocks,
+                     const void *k_cache, const void *v_cache, const float *k_scales, const float *v_scales,
+                     int kv_dtype, int num_tokens, int num_kv_heads, int head_dim, int block_size,
+                     long long page_stride, long long scale_page_stride, long long scale_head_stride,
+                     long long scale_token_stride, void *stream) {
+    t_last_error.clear();
+    GatherArgs a{};
+    int rc = check_pool(kv_dtype, k_scales, v_scales, num_kv_heads, head_dim, block_size, max_blocks_per_seq, num_blocks,
+                        page_stride, &a.page_stride);
+    if (rc) return rc;
+    if (!float_dtype(out_dtype)) return fail(GOLLEK_ERR_UNSUPPORTED, "output dtype %d (F32, BF16 or F16 only)", out_dtype);
+    if (num_tokens < 0 || num_seqs < 0) return fail(GOLLEK_ERR_INVALID_ARGUMENT, "negative size");
+    if (num_tokens == 0) return GOLLEK_OK;
+    if (!key || !value || !token_pos || !block_tables || !k_cache || !v_cache)
+        return fail(GOLLEK_ERR_INVALID_ARGUMENT, "null tensor pointer");
+    a.key = key;
+    a.value = value;
+    a.k = k_cache;
+    a.v = v_cache;
+    a.k_scales = quantised(kv_dtype) ? k_scales : nullptr;
+    a.v_scales = quantised(kv_dtype) ? v_scales : nullptr;
+    a.token_seq = token_seq;
+    a.token_pos = token_pos;
+    a.block_tables = block_tables;
+    a.scale_page_stride = scale_page_stride;
+    a.scale_head_stride = scale_head_stride;
+    a.scale_token_stride = scale_token_stride;
+    a.num_tokens = num_tokens;
+    a.num_seqs = num_seqs;
+    a.num_kv_heads = num_kv_heads;
+    a.head_dim = head_dim;
+    a.block_size = block_size;
+    a.max_blocks = max_blocks_per_seq;
+    a.num_blocks = num_blocks;
+    a.kv_dtype = kv_dtype;
+    a.out_dtype = out_dtype;
+    int dev = 0;
+    GK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
+    const long long total = static_cast<long long>(num_tokens) * num_kv_heads * head_dim;
+    const long long grid = std::min<long long>((total + 255) / 256, 32LL * std::max(1, sm_count(dev)));
+    kv_gather_generic_kernel<<<static_cast<unsigned>(grid), 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    GK_CUDA(cudaGetLastError(), "kv_gather_generic_kernel launch");
+    return GOLLEK_OK;
+}
+
+}  // extern "C"

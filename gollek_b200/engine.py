@@ -5,6 +5,7 @@ engine/generation/:
   kv/BlockManager.java                   -> BlockManager (slabs [maxBlocks][H][BS][D] in HBM)
   kv/KVCacheManager.KVCacheSession       -> KVCacheSession (one block table per layer)
   attention/PagedKvCacheIO.updateCache   -> update_cache (gollek_kv_append)
+  attention/PagedKvCacheIO (gather)      -> gather_cache (gollek_kv_gather)
   attention/PagedAttentionVectorAPI.compute -> paged_attention_compute (gollek_paged_attention_v2)
 
 FP32, INT8 and INT4 storage follow the reference bit for bit on the write side (per
@@ -199,6 +200,31 @@ def update_cache(key, value, session: KVCacheSession, layer_idx: int, start_pos:
                   value.reshape(seq_len, session.num_kv_heads, session.head_dim).contiguous(),
                   pos, table, bm.k_slab, bm.v_slab, block_size=session.tokens_per_block,
                   num_blocks=bm.max_blocks, token_seq=seq, **_kv_args(bm))
+
+
+def gather_cache(session: KVCacheSession, layer_idx: int, start_pos: int, seq_len: int, dtype=None,
+                 out=None):
+    """PagedKvCacheIO's gather (attention/PagedKvCacheIO.java): positions start_pos ..
+    start_pos+seq_len-1 of a layer, read back and dequantised: (key, value), each
+    [seq_len, num_kv_heads, head_dim] of `dtype` (default fp32), contiguous for a dense pass
+    or for storing a prompt outside the pool.  out: (key, value) tensors to fill."""
+    import torch
+
+    from . import ops
+    if start_pos < 0 or seq_len < 0:
+        raise ValueError("start_pos and seq_len must not be negative")
+    if start_pos + seq_len > len(session.block_tables[layer_idx]) * session.tokens_per_block:
+        raise IllegalStateError(f"Missing KV block for layer {layer_idx} token {start_pos + seq_len - 1}")
+    bm = session.block_manager
+    pos = torch.arange(start_pos, start_pos + seq_len, dtype=torch.int32, device=bm.k_slab.device)
+    key, value = out if out is not None else (None, None)
+    if dtype is None:
+        dtype = key.dtype if key is not None else torch.float32
+    return ops.kv_gather(bm.k_slab, bm.v_slab, pos, session.block_table_tensor(layer_idx),
+                         num_kv_heads=session.num_kv_heads, head_dim=session.head_dim,
+                         block_size=session.tokens_per_block, num_blocks=bm.max_blocks,
+                         token_seq=torch.zeros_like(pos), dtype=dtype, key=key, value=value,
+                         **_kv_args(bm))
 
 
 def paged_attention_compute(q, session: KVCacheSession, layer_idx: int, total_tokens: int,

@@ -131,6 +131,229 @@ def kv_append(key, value, token_pos, block_tables, k_cache, v_cache, *, block_si
     check(rc)
 
 
+def _check(name, t, shape=None, dtype=None, device=None, optional=False, packed=True):
+    """Shape, type, device and layout of one argument of the functions below."""
+    if t is None:
+        if optional:
+            return
+        raise ValueError(f"{name} is required")
+    if not t.is_cuda:
+        raise ValueError("gollek_b200 ops take CUDA tensors only (no CPU path)")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not {device}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
+    if shape is not None and (t.dim() != len(shape) or
+                              any(w is not None and w != n for w, n in zip(shape, t.shape))):
+        raise ValueError(f"{name} must have shape {tuple('*' if w is None else w for w in shape)}, "
+                         f"not {tuple(t.shape)}")
+    if packed and not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _behind(t):
+    """Elements from a tensor's first one to the end of its storage: what a base pointer with
+    strides of its own (one layer of a pool) may reach."""
+    return t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
+
+
+def _check_pool(k_cache, v_cache, k_scales, v_scales, scale_strides, num_kv_heads, head_dim,
+                block_size, num_blocks, page_stride, int4, device):
+    """A K/V pool: both caches of one type (int4: bytes) on `device`, reaching num_blocks
+    pages (scales too) when that is given.  With page_stride the tensors are base pointers
+    (one layer of a larger pool); without it they are whole and contiguous."""
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        _check(name, t, device=device, packed=not page_stride)
+        if int4:
+            if t.dtype not in (torch.uint8, torch.int8):
+                raise ValueError(f"an int4 {name} is a tensor of bytes, not {t.dtype}")
+        elif t.dtype not in _TORCH_DTYPE:
+            raise ValueError(f"unsupported KV dtype {t.dtype}")
+    if k_cache.dtype != v_cache.dtype:
+        raise ValueError("k_cache and v_cache have different types")
+    for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+        _check(name, t, dtype=torch.float32, device=device, optional=True, packed=False)
+    if num_blocks > 0 and num_kv_heads > 0 and block_size > 0 and head_dim > 0:
+        page = num_kv_heads * block_size * head_dim
+        need = (num_blocks - 1) * (page_stride or page) + page
+        for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+            if _behind(t) * (2 if int4 else 1) < need:
+                raise ValueError(f"{name} is smaller than {num_blocks} pages")
+        if int4 or k_cache.dtype == torch.int8:
+            sps, shs, sts = scale_strides
+            last = (num_blocks - 1) * sps + (num_kv_heads - 1) * shs + (block_size - 1) * sts
+            for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+                if t is not None and (min(sps, shs, sts) < 0 or _behind(t) <= last):
+                    raise ValueError(f"{name} is smaller than {num_blocks} pages of its strides")
+
+
+class _on:
+    """Runs a call on the device of its tensors and on `stream` (default: that device's
+    current stream); what is allocated inside belongs to that stream."""
+
+    def __init__(self, device, stream):
+        self.device, self.given = device, stream
+
+    def __enter__(self):
+        self.guard = None
+        if self.given is not None:
+            s = self.given
+            if not hasattr(s, "cuda_stream"):
+                s = torch.cuda.ExternalStream(int(s), device=self.device)
+            self.guard = torch.cuda.stream(s)
+        elif torch.cuda.current_device() != self.device.index:
+            self.guard = torch.cuda.device(self.device)
+        if self.guard is not None:
+            self.guard.__enter__()
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _scratch(need, workspace, device):
+    """The caller's workspace (checked), or a fresh one from torch's allocator: stream
+    ordered, and private to a captured graph."""
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    else:
+        _check("workspace", workspace, device=device)
+    return workspace, 0 if workspace is None else workspace.numel() * workspace.element_size()
+
+
+def varlen_workspace_size(num_seqs, total_queries, num_q_heads, num_kv_heads, head_dim) -> int:
+    return int(_lib.load().gollek_paged_attention_varlen_workspace_size(
+        num_seqs, total_queries, num_q_heads, num_kv_heads, head_dim))
+
+
+def paged_attention_varlen(q, k_cache, v_cache, block_tables, cu_seqlens_q, context_lens, *,
+                           num_kv_heads, block_size, scale=None, causal=True, num_blocks=0,
+                           page_stride=0, k_scales=None, v_scales=None, scale_strides=(0, 0, 0),
+                           soft_cap=0.0, sliding_window=0, alibi_slopes=None, prefix_lens=None,
+                           token_starts=None, int4=False, out=None, workspace=None, stream=None):
+    """Ragged attention (gollek_paged_attention_varlen): q [total, Hq, D] fp32/bf16/f16, the
+    queries of sequence s in rows cu_seqlens_q[s] .. cu_seqlens_q[s+1] - 1, the last of them
+    at position context_lens[s] - 1.
+
+    alibi_slopes [Hq] subtracts slope * |distance| from the scores; prefix_lens [S] makes each
+    sequence's first positions visible to all its queries; token_starts [total] is the first
+    position each query may attend.  Rows of `out` in no sequence are not written.
+    """
+    _check("q", q, (None, None, None))
+    dev = q.device
+    total, Hq, D = q.shape
+    if q.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"unsupported q dtype {q.dtype}")
+    _check("block_tables", block_tables, (None, None), torch.int32, dev)
+    S = block_tables.shape[0]
+    _check("cu_seqlens_q", cu_seqlens_q, (S + 1,), torch.int32, dev)
+    _check("context_lens", context_lens, (S,), torch.int32, dev)
+    _check("alibi_slopes", alibi_slopes, (Hq,), torch.float32, dev, optional=True)
+    _check("prefix_lens", prefix_lens, (S,), torch.int32, dev, optional=True)
+    _check("token_starts", token_starts, (total,), torch.int32, dev, optional=True)
+    _check("out", out, tuple(q.shape), q.dtype, dev, optional=True)
+    _check_pool(k_cache, v_cache, k_scales, v_scales, scale_strides, int(num_kv_heads), D,
+                int(block_size), int(num_blocks), int(page_stride), int4, dev)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    sps, shs, sts = scale_strides
+    lib = _lib.load()
+    with _on(dev, stream) as st:
+        if out is None:
+            out = torch.empty_like(q)
+        ws, nbytes = _scratch(0 if workspace is not None else varlen_workspace_size(
+            S, total, Hq, int(num_kv_heads), D), workspace, dev)
+        check(lib.gollek_paged_attention_varlen(
+            _ptr(out), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales), _ptr(v_scales),
+            _ptr(block_tables), _ptr(cu_seqlens_q), _ptr(context_lens), _ptr(alibi_slopes),
+            _ptr(prefix_lens), _ptr(token_starts), S, total, Hq, int(num_kv_heads), D,
+            int(block_size), block_tables.shape[1], int(num_blocks), int(page_stride),
+            _TORCH_DTYPE[q.dtype], kv_dtype_code(k_cache, int4), int(sps), int(shs), int(sts),
+            float(scale), float(soft_cap), int(sliding_window), int(bool(causal)), _ptr(ws),
+            nbytes, st))
+    return out
+
+
+def shared_prefix_workspace_size(num_groups, num_seqs, num_q_heads, num_kv_heads, head_dim) -> int:
+    return int(_lib.load().gollek_paged_attention_shared_prefix_workspace_size(
+        num_groups, num_seqs, num_q_heads, num_kv_heads, head_dim))
+
+
+def paged_attention_shared_prefix(q, k_cache, v_cache, prefix_tables, prefix_lens, group_starts,
+                                  block_tables, context_lens, *, num_kv_heads, block_size,
+                                  scale=None, num_blocks=0, page_stride=0, k_scales=None,
+                                  v_scales=None, scale_strides=(0, 0, 0), soft_cap=0.0, int4=False,
+                                  out=None, workspace=None, stream=None):
+    """Decode attention of groups that share prefixes (gollek_paged_attention_shared_prefix):
+    q [S, Hq, D] fp32/bf16/f16; sequences group_starts[g] .. group_starts[g+1] - 1 attend the
+    prefix_lens[g] tokens of prefix_tables[g], read once for the group, and then their own
+    context_lens[s] tokens."""
+    _check("q", q, (None, None, None))
+    dev = q.device
+    S, Hq, D = q.shape
+    if q.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"unsupported q dtype {q.dtype}")
+    _check("prefix_tables", prefix_tables, (None, None), torch.int32, dev)
+    groups = prefix_tables.shape[0]
+    _check("prefix_lens", prefix_lens, (groups,), torch.int32, dev)
+    _check("group_starts", group_starts, (groups + 1,), torch.int32, dev)
+    _check("block_tables", block_tables, (S, None), torch.int32, dev)
+    _check("context_lens", context_lens, (S,), torch.int32, dev)
+    _check("out", out, tuple(q.shape), q.dtype, dev, optional=True)
+    _check_pool(k_cache, v_cache, k_scales, v_scales, scale_strides, int(num_kv_heads), D,
+                int(block_size), int(num_blocks), int(page_stride), int4, dev)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    sps, shs, sts = scale_strides
+    lib = _lib.load()
+    with _on(dev, stream) as st:
+        if out is None:
+            out = torch.empty_like(q)
+        ws, nbytes = _scratch(0 if workspace is not None else shared_prefix_workspace_size(
+            groups, S, Hq, int(num_kv_heads), D), workspace, dev)
+        check(lib.gollek_paged_attention_shared_prefix(
+            _ptr(out), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales), _ptr(v_scales),
+            _ptr(prefix_tables), _ptr(prefix_lens), _ptr(group_starts), _ptr(block_tables),
+            _ptr(context_lens), groups, prefix_tables.shape[1], S, Hq, int(num_kv_heads), D,
+            int(block_size), block_tables.shape[1], int(num_blocks), int(page_stride),
+            _TORCH_DTYPE[q.dtype], kv_dtype_code(k_cache, int4), int(sps), int(shs), int(sts),
+            float(scale), float(soft_cap), _ptr(ws), nbytes, st))
+    return out
+
+
+def kv_gather(k_cache, v_cache, token_pos, block_tables, *, num_kv_heads, head_dim, block_size,
+              num_blocks=0, token_seq=None, page_stride=0, k_scales=None, v_scales=None,
+              scale_strides=(0, 0, 0), int4=False, dtype=torch.float32, key=None, value=None,
+              stream=None):
+    """Read rows of the cache back (gollek_kv_gather): (key, value), each [T, Hkv, head_dim] of
+    `dtype` (fp32/bf16/f16), dequantised; row i is position token_pos[i] of sequence
+    token_seq[i] (default: i)."""
+    _check("token_pos", token_pos, (None,), torch.int32)
+    dev = token_pos.device
+    T = token_pos.shape[0]
+    _check("token_seq", token_seq, (T,), torch.int32, dev, optional=True)
+    _check("block_tables", block_tables, (None, None), torch.int32, dev)
+    if dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"unsupported output dtype {dtype}")
+    shape = (T, int(num_kv_heads), int(head_dim))
+    _check("key", key, shape, dtype, dev, optional=True)
+    _check("value", value, shape, dtype, dev, optional=True)
+    _check_pool(k_cache, v_cache, k_scales, v_scales, scale_strides, int(num_kv_heads),
+                int(head_dim), int(block_size), int(num_blocks), int(page_stride), int4, dev)
+    sps, shs, sts = scale_strides
+    with _on(dev, stream) as st:
+        key = torch.empty(shape, dtype=dtype, device=dev) if key is None else key
+        value = torch.empty(shape, dtype=dtype, device=dev) if value is None else value
+        check(_lib.load().gollek_kv_gather(
+            _ptr(key), _ptr(value), _TORCH_DTYPE[dtype], _ptr(token_seq), _ptr(token_pos),
+            _ptr(block_tables), block_tables.shape[0], block_tables.shape[1], int(num_blocks),
+            _ptr(k_cache), _ptr(v_cache), _ptr(k_scales), _ptr(v_scales),
+            kv_dtype_code(k_cache, int4), T, int(num_kv_heads), int(head_dim), int(block_size),
+            int(page_stride), int(sps), int(shs), int(sts), st))
+    return key, value
+
+
 def pool_blocks(pool, block_stride, bytes_per_block) -> int:
     """Whole blocks of `bytes_per_block` bytes, `block_stride` bytes apart, that fit in
     the tensor `pool` (the bound the migration and checksum kernels check ids against)."""

@@ -218,6 +218,88 @@ GOLLEK_API int gollek_paged_attention_v2_noalloc(
     int sliding_window, void *stream);
 
 /* ======================================================================== *
+ * Ragged and shared-prefix attention
+ * ======================================================================== */
+
+/*
+ * Attention of ragged new tokens over the paged pool: continuous batching (prompt chunks of
+ * any length beside decode steps) with score bias and masks.  Extends
+ * PagedAttentionVectorAPI.compute (ST/generation/attention/PagedAttentionVectorAPI.java:60-180),
+ * whose queries are a rectangle with one causal or windowed mask.
+ *
+ *   q, out        [total_queries, num_q_heads, head_dim] of q_dtype (F32, BF16 or F16).
+ *   cu_seqlens_q  [num_seqs + 1] non-decreasing: the queries of sequence s are rows
+ *                 cu[s] .. cu[s+1] - 1 (none: allowed).  Rows of `out` in no sequence are
+ *                 left as they were.
+ *   context_lens  [num_seqs] tokens of each sequence, its n = cu[s+1] - cu[s] new ones
+ *                 included: query i sits at position pos = context_lens[s] - n + i.
+ *   A query attends the positions lo <= j < hi of its sequence,
+ *       hi = causal ? max(pos + 1, min(prefix_lens[s], len)) : len
+ *       lo = max(0, pos - sliding_window + 1 if sliding_window > 0, token_starts[row])
+ *   with the score soft_cap*tanh(scale*q.k/soft_cap) (soft_cap <= 0: scale*q.k) minus
+ *   alibi_slopes[q head] * |pos - j|.  A row with nothing to attend gets zeros.
+ *   alibi_slopes  [num_q_heads] fp32, or NULL (no bias).
+ *   prefix_lens   [num_seqs] or NULL: positions before it are visible to every query of
+ *                 the sequence (prefix mask).
+ *   token_starts  [total_queries] or NULL: first position a query may attend (packed
+ *                 documents: the first position of the query's own document).
+ *   sliding_window > 0 needs causal (GOLLEK_ERR_UNSUPPORTED otherwise).
+ *   workspace     >= gollek_paged_attention_varlen_workspace_size(...) bytes, its contents
+ *                 do not matter; not shared by calls that may overlap on the device (two
+ *                 streams, two captured graphs).  NULL = library-owned scratch per (device,
+ *                 stream), which such calls and graphs would share: pass a workspace there.
+ * Pool, scales, tables and num_blocks as in gollek_paged_attention_v2; any head_dim up to
+ * 256, any GQA group.  K and V at positions that no query attends may hold anything; a NaN
+ * or infinity at a position that some query of a sequence attends may also reach outputs of
+ * that sequence's other queries.  Asynchronous on `stream`.  Scores, softmax statistics and
+ * sums are fp32.
+ */
+GOLLEK_API int gollek_paged_attention_varlen(
+    void *out, const void *q, const void *k_cache, const void *v_cache, const float *k_scales,
+    const float *v_scales, const int *block_tables, const int *cu_seqlens_q, const int *context_lens,
+    const float *alibi_slopes, const int *prefix_lens, const int *token_starts, int num_seqs,
+    int total_queries, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+    int max_blocks_per_seq, int num_blocks, long long page_stride, int q_dtype, int kv_dtype,
+    long long scale_page_stride, long long scale_head_stride, long long scale_token_stride,
+    float scale, float soft_cap, int sliding_window, int causal, void *workspace,
+    size_t workspace_bytes, void *stream);
+
+/* Bytes of scratch gollek_paged_attention_varlen needs for these sizes. */
+GOLLEK_API size_t gollek_paged_attention_varlen_workspace_size(int num_seqs, int total_queries,
+                                                    int num_q_heads, int num_kv_heads, int head_dim);
+
+/*
+ * Decode attention of a batch whose sequences share prefixes: sequences group_starts[g] ..
+ * group_starts[g+1] - 1 all attend the prefix_lens[g] tokens of group g's table and then
+ * their own context_lens[s] tokens, one softmax over both; the prefix is read once for the
+ * group.  The pages of a prefix are those that the prompt cache shares between requests
+ * (optimization/gollek-plugin-prompt-cache/src/main/java/tech/kayys/gollek/cache/PagedKVCacheManagerExtension.java:45-180).
+ *
+ *   q, out         [num_seqs, num_q_heads, head_dim] of q_dtype (F32, BF16 or F16).
+ *   prefix_tables  [num_groups, max_prefix_blocks], prefix_lens [num_groups] (0: allowed;
+ *                  need not end on a page).
+ *   group_starts   [num_groups + 1] non-decreasing; sequences before the first or behind
+ *                  the last have no prefix.
+ *   block_tables   [num_seqs, max_blocks_per_seq], context_lens [num_seqs]: each sequence's
+ *                  own tokens, the new one included (0: allowed, the prefix alone; with no
+ *                  prefix either the row is zeros).
+ * Everything else as gollek_paged_attention_varlen.
+ */
+GOLLEK_API int gollek_paged_attention_shared_prefix(
+    void *out, const void *q, const void *k_cache, const void *v_cache, const float *k_scales,
+    const float *v_scales, const int *prefix_tables, const int *prefix_lens, const int *group_starts,
+    const int *block_tables, const int *context_lens, int num_groups, int max_prefix_blocks,
+    int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int block_size,
+    int max_blocks_per_seq, int num_blocks, long long page_stride, int q_dtype, int kv_dtype,
+    long long scale_page_stride, long long scale_head_stride, long long scale_token_stride,
+    float scale, float soft_cap, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Bytes of scratch gollek_paged_attention_shared_prefix needs for these sizes. */
+GOLLEK_API size_t gollek_paged_attention_shared_prefix_workspace_size(int num_groups, int num_seqs,
+                                                           int num_q_heads, int num_kv_heads,
+                                                           int head_dim);
+
+/* ======================================================================== *
  * KV append (the write path)
  * ======================================================================== */
 
@@ -248,6 +330,29 @@ GOLLEK_API int gollek_kv_append(const void *key, const void *value, int src_dtyp
                      int head_dim, int block_size, long long page_stride,
                      long long scale_page_stride, long long scale_head_stride,
                      long long scale_token_stride, void *stream);
+
+/*
+ * Reads rows of the cache back: the inverse of gollek_kv_append.  Replaces
+ * PagedKvCacheIO's gather (ST/generation/attention/PagedKvCacheIO.java), which packs a
+ * sequence's paged rows for a dense pass, with the dequantisation of
+ * PagedKvCacheQuantization (ST/generation/attention/PagedKvCacheQuantization.java).
+ *
+ *   key, value [num_tokens, num_kv_heads, head_dim] of out_dtype (F32, BF16 or F16).  Row i
+ *   is position token_pos[i] of sequence token_seq[i] (token_seq NULL: sequence i); the
+ *   same row may be asked for any number of times, in any order.  Values of quantised
+ *   pools are multiplied by their scale in fp32 (either scale granularity) and rounded
+ *   once to out_dtype.  A row whose sequence, position or page is out of range is set to
+ *   zeros and raises GOLLEK_STATUS_BAD_POSITION or GOLLEK_STATUS_BAD_BLOCK_ID.
+ * Pool layout, scale strides and num_blocks as in gollek_paged_attention_v2; num_seqs is the
+ * number of rows of block_tables.  Asynchronous on `stream`.
+ */
+GOLLEK_API int gollek_kv_gather(void *key, void *value, int out_dtype, const int *token_seq,
+                     const int *token_pos, const int *block_tables, int num_seqs,
+                     int max_blocks_per_seq, int num_blocks, const void *k_cache,
+                     const void *v_cache, const float *k_scales, const float *v_scales,
+                     int kv_dtype, int num_tokens, int num_kv_heads, int head_dim,
+                     int block_size, long long page_stride, long long scale_page_stride,
+                     long long scale_head_stride, long long scale_token_stride, void *stream);
 
 /* ======================================================================== *
  * KV block migration (prefill -> decode)
