@@ -77,6 +77,29 @@ int launch_generic(AttnArgs &a, cudaStream_t st) {
     return GOLLEK_OK;
 }
 
+template <int KV>
+const void *gather_fn(int out) {
+    if (out == GOLLEK_DTYPE_F32) return reinterpret_cast<const void *>(&kv_gather_kernel<KV, float>);
+    if (out == GOLLEK_DTYPE_BF16) return reinterpret_cast<const void *>(&kv_gather_kernel<KV, __nv_bfloat16>);
+    return reinterpret_cast<const void *>(&kv_gather_kernel<KV, __half>);
+}
+
+// Whether every row is whole 8-element chunks at addresses that the vector loads and stores
+// of kv_gather_kernel may use; its kernel, or null.
+const void *gather_vectors(const GatherArgs &a) {
+    if (a.head_dim % 8 || a.page_stride % 8 || !aligned16(a.key) || !aligned16(a.value)) return nullptr;
+    if (static_cast<long long>(a.num_kv_heads) * a.head_dim > (1 << 20)) return nullptr;  // 32-bit chunk indexes
+    const uintptr_t mask = a.kv_dtype == GOLLEK_DTYPE_I8 ? 7 : a.kv_dtype == GOLLEK_DTYPE_I4 ? 3 : 15;
+    if ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) & mask) return nullptr;
+    switch (a.kv_dtype) {
+        case GOLLEK_DTYPE_F32: return gather_fn<GOLLEK_DTYPE_F32>(a.out_dtype);
+        case GOLLEK_DTYPE_BF16: return gather_fn<GOLLEK_DTYPE_BF16>(a.out_dtype);
+        case GOLLEK_DTYPE_F16: return gather_fn<GOLLEK_DTYPE_F16>(a.out_dtype);
+        case GOLLEK_DTYPE_I8: return gather_fn<GOLLEK_DTYPE_I8>(a.out_dtype);
+        default: return gather_fn<GOLLEK_DTYPE_I4>(a.out_dtype);
+    }
+}
+
 }  // namespace
 }  // namespace gk
 
@@ -248,8 +271,21 @@ int gollek_kv_gather(void *key, void *value, int out_dtype, const int *token_seq
     a.out_dtype = out_dtype;
     int dev = 0;
     GK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
+    const int sms = std::max(1, sm_count(dev));
+    if (const void *fn = gather_vectors(a)) {
+        // About 2048 chunks per block (8 a thread), fewer where that leaves fewer than four
+        // blocks per SM.
+        const int cpt = num_kv_heads * head_dim / 8;
+        int tpb = std::min(std::max(2048 / cpt, 1), kGatherTokens);
+        tpb = std::min(tpb, std::max(1, num_tokens / (4 * sms)));
+        void *args[] = {&a, &tpb};
+        GK_CUDA(cudaLaunchKernel(fn, dim3((num_tokens + tpb - 1) / tpb), dim3(kGatherThreads), args, 0,
+                                 static_cast<cudaStream_t>(stream)),
+                "kv_gather_kernel launch");
+        return GOLLEK_OK;
+    }
     const long long total = static_cast<long long>(num_tokens) * num_kv_heads * head_dim;
-    const long long grid = std::min<long long>((total + 255) / 256, 32LL * std::max(1, sm_count(dev)));
+    const long long grid = std::min<long long>((total + 255) / 256, 32LL * sms);
     kv_gather_generic_kernel<<<static_cast<unsigned>(grid), 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
     GK_CUDA(cudaGetLastError(), "kv_gather_generic_kernel launch");
     return GOLLEK_OK;
