@@ -2,6 +2,7 @@
 // cache read-back: argument checks, kernel selection and their C ABI (gollek_kernels.h).
 #include <algorithm>
 
+#include "attn_tile.cuh"
 #include "host.cuh"
 #include "kv_gather.cuh"
 #include "varlen.cuh"
@@ -75,6 +76,131 @@ int launch_generic(AttnArgs &a, cudaStream_t st) {
     GK_CUDA(cudaLaunchKernel(fn, dim3(a.total_q, a.num_kv_heads, (G + GC - 1) / GC), dim3(kAgWarps * 32), args, 0, st),
             "attn_generic_kernel launch");
     return GOLLEK_OK;
+}
+
+// Whether the tile kernel takes the call: 16-bit pool and q of one type, head_dim 64 or 128,
+// pages of 8 or a multiple of 16 tokens in whole 8-row groups, 16-byte aligned tensors.
+bool tile_takes(const AttnArgs &a) {
+    if (a.q_dtype != a.kv_dtype || (a.kv_dtype != GOLLEK_DTYPE_BF16 && a.kv_dtype != GOLLEK_DTYPE_F16)) return false;
+    if (a.head_dim != 64 && a.head_dim != 128) return false;
+    if (a.block_size != 8 && a.block_size % 16 != 0) return false;
+    if (a.page_stride % (8 * a.head_dim) != 0) return false;
+    if (!aligned16(a.k) || !aligned16(a.v) || !aligned16(a.q) || !aligned16(a.out)) return false;
+    const long long page_rows = a.page_stride / a.head_dim;
+    return a.num_blocks == 0 || a.num_blocks * page_rows < (1LL << 31);
+}
+
+long long tile_entities(int num_groups, int num_seqs) { return static_cast<long long>(num_groups) + num_seqs; }
+
+// Rows of all entities: each query token's heads of one group; shared: twice (prefix, own).
+long long tile_rows(int total_q, int G, bool shared) { return static_cast<long long>(total_q) * G * (shared ? 2 : 1); }
+
+// 4-D map over a pool of 16-bit rows: (64 columns, 8 rows, column slabs, 8-row blocks), so a
+// box of (64, 8, slabs, box_rows / 8) lands in the layout of kv_chunk_off.
+int encode_tile_map(CUtensorMap *m, const void *base, int kv_dtype, int D, long long rows, int box_rows) {
+    auto enc = encode_fn();
+    if (!enc) return fail(GOLLEK_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled unavailable");
+    const cuuint32_t slabs = D / 64;
+    const cuuint64_t pitch = static_cast<cuuint64_t>(D) * 2;
+    cuuint64_t dims[4] = {64, 8, slabs, static_cast<cuuint64_t>(rows / 8)};
+    cuuint64_t strides[3] = {pitch, 128, 8 * pitch};
+    cuuint32_t box[4] = {64, 8, slabs, static_cast<cuuint32_t>(box_rows / 8)};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = enc(m, kv_dtype == GOLLEK_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                     const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(GOLLEK_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return GOLLEK_OK;
+}
+
+// A launch that may begin before the kernel in front of it has ended (that kernel's results are
+// read behind griddepcontrol.wait).
+int launch_dependent(const void *fn, dim3 grid, int threads, size_t smem, cudaStream_t st, void **args, const char *what) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    GK_CUDA(cudaLaunchKernelExC(&cfg, fn, args), what);
+    return GOLLEK_OK;
+}
+
+template <typename T, int D>
+int launch_tile_as(TileArgs &p, const CUtensorMap &tmk, const CUtensorMap &tmv, cudaStream_t st) {
+    const AttnArgs &a = p.a;
+    const void *fn = reinterpret_cast<const void *>(&attn_tile_kernel<T, D>);
+    GK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, TileSmem<D>::total), "cudaFuncSetAttribute");
+    tile_plan_kernel<<<1, kPlanThreads, 0, st>>>(p);
+    GK_CUDA(cudaGetLastError(), "tile_plan_kernel launch");
+    void *args[] = {const_cast<CUtensorMap *>(&tmk), const_cast<CUtensorMap *>(&tmv), &p};
+    int rc = launch_dependent(fn, dim3(p.grid), kTileThreads, TileSmem<D>::total, st, args, "attn_tile_kernel launch");
+    if (rc) return rc;
+    void *margs[] = {&p};
+    if (a.num_groups == 0)
+        return launch_dependent(reinterpret_cast<const void *>(&tile_merge_kernel<T, D>), dim3(p.grid, kMergeSplit),
+                                kMergeThreads, 0, st, margs, "tile_merge_kernel launch");
+    const long long rows = static_cast<long long>(a.num_seqs) * a.num_q_heads;
+    return launch_dependent(reinterpret_cast<const void *>(&tile_merge_shared_kernel<T, D>),
+                            dim3(static_cast<unsigned>((rows + kMergeThreads / 32 - 1) / (kMergeThreads / 32))), kMergeThreads,
+                            0, st, margs, "tile_merge_shared_kernel launch");
+}
+
+int launch_tile(AttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
+    const bool shared = a.num_groups > 0;
+    const int G = a.num_q_heads / a.num_kv_heads;
+    TileArgs p{};
+    p.entities = a.num_groups + a.num_seqs;
+    const TileWs w = tile_ws(tile_entities(a.num_groups, a.num_seqs), tile_rows(a.total_q, G, shared),
+                             static_cast<long long>(a.total_q) * a.num_q_heads, a.head_dim, shared);
+    if (w.max_blocks > (1LL << 30)) return fail(GOLLEK_ERR_UNSUPPORTED, "too many query rows for one call");
+    int dev = 0;
+    GK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
+    if (!ws) {
+        int rc = library_workspace(dev, stream, w.total, &ws, &ws_bytes);
+        if (rc) return rc;
+    }
+    if (ws_bytes < w.total)
+        return fail(GOLLEK_ERR_WORKSPACE, "workspace of %zu bytes < %zu needed", ws_bytes, w.total);
+    if (reinterpret_cast<uintptr_t>(ws) & 255) return fail(GOLLEK_ERR_INVALID_ARGUMENT, "workspace not 256-byte aligned");
+    uint8_t *base = static_cast<uint8_t *>(ws);
+    p.a = a;
+    p.head = reinterpret_cast<PlanHead *>(base);
+    p.blks = reinterpret_cast<TileBlk *>(base + w.blks);
+    p.cost = reinterpret_cast<long long *>(base + w.cost);
+    p.ents = reinterpret_cast<int *>(base + w.ents);
+    p.slots = reinterpret_cast<float *>(base + w.slots);
+    p.ml = reinterpret_cast<float2 *>(base + w.ml);
+    p.acc = reinterpret_cast<float *>(base + w.acc);
+    p.max_blocks = static_cast<int>(w.max_blocks);
+    p.page_rows = a.page_stride / a.head_dim;
+    p.grid = std::min(std::max(1, sm_count(dev)), kMaxTileCtas);
+    const long long rows = a.num_blocks > 0 ? a.num_blocks * p.page_rows : (1LL << 31) - 8;
+    const int box = std::min(a.block_size, 16);
+    CUtensorMap tmk, tmv;
+    int rc = encode_tile_map(&tmk, a.k, a.kv_dtype, a.head_dim, rows, box);
+    if (!rc) rc = encode_tile_map(&tmv, a.v, a.kv_dtype, a.head_dim, rows, box);
+    if (rc) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool bf16 = a.kv_dtype == GOLLEK_DTYPE_BF16;
+    if (a.head_dim == 128)
+        return bf16 ? launch_tile_as<__nv_bfloat16, 128>(p, tmk, tmv, st) : launch_tile_as<__half, 128>(p, tmk, tmv, st);
+    return bf16 ? launch_tile_as<__nv_bfloat16, 64>(p, tmk, tmv, st) : launch_tile_as<__half, 64>(p, tmk, tmv, st);
+}
+
+int launch_attn(AttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
+    if (tile_takes(a)) return launch_tile(a, ws, ws_bytes, stream);
+    return launch_generic(a, static_cast<cudaStream_t>(stream));
+}
+
+size_t attn_workspace(int num_groups, int num_seqs, int total_q, int hq, int hkv, int D) {
+    if (num_seqs <= 0 || total_q <= 0 || num_groups < 0 || hkv <= 0 || hq <= 0 || hq % hkv || D <= 0) return 0;
+    return tile_ws(tile_entities(num_groups, num_seqs), tile_rows(total_q, hq / hkv, num_groups > 0),
+                   static_cast<long long>(total_q) * hq, D, num_groups > 0).total;
 }
 
 template <int KV>
@@ -159,15 +285,12 @@ int gollek_paged_attention_varlen(void *out, const void *q, const void *k_cache,
     a.q_scale = a.soft_cap > 0.f ? scale : scale * kLog2e;
     rc = check_attn(a);
     if (rc) return rc;
-    (void)workspace;
-    (void)workspace_bytes;
-    return launch_generic(a, static_cast<cudaStream_t>(stream));
+    return launch_attn(a, workspace, workspace_bytes, stream);
 }
 
 size_t gollek_paged_attention_varlen_workspace_size(int num_seqs, int total_queries, int num_q_heads, int num_kv_heads,
                                                     int head_dim) {
-    (void)num_seqs, (void)total_queries, (void)num_q_heads, (void)num_kv_heads, (void)head_dim;
-    return 0;
+    return attn_workspace(0, num_seqs, total_queries, num_q_heads, num_kv_heads, head_dim);
 }
 
 int gollek_paged_attention_shared_prefix(void *out, const void *q, const void *k_cache, const void *v_cache,
@@ -221,15 +344,12 @@ int gollek_paged_attention_shared_prefix(void *out, const void *q, const void *k
     a.q_scale = a.soft_cap > 0.f ? scale : scale * kLog2e;
     rc = check_attn(a);
     if (rc) return rc;
-    (void)workspace;
-    (void)workspace_bytes;
-    return launch_generic(a, static_cast<cudaStream_t>(stream));
+    return launch_attn(a, workspace, workspace_bytes, stream);
 }
 
 size_t gollek_paged_attention_shared_prefix_workspace_size(int num_groups, int num_seqs, int num_q_heads,
                                                            int num_kv_heads, int head_dim) {
-    (void)num_groups, (void)num_seqs, (void)num_q_heads, (void)num_kv_heads, (void)head_dim;
-    return 0;
+    return num_groups <= 0 ? 0 : attn_workspace(num_groups, num_seqs, num_seqs, num_q_heads, num_kv_heads, head_dim);
 }
 
 int gollek_kv_gather(void *key, void *value, int out_dtype, const int *token_seq, const int *token_pos,
