@@ -354,12 +354,31 @@ struct TileSmem {
     static constexpr uint32_t total = misc + 16;
 };
 
+// Bounded wait of a whole warp: each lane tests on its own, one vote at the end (the
+// result is warp-uniform); gives up once another warp did.
+__device__ __forceinline__ bool tile_wait(uint64_t *bar, uint32_t parity, volatile int *abort) {
+    bool ok = mbar_try_wait(bar, parity);
+    for (unsigned i = 0; !ok && i < kSuspendTries; ++i) {
+        if (*abort) break;
+        ok = mbar_try_wait_suspend(bar, parity, kSuspendNs);
+        if (!ok && i + 1 == kSuspendTries) raise_status(GOLLEK_STATUS_TIMEOUT);
+    }
+    return __all_sync(0xffffffffu, ok);
+}
+
 // D[tmem] (+)= A[tmem] * B, issued by one thread.
 __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
         "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc));
+}
+
+// One lane of the converged warp, always the same.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
 }
 
 // Byte offset of 16-byte chunk ch (elements 8 ch ..) of token tok in a K or V tile: 8-token
@@ -373,8 +392,13 @@ __device__ __forceinline__ uint32_t kv_chunk_off(int tok, int ch) {
 // Page lookups and TMA boxes of a run's tiles: lane g < 8 owns the 16 positions 16 g .. of
 // each tile (one box; two of 8 rows where pages hold 8).
 struct PageLoc {
-    int row[2];   // first pool row of the box / 8, or -1
+    int row0, row1;  // first pool row of the box / 8, or -1
 };
+
+// Ring positions, from the run's first, of K and V of tile j of n: a value product follows
+// the scores of the next tile, so V is copied behind the next K and waits less for its use.
+__device__ __forceinline__ int k_at(int j) { return j == 0 ? 0 : 2 * j - 1; }
+__device__ __forceinline__ int v_at(int j, int n) { return j == n - 1 ? 2 * n - 1 : 2 * j + 2; }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kTileThreads, 1)
@@ -440,54 +464,71 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         TileRun r;
         if (warp == 9) {
             // ===================================================================== producer
-            int c = 0;  // ring position: K and V of tile j at 2 j, 2 j + 1
-            bool ok = true;
-            while (ok && it.next(p, r)) {
-                const int *bt = r.b.kind == kPrefix ? a.prefix_tables + static_cast<long long>(r.b.tab) * a.max_pblocks
-                                                    : a.block_tables + static_cast<long long>(r.b.tab) * a.max_blocks;
-                const int tile0 = r.b.lo / kTileTok;
-                const int R = a.block_size < 16 ? a.block_size : 16, per = 16 / R;
-                // pool rows of the lane's box(es) in tile t, -1: nothing to load there
-                auto locate = [&](int t) {
-                    PageLoc l{{-1, -1}};
-                    if (t >= r.tb || lane >= 8) return l;
-                    for (int j = 0; j < per; ++j) {
-                        const int pos = (tile0 + t) * kTileTok + lane * 16 + j * R;
-                        if (pos >= r.b.hi || pos + R <= r.b.lo) continue;
-                        const int pg = pos / a.block_size;
-                        int e = __ldg(bt + pg);
-                        if (e < 0 || (a.num_blocks > 0 && e >= a.num_blocks)) {
-                            raise_status(GOLLEK_STATUS_BAD_BLOCK_ID);
-                            e = 0;
-                        }
-                        l.row[j] = static_cast<int>((e * p.page_rows + static_cast<long long>(r.h) * a.block_size +
-                                                     (pos - pg * a.block_size)) >> 3);
-                    }
-                    return l;
-                };
-                PageLoc cur = locate(r.ta), nxt = locate(r.ta + 1);
-                for (int t = r.ta; t < r.tb && ok; ++t) {
-                    const PageLoc ahead = locate(t + 2);
-                    const int boxes = (cur.row[0] >= 0) + (cur.row[1] >= 0);
-                    const uint32_t bytes = __reduce_add_sync(0xffffffffu, static_cast<unsigned>(boxes)) * R * D * 2;
-                    for (int kv = 0; kv < 2; ++kv, ++c) {
-                        const int slot = c % NS;
-                        if (c >= NS) {
-                            if (lane == 0)
-                                ok = mbar_wait_or_abort(&empty[slot], (c / NS - 1) & 1, abort, kSuspendTries, kSuspendNs);
-                            ok = __shfl_sync(0xffffffffu, ok, 0);
-                            if (!ok) break;
-                        }
-                        if (lane == 0) mbar_arrive_expect_tx(&full[slot], bytes);
-                        __syncwarp();
-                        uint8_t *dst = ring + slot * L::kSlot + lane * (16 * D * 2);
-                        for (int j = 0; j < per; ++j)
-                            if (cur.row[j] >= 0)
-                                tma_load_4d(dst + j * R * D * 2, kv ? &tm_v : &tm_k, 0, 0, 0, cur.row[j], &full[slot]);
-                    }
-                    cur = nxt;
-                    nxt = ahead;
+            // Tiles of all runs in one line, the page lookups two tiles ahead of the copies (so a run's
+            // first pages are known before the last ones of the run in front have a slot).
+            struct Step {
+                PageLoc loc;
+                bool live, first, last;
+            };
+            const int R = a.block_size < 16 ? a.block_size : 16, per = 16 / R;
+            const int *bt = nullptr;
+            int t = 0, tb = 0, ta = 0;
+            auto step = [&]() {
+                Step s{{-1, -1}, false, false, false};
+                if (t >= tb) {
+                    if (!it.next(p, r)) return s;
+                    bt = r.b.kind == kPrefix ? a.prefix_tables + static_cast<long long>(r.b.tab) * a.max_pblocks
+                                             : a.block_tables + static_cast<long long>(r.b.tab) * a.max_blocks;
+                    t = ta = r.ta;
+                    tb = r.tb;
                 }
+                s.live = true;
+                s.first = t == ta;
+                s.last = t == tb - 1;
+                // pool rows / 8 of the lane's box(es); -1: nothing to load there
+                const int pos = (r.b.lo / kTileTok + t) * kTileTok + lane * 16;
+                auto row8 = [&](int at) {
+                    if (lane >= 8 || at >= r.b.hi || at + R <= r.b.lo) return -1;
+                    const int pg = at / a.block_size;
+                    int e = __ldg(bt + pg);
+                    if (e < 0 || (a.num_blocks > 0 && e >= a.num_blocks)) {
+                        raise_status(GOLLEK_STATUS_BAD_BLOCK_ID);
+                        e = 0;
+                    }
+                    return static_cast<int>((e * p.page_rows + static_cast<long long>(r.h) * a.block_size +
+                                             (at - pg * a.block_size)) >> 3);
+                };
+                s.loc.row0 = row8(pos);
+                if (per == 2) s.loc.row1 = row8(pos + R);
+                ++t;
+                return s;
+            };
+            int c = 0;  // ring position
+            auto copy = [&](const PageLoc &l, const CUtensorMap *map) {
+                const int slot = c % NS;
+                if (c >= NS && !tile_wait(&empty[slot], (c / NS - 1) & 1, abort)) return false;
+                const unsigned boxes = (l.row0 >= 0) + (l.row1 >= 0);
+                const uint32_t bytes = __reduce_add_sync(0xffffffffu, boxes) * R * D * 2;
+                if (lane == 0) mbar_arrive_expect_tx(&full[slot], bytes);
+                __syncwarp();
+                uint8_t *dst = ring + slot * L::kSlot + lane * (16 * D * 2);
+                if (l.row0 >= 0) tma_load_4d(dst, map, 0, 0, 0, l.row0, &full[slot]);
+                if (l.row1 >= 0) tma_load_4d(dst + R * D * 2, map, 0, 0, 0, l.row1, &full[slot]);
+                ++c;
+                return true;
+            };
+            // ring order of a run: K0, K1, V0, K2, V1, ... V(n-1) (k_at, v_at)
+            bool ok = true;
+            Step s0 = step(), s1 = step();
+            PageLoc before{-1, -1};
+            while (ok && s0.live) {
+                const Step s2 = step();
+                ok = copy(s0.loc, &tm_k);
+                if (ok && !s0.first) ok = copy(before, &tm_v);
+                if (ok && s0.last) ok = copy(s0.loc, &tm_v);
+                before = s0.loc;
+                s0 = s1;
+                s1 = s2;
             }
             if (!ok && lane == 0) *abort = 1;
             // every copy issued lands before the shared memory is released
@@ -496,33 +537,46 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             __syncwarp();
         } else if (warp == 8) {
             // ===================================================================== MMA issuer
+            // The whole warp walks the tiles with warp-uniform values (so descriptors stay in uniform
+            // registers) and one elected lane issues: a lane that computed descriptors on its own took
+            // 2,300 cycles for the 16 MMAs of a step that run in about 1,000.
             constexpr uint32_t id_s = umma_idesc_16bit(128, kTileTok, kBf16, 0, 0);
             constexpr uint32_t id_o = umma_idesc_16bit(128, D, kBf16, 0, 1);
-            const uint32_t ring_s = smem_u32(ring);
+            const uint64_t q_desc = umma_desc_sw128(q_s, 16, 1024);
+            const uint64_t k_desc = umma_desc_sw128(smem_u32(ring), 16, 16 * D);
+            const uint64_t v_desc = umma_desc_sw128(smem_u32(ring), 1024, 16 * D);
+            const bool leader = elect_one();
             int c0 = 0;                   // ring position of the run's first K
-            int sp[2] = {0, 0};           // tiles given to group t so far
             int pp[2] = {0, 0};           // probabilities taken from group t so far
             int ou[2] = {0, 0};           // runs that used O of group t so far
             int qu[2] = {0, 0};           // fills of q buffer t consumed so far
             int qb = 1;                   // q buffer of the last small block; 1 after a large one
             bool ok = true;
-            auto wait = [&](uint64_t *bar, uint32_t par) { return mbar_wait_or_abort(bar, par, abort, kSuspendTries, kSuspendNs); };
+            auto wait = [&](uint64_t *bar, uint32_t par) { return tile_wait(bar, par, abort); };
+            auto commit = [&](uint64_t *bar) {
+                if (leader) umma_commit(bar);
+            };
             auto score = [&](int t, int buf, int c) {
-                const uint32_t kb = ring_s + (c % NS) * L::kSlot;
-                const uint32_t qa = q_s + buf * L::kQ;
+                const int slot = __shfl_sync(0xffffffffu, c % NS, 0);
+                const uint64_t qd = q_desc + buf * (L::kQ >> 4), kd = k_desc + slot * (L::kSlot >> 4);
+                const uint32_t d = tmem + 128 * t;
+                if (leader) {
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk)
-                    umma_f16(tmem + 128 * t, umma_desc_sw128(qa + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024),
-                             umma_desc_sw128(kb + (kk >> 2) * 1024 + (kk & 3) * 32, 16, 16 * D), id_s, kk > 0);
-                umma_commit(&s_full[t]);
-                ++sp[t];
+                    for (int kk = 0; kk < D / 16; ++kk)
+                        umma_f16(d, qd + (kk >> 2) * (16384 >> 4) + (kk & 3) * 2, kd + (kk >> 2) * (1024 >> 4) + (kk & 3) * 2,
+                                 id_s, kk > 0);
+                    umma_commit(&s_full[t]);
+                }
             };
             auto value = [&](int t, int c, bool first) {
-                const uint32_t vb = ring_s + (c % NS) * L::kSlot;
+                const int slot = __shfl_sync(0xffffffffu, c % NS, 0);
+                const uint64_t vd = v_desc + slot * (L::kSlot >> 4);
+                const uint32_t d = tmem + 256 + 128 * t, pa = tmem + 128 * t;
+                if (leader) {
 #pragma unroll
-                for (int kk = 0; kk < kTileTok / 16; ++kk)
-                    umma_f16_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * kk,
-                                umma_desc_sw128(vb + kk * (32 * D), 1024, 16 * D), id_o, !(first && kk == 0));
+                    for (int kk = 0; kk < kTileTok / 16; ++kk)
+                        umma_f16_ts(d, pa + 8 * kk, vd + kk * (32 * D >> 4), id_o, !(first && kk == 0));
+                }
                 ++pp[t];
             };
             // P of group t is there, V of ring position c is there, and (first use in a run) O is free
@@ -531,64 +585,71 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 if (w && first && ou[t] > 0) w = wait(&o_free[t], (ou[t] - 1) & 1);
                 return w;
             };
-            if (lane == 0) {
-                while (ok && it.next(p, r)) {
-                    const int n = r.tb - r.ta;
-                    if (r.b.nrows > 128) {
-                        // tile j: the values of j - 1 and the scores of j of each group in turn
-                        for (int t = 0; t < 2 && ok; ++t) ok = wait(&q_full[t], qu[t]++ & 1);
-                        for (int j = 0; ok && j <= n; ++j) {
-                            const int ck = c0 + 2 * j, cv = c0 + 2 * j - 1;
-                            if (j < n) ok = wait(&full[ck % NS], (ck / NS) & 1);
-                            for (int t = 0; ok && t < 2; ++t) {
-                                if (j > 0) {
-                                    ok = value_ready(t, cv, j == 1);
-                                    if (!ok) break;
-                                    tc_fence_after();
-                                    value(t, cv, j == 1);
-                                    if (j == n) umma_commit(&o_full[t]);
-                                }
-                                tc_fence_after();
-                                if (j < n) score(t, t, ck);
-                            }
+            while (ok && it.next(p, r)) {
+                const int n = r.tb - r.ta;
+                if (r.b.nrows > 128) {
+                    // tile j: the values of j - 1 and the scores of j of each group in turn
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) ok = ok && wait(&q_full[t], qu[t]++ & 1);
+                    for (int j = 0; ok && j <= n; ++j) {
+                        const int ck = c0 + k_at(j), cv = c0 + v_at(j - 1, n);
+                        if (j < n) ok = wait(&full[ck % NS], (ck / NS) & 1);
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
                             if (!ok) break;
-                            if (j > 0) umma_commit(&empty[cv % NS]);
-                            if (j < n) umma_commit(&empty[ck % NS]);
+                            if (j > 0) {
+                                ok = value_ready(t, cv, j == 1);
+                                if (!ok) break;
+                                tc_fence_after();
+                                value(t, cv, j == 1);
+                                if (j == n) commit(&o_full[t]);
+                            }
+                            tc_fence_after();
+                            if (j < n) score(t, t, ck);
                         }
-                        ++ou[0];
-                        ++ou[1];
-                        qb = 1;
-                    } else {
-                        // tile j belongs to group j & 1: its scores follow the values of j - 2
-                        qb ^= 1;
-                        ok = wait(&q_full[qb], qu[qb]++ & 1);
-                        for (int j = 0; ok && j < n + 2; ++j) {
-                            const int t = j & 1;
+                        if (!ok) break;
+                        if (j > 0) commit(&empty[cv % NS]);
+                        if (j < n) commit(&empty[ck % NS]);
+                    }
+                    ++ou[0];
+                    ++ou[1];
+                    qb = 1;
+                } else {
+                    // tile j belongs to group j & 1: its scores follow the values of j - 2
+                    qb ^= 1;
+                    ok = qb ? wait(&q_full[1], qu[1]++ & 1) : wait(&q_full[0], qu[0]++ & 1);
+                    for (int j0 = 0; ok && j0 < n + 2; j0 += 2) {
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            const int j = j0 + t;
+                            if (!ok) break;
                             if (j >= 2 && j - 2 < n) {
-                                const int cv = c0 + 2 * (j - 2) + 1;
+                                const int cv = c0 + v_at(j - 2, n);
                                 ok = value_ready(t, cv, j - 2 < 2);
                                 if (!ok) break;
                                 tc_fence_after();
                                 value(t, cv, j - 2 < 2);
-                                if (j >= n) umma_commit(&o_full[t]);
-                                umma_commit(&empty[cv % NS]);
+                                if (j >= n) commit(&o_full[t]);
+                                commit(&empty[cv % NS]);
                             }
                             if (j < n) {
-                                const int ck = c0 + 2 * j;
+                                const int ck = c0 + k_at(j);
                                 ok = wait(&full[ck % NS], (ck / NS) & 1);
                                 if (!ok) break;
                                 tc_fence_after();
                                 score(t, qb, ck);
-                                umma_commit(&empty[ck % NS]);
+                                commit(&empty[ck % NS]);
                             }
                         }
-                        ++ou[0];
-                        if (n > 1) ++ou[1];
                     }
-                    c0 += 2 * n;
+                    ++ou[0];
+                    if (n > 1) ++ou[1];
                 }
-                if (!ok) *abort = 1;
-                // every MMA issued has completed before tensor memory and shared memory go
+                c0 += 2 * n;
+            }
+            if (!ok && lane == 0) *abort = 1;
+            // every MMA issued has completed before tensor memory and shared memory go
+            if (leader) {
                 umma_commit(drained);
                 mbar_wait(drained, 0);
             }
@@ -607,11 +668,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const bool cap = a.soft_cap > 0.f, biased = a.slopes != nullptr;
         const bool scaled = cap || biased || !(a.q_scale > 0.f);  // scores enter the exponent domain early
         const float f = scaled ? 1.f : a.q_scale;
+        const float cap1 = cap ? 2.f * kLog2e * a.q_scale / a.soft_cap : 0.f, cap2 = a.soft_cap * kLog2e;
         int c0 = 0, sn = 0;
         int qb = 0;                        // small blocks: q buffer (0 behind a large block, then in turn)
         int ou[2] = {0, 0};                // runs that used O of group 0, 1 so far
         int mln = 0;                       // small blocks of more than one tile so far
-        auto wait = [&](uint64_t *bar, int phase) { return warp_wait(bar, phase & 1, kSuspendTries, abort, kSuspendNs); };
+        auto wait = [&](uint64_t *bar, int phase) { return tile_wait(bar, phase & 1, abort); };
 
         // 128 rows of q from row `first` of the run's block into buffer `buf`
         auto fill = [&](const TileRun &u, int buf, int first) {
@@ -644,6 +706,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         while (have) {
             const int n = r.tb - r.ta;
             const bool big = r.b.nrows > 128;
+            TileRun u = r;  // the next run
+            const bool more = it.next(p, u);
+            const bool ubig = more && u.b.nrows > 128;
+            const int qn = big ? 0 : (qb ^ 1);
             const int ri = big ? 128 * t + row : row;  // row of the block
             const bool live = ri < r.b.nrows;
             // the row's query, its positions [lo, hi) and its bias
@@ -674,36 +740,52 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 if (!ok) break;
                 tc_fence_after();
                 if (warp_live) {
-                    float v[128];
+                    // Pass 1, 32 columns at a time: the row's largest score; scores that bias, cap or
+                    // mask change are written back, so that pass 2 is the same for all.
+                    const bool masked = __any_sync(0xffffffffu, live && (jlo > 0 || jhi < kTileTok));
+                    float mx0 = -INFINITY, mx1 = -INFINITY;
+                    auto largest = [&](float (&v)[32], int k) {
+                        if (scaled) {
+                            if (cap) {
+                                // cap tanh(y) = cap - 2 cap / (1 + e^2y): absolute error about 2^-22 cap
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tmem_ld<32>(t_s + 32 * k, v + 32 * k);
-                    tmem_wait_ld();
-                    if (scaled) {
-                        if (cap) {
-                            // cap tanh(y) = cap - 2 cap / (1 + e^2y): two exponent-pipe operations, absolute error
-                            // about 2^-22 cap
-                            const float c1 = 2.f * kLog2e * a.q_scale / a.soft_cap, c2 = a.soft_cap * kLog2e;
+                                for (int i = 0; i < 32; ++i)
+                                    v[i] = fmaf(-2.f * cap2, __fdividef(1.f, 1.f + fast_exp2(v[i] * cap1)), cap2);
+                            } else {
 #pragma unroll
-                            for (int i = 0; i < 128; ++i)
-                                v[i] = fmaf(-2.f * c2, __fdividef(1.f, 1.f + fast_exp2(v[i] * c1)), c2);
-                        } else {
+                                for (int i = 0; i < 32; ++i) v[i] *= a.q_scale;
+                            }
+                            if (biased) {
+                                const float d0 = static_cast<float>(t0 + 32 * k - pos);
 #pragma unroll
-                            for (int i = 0; i < 128; ++i) v[i] *= a.q_scale;
+                                for (int i = 0; i < 32; ++i) v[i] = fmaf(-slope, fabsf(d0 + static_cast<float>(i)), v[i]);
+                            }
                         }
-                        if (biased) {
-                            const float d0 = static_cast<float>(t0 - pos);
+                        if (masked) {
+                            const int l0 = jlo - 32 * k, h0 = jhi - 32 * k;
 #pragma unroll
-                            for (int i = 0; i < 128; ++i) v[i] = fmaf(-slope, fabsf(d0 + static_cast<float>(i)), v[i]);
+                            for (int i = 0; i < 32; ++i) v[i] = (i >= l0 && i < h0) ? v[i] : -INFINITY;
                         }
-                    }
-                    if (__any_sync(0xffffffffu, live && (jlo > 0 || jhi < kTileTok))) {
+                        if (scaled || masked) tmem_st32(t_s + 32 * k, v);
 #pragma unroll
-                        for (int i = 0; i < 128; ++i) v[i] = (i >= jlo && i < jhi) ? v[i] : -INFINITY;
+                        for (int i = 0; i < 32; i += 4) {
+                            mx0 = fmaxf(mx0, fmaxf(v[i], v[i + 1]));
+                            mx1 = fmaxf(mx1, fmaxf(v[i + 2], v[i + 3]));
+                        }
+                    };
+                    float va[32], vb[32];
+                    tmem_ld<32>(t_s, va);
+#pragma unroll 1
+                    for (int k = 0; k < 4; k += 2) {
+                        tmem_wait_ld();
+                        tmem_ld<32>(t_s + 32 * k + 32, vb);
+                        largest(va, k);
+                        tmem_wait_ld();
+                        if (k == 0) tmem_ld<32>(t_s + 64, va);
+                        largest(vb, k + 1);
                     }
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
+                    if (scaled || masked) tmem_wait_st();
+                    const float top = fmaxf(mx0, mx1) * f;
                     const bool move = live && (m == -INFINITY ? top > -INFINITY : top > m + kLazyMax);
                     if (__any_sync(0xffffffffu, move)) {
                         const float mn = move ? top : m;
@@ -723,29 +805,39 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                             }
                         }
                     }
+                    // Pass 2: P = 2^(x - m) over the columns read already, its sum, 64 columns in flight.
                     const float ref = m == -INFINITY ? 0.f : m;
-                    float ls[4] = {0.f, 0.f, 0.f, 0.f};
+                    float ls0 = 0.f, ls1 = 0.f;
+                    auto probs = [&](const float (&v)[32], int k) {
+                        uint32_t pk[16];
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        float pk[32];
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const float e0 = fast_exp2(fmaf(v[64 * k + 2 * i], f, -ref));
-                            const float e1 = fast_exp2(fmaf(v[64 * k + 2 * i + 1], f, -ref));
-                            ls[(2 * i) & 3] += e0;
-                            ls[(2 * i + 1) & 3] += e1;
-                            pk[i] = __uint_as_float(pack2<T>(e0, e1));
+                        for (int i = 0; i < 16; ++i) {
+                            const float e0 = fast_exp2(fmaf(v[2 * i], f, -ref));
+                            const float e1 = fast_exp2(fmaf(v[2 * i + 1], f, -ref));
+                            ls0 += e0;
+                            ls1 += e1;
+                            pk[i] = pack2<T>(e0, e1);
                         }
-                        tmem_st32(t_s + 32 * k, pk);
+                        tmem_st16(t_s + 16 * k, pk);
+                    };
+                    tmem_ld<32>(t_s, va);
+#pragma unroll 1
+                    for (int k = 0; k < 4; k += 2) {
+                        tmem_wait_ld();
+                        tmem_ld<32>(t_s + 32 * k + 32, vb);
+                        probs(va, k);
+                        tmem_wait_ld();
+                        if (k == 0) tmem_ld<32>(t_s + 64, va);
+                        probs(vb, k + 1);
                     }
-                    l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+                    l += ls0 + ls1;
                     tmem_wait_st();
                 }
                 // V rows that no row of the block attends are cleared (a zero probability does not
                 // cancel a NaN): by group 0 for both groups, or by the tile's own group
                 const int vlo = r.b.lo - t0, vhi = r.b.hi - t0;
                 if ((vlo > 0 || vhi < kTileTok) && (t == 0 || !big)) {
-                    const int cv = c0 + 2 * j + 1;
+                    const int cv = c0 + v_at(j, n);
                     ok = wait(&full[cv % NS], cv / NS);
                     if (!ok) break;
                     const uint32_t vt = smem_u32(ring) + (cv % NS) * L::kSlot;
@@ -758,20 +850,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[t]);
+                // this tile's scores came behind every score of the run in front: its q buffer is free
+                if (j == 0 && t == 0 && more && !big && !ubig) fill(u, qn, 0);
             }
             if (!ok) break;
 
-            // ------------------------------------------------ the next run's q
-            TileRun u = r;
-            const bool more = it.next(p, u);
-            const bool ubig = more && u.b.nrows > 128;
-            const bool late = !big && ubig;  // both groups read one buffer in this run, each fills one in the next
-            const int qn = big ? 0 : (qb ^ 1);
-            if (more && !late) {
+            // The next run's q.  Behind a small run, both groups read one buffer: a large run's fills
+            // wait for the end (`late`), a small one's took the other buffer after the first tile.
+            const bool late = !big && ubig;
+            if (more && big) {
                 if (ubig)
                     fill(u, t, 128 * t);
                 else if (t == 0)
-                    fill(u, qn, 0);
+                    fill(u, 0, 0);
             }
 
             // ------------------------------------------------ end of the run
