@@ -349,7 +349,7 @@ struct TileSmem {
     static constexpr uint32_t ring = 2 * kQ;
     static constexpr uint32_t ml = ring + kSlots * kSlot;  // [2 runs][2][128] floats
     static constexpr uint32_t bars = ml + 2 * 2 * 128 * 4;
-    static constexpr int kBars = 2 * kSlots + 2 * 5 + 2;
+    static constexpr int kBars = 2 * kSlots + 2 * 6 + 2;
     static constexpr uint32_t misc = bars + kBars * 8;
     static constexpr uint32_t total = misc + 16;
 };
@@ -364,6 +364,21 @@ __device__ __forceinline__ bool tile_wait(uint64_t *bar, uint32_t parity, volati
         if (!ok && i + 1 == kSuspendTries) raise_status(GOLLEK_STATUS_TIMEOUT);
     }
     return __all_sync(0xffffffffu, ok);
+}
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t &>(d))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)), "l"(reinterpret_cast<uint64_t &>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t &>(d))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return d;
 }
 
 // D[tmem] (+)= A[tmem] * B, issued by one thread.
@@ -420,7 +435,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     uint64_t *o_free = o_full + 2;  // [2] O read
     uint64_t *q_full = o_free + 2;  // [2] q staged in buffer 0, 1
     uint64_t *ml_full = q_full + 2; // group 1's (m, l) handed over
-    uint64_t *drained = ml_full + 1;
+    uint64_t *p_half = ml_full + 1; // [2] probabilities of the tile's first 64 positions
+    uint64_t *drained = p_half + 2;
     volatile int *abort = reinterpret_cast<volatile int *>(smem + L::misc);
     uint32_t *sm_tmem = reinterpret_cast<uint32_t *>(smem + L::misc + 4);
 
@@ -433,6 +449,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&s_full[t], 1);
+            mbar_init(&p_half[t], 4);
             mbar_init(&p_full[t], 4);
             mbar_init(&o_full[t], 1);
             mbar_init(&o_free[t], 4);
@@ -568,22 +585,26 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     umma_commit(&s_full[t]);
                 }
             };
+            // O += P V of group t with V of ring position c, in two halves as P arrives; O is free
+            // first (its last user's run has read it)
             auto value = [&](int t, int c, bool first) {
                 const int slot = __shfl_sync(0xffffffffu, c % NS, 0);
                 const uint64_t vd = v_desc + slot * (L::kSlot >> 4);
                 const uint32_t d = tmem + 256 + 128 * t, pa = tmem + 128 * t;
-                if (leader) {
+                if (first && ou[t] > 0 && !wait(&o_free[t], (ou[t] - 1) & 1)) return false;
+                if (!wait(&full[slot], (c / NS) & 1)) return false;
 #pragma unroll
-                    for (int kk = 0; kk < kTileTok / 16; ++kk)
-                        umma_f16_ts(d, pa + 8 * kk, vd + kk * (32 * D >> 4), id_o, !(first && kk == 0));
+                for (int half = 0; half < 2; ++half) {
+                    if (!wait(half ? &p_full[t] : &p_half[t], pp[t] & 1)) return false;
+                    tc_fence_after();
+                    if (leader) {
+#pragma unroll
+                        for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+                            umma_f16_ts(d, pa + 8 * kk, vd + kk * (32 * D >> 4), id_o, !(first && kk == 0));
+                    }
                 }
                 ++pp[t];
-            };
-            // P of group t is there, V of ring position c is there, and (first use in a run) O is free
-            auto value_ready = [&](int t, int c, bool first) {
-                bool w = wait(&p_full[t], pp[t] & 1) && wait(&full[c % NS], (c / NS) & 1);
-                if (w && first && ou[t] > 0) w = wait(&o_free[t], (ou[t] - 1) & 1);
-                return w;
+                return true;
             };
             while (ok && it.next(p, r)) {
                 const int n = r.tb - r.ta;
@@ -598,10 +619,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         for (int t = 0; t < 2; ++t) {
                             if (!ok) break;
                             if (j > 0) {
-                                ok = value_ready(t, cv, j == 1);
+                                ok = value(t, cv, j == 1);
                                 if (!ok) break;
-                                tc_fence_after();
-                                value(t, cv, j == 1);
                                 if (j == n) commit(&o_full[t]);
                             }
                             tc_fence_after();
@@ -625,10 +644,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                             if (!ok) break;
                             if (j >= 2 && j - 2 < n) {
                                 const int cv = c0 + v_at(j - 2, n);
-                                ok = value_ready(t, cv, j - 2 < 2);
+                                ok = value(t, cv, j - 2 < 2);
                                 if (!ok) break;
-                                tc_fence_after();
-                                value(t, cv, j - 2 < 2);
                                 if (j >= n) commit(&o_full[t]);
                                 commit(&empty[cv % NS]);
                             }
@@ -695,6 +712,37 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (lane == 0) mbar_arrive(&q_full[buf]);
         };
 
+        // Bias, cap and mask of the tile at position t0: S becomes the score in the exponent domain
+        // (scaled), -inf outside columns [jlo, jhi).
+        auto rewrite = [&](int t0, int jlo, int jhi, bool masked, float slope, int pos) {
+#pragma unroll 1
+            for (int k = 0; k < 128; k += 32) {
+                float v[32];
+                tmem_ld<32>(t_s + k, v);
+                tmem_wait_ld();
+                if (cap) {
+                    // cap tanh(y) = cap - 2 cap / (1 + e^2y): absolute error about 2^-22 cap
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        v[i] = fmaf(-2.f * cap2, __fdividef(1.f, 1.f + fast_exp2(v[i] * cap1)), cap2);
+                } else if (scaled) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] *= a.q_scale;
+                }
+                if (biased) {
+                    const float d0 = static_cast<float>(t0 + k - pos);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = fmaf(-slope, fabsf(d0 + static_cast<float>(i)), v[i]);
+                }
+                if (masked) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = (i >= jlo - k && i < jhi - k) ? v[i] : -INFINITY;
+                }
+                tmem_st32(t_s + k, v);
+            }
+            tmem_wait_st();
+        };
+
         bool ok = true;
         bool have = it.next(p, r);
         if (have) {
@@ -739,100 +787,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 ok = wait(&s_full[t], sn++);
                 if (!ok) break;
                 tc_fence_after();
-                if (warp_live) {
-                    // Pass 1, 32 columns at a time: the row's largest score; scores that bias, cap or
-                    // mask change are written back, so that pass 2 is the same for all.
-                    const bool masked = __any_sync(0xffffffffu, live && (jlo > 0 || jhi < kTileTok));
-                    float mx0 = -INFINITY, mx1 = -INFINITY;
-                    auto largest = [&](float (&v)[32], int k) {
-                        if (scaled) {
-                            if (cap) {
-                                // cap tanh(y) = cap - 2 cap / (1 + e^2y): absolute error about 2^-22 cap
-#pragma unroll
-                                for (int i = 0; i < 32; ++i)
-                                    v[i] = fmaf(-2.f * cap2, __fdividef(1.f, 1.f + fast_exp2(v[i] * cap1)), cap2);
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) v[i] *= a.q_scale;
-                            }
-                            if (biased) {
-                                const float d0 = static_cast<float>(t0 + 32 * k - pos);
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) v[i] = fmaf(-slope, fabsf(d0 + static_cast<float>(i)), v[i]);
-                            }
-                        }
-                        if (masked) {
-                            const int l0 = jlo - 32 * k, h0 = jhi - 32 * k;
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = (i >= l0 && i < h0) ? v[i] : -INFINITY;
-                        }
-                        if (scaled || masked) tmem_st32(t_s + 32 * k, v);
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            mx0 = fmaxf(mx0, fmaxf(v[i], v[i + 1]));
-                            mx1 = fmaxf(mx1, fmaxf(v[i + 2], v[i + 3]));
-                        }
-                    };
-                    float va[32], vb[32];
-                    tmem_ld<32>(t_s, va);
-#pragma unroll 1
-                    for (int k = 0; k < 4; k += 2) {
-                        tmem_wait_ld();
-                        tmem_ld<32>(t_s + 32 * k + 32, vb);
-                        largest(va, k);
-                        tmem_wait_ld();
-                        if (k == 0) tmem_ld<32>(t_s + 64, va);
-                        largest(vb, k + 1);
-                    }
-                    if (scaled || masked) tmem_wait_st();
-                    const float top = fmaxf(mx0, mx1) * f;
-                    const bool move = live && (m == -INFINITY ? top > -INFINITY : top > m + kLazyMax);
-                    if (__any_sync(0xffffffffu, move)) {
-                        const float mn = move ? top : m;
-                        const float alpha = (mn == m || m == -INFINITY) ? 1.f : fast_exp2(m - mn);
-                        m = mn;
-                        l *= alpha;
-                        // the scores' commit covers the group's earlier value MMAs: O is at rest
-                        if (__any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll 1
-                            for (int k = 0; k < D / 32; ++k) {
-                                float o[32];
-                                tmem_ld<32>(t_o + 32 * k, o);
-                                tmem_wait_ld();
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) o[i] *= alpha;
-                                tmem_st32(t_o + 32 * k, o);
-                            }
-                        }
-                    }
-                    // Pass 2: P = 2^(x - m) over the columns read already, its sum, 64 columns in flight.
-                    const float ref = m == -INFINITY ? 0.f : m;
-                    float ls0 = 0.f, ls1 = 0.f;
-                    auto probs = [&](const float (&v)[32], int k) {
-                        uint32_t pk[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float e0 = fast_exp2(fmaf(v[2 * i], f, -ref));
-                            const float e1 = fast_exp2(fmaf(v[2 * i + 1], f, -ref));
-                            ls0 += e0;
-                            ls1 += e1;
-                            pk[i] = pack2<T>(e0, e1);
-                        }
-                        tmem_st16(t_s + 16 * k, pk);
-                    };
-                    tmem_ld<32>(t_s, va);
-#pragma unroll 1
-                    for (int k = 0; k < 4; k += 2) {
-                        tmem_wait_ld();
-                        tmem_ld<32>(t_s + 32 * k + 32, vb);
-                        probs(va, k);
-                        tmem_wait_ld();
-                        if (k == 0) tmem_ld<32>(t_s + 64, va);
-                        probs(vb, k + 1);
-                    }
-                    l += ls0 + ls1;
-                    tmem_wait_st();
-                }
                 // V rows that no row of the block attends are cleared (a zero probability does not
                 // cancel a NaN): by group 0 for both groups, or by the tile's own group
                 const int vlo = r.b.lo - t0, vhi = r.b.hi - t0;
@@ -846,6 +800,90 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         if (tok < vlo || tok >= vhi) sts_u4(vt + kv_chunk_off<D>(tok, i % (D / 8)), make_uint4(0, 0, 0, 0));
                     }
                     fence_proxy_async_smem();
+                }
+                // Short loops: the code of a tile has to fit the instruction cache closest to the warp
+                // (fully unrolled over the 128 columns it ran a third slower).
+                float ref = 0.f;
+                if (warp_live) {
+                    // bias, cap and mask, where a tile has any: the scores are rewritten in place
+                    const bool masked = __any_sync(0xffffffffu, live && (jlo > 0 || jhi < kTileTok));
+                    if (scaled || masked) rewrite(t0, jlo, jhi, masked, slope, pos);
+                    // pass 1: the row's largest score
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    float va[16], vb[16];
+                    auto largest = [&](const float (&v)[16]) {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 8)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(v[i + e], v[i + e + 4]));
+                    };
+                    tmem_ld<16>(t_s, va);
+#pragma unroll 1
+                    for (int k = 0; k < 128; k += 32) {
+                        tmem_wait_ld();
+                        tmem_ld<16>(t_s + k + 16, vb);
+                        largest(va);
+                        tmem_wait_ld();
+                        tmem_ld<16>(t_s + (k + 32 & 127), va);  // the last one reads the first columns for pass 2
+                        largest(vb);
+                    }
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
+                    const bool move = live && (m == -INFINITY ? top > -INFINITY : top > m + kLazyMax);
+                    if (__any_sync(0xffffffffu, move)) {
+                        const float mn = move ? top : m;
+                        const float alpha = (mn == m || m == -INFINITY) ? 1.f : fast_exp2(m - mn);
+                        m = mn;
+                        l *= alpha;
+                        // the scores' commit covers the group's earlier value MMAs: O is at rest
+                        if (__any_sync(0xffffffffu, alpha != 1.f)) {
+                            tmem_wait_ld();
+#pragma unroll 1
+                            for (int k = 0; k < D / 32; ++k) {
+                                float o[32];
+                                tmem_ld<32>(t_o + 32 * k, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] *= alpha;
+                                tmem_st32(t_o + 32 * k, o);
+                            }
+                        }
+                    }
+                    ref = m == -INFINITY ? 0.f : m;
+                    // pass 2: P = 2^(x - m) over the columns read already, and its sum; the value MMA of
+                    // the first 64 positions starts while the others are computed
+                    float2 sum = make_float2(0.f, 0.f);
+                    const float2 ff = make_float2(f, f), rr = make_float2(-ref, -ref);
+                    auto probs = [&](const float (&v)[16], uint32_t (&pk)[16], int at) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            float2 x = fma2(make_float2(v[2 * i], v[2 * i + 1]), ff, rr);
+                            x.x = fast_exp2(x.x);
+                            x.y = fast_exp2(x.y);
+                            sum = add2(sum, x);
+                            pk[at + i] = pack2<T>(x.x, x.y);
+                        }
+                    };
+#pragma unroll 1
+                    for (int k = 0; k < 128; k += 32) {
+                        uint32_t pk[16];
+                        tmem_wait_ld();
+                        tmem_ld<16>(t_s + k + 16, vb);
+                        probs(va, pk, 0);
+                        tmem_wait_ld();
+                        if (k < 96) tmem_ld<16>(t_s + k + 32, va);
+                        probs(vb, pk, 8);
+                        tmem_st16(t_s + (k >> 1), pk);
+                        if (k == 32) {
+                            tmem_wait_st();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&p_half[t]);
+                        }
+                    }
+                    tmem_wait_st();
+                    l += sum.x + sum.y;
+                } else if (lane == 0) {
+                    mbar_arrive(&p_half[t]);
                 }
                 tc_fence_before();
                 __syncwarp();
