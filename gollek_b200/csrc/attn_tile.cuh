@@ -41,7 +41,7 @@ constexpr int kTileTok = 128;
 constexpr int kBlkRows = 256;
 constexpr int kRunCostTiles = 2;      // start-up of a run (q, pipeline fill, output), in tiles
 constexpr int kMaxTileCtas = 160;
-constexpr int kTileThreads = 384;     // 8 row warps, 1 MMA issuer, 1 producer, 2 idle
+constexpr int kTileThreads = 384;     // 8 row warps, 2 MMA issuers, 1 producer, 1 idle
 // Registers: launched with 168 a thread (384 x 168 = 64,512 of the SM's 65,536), of which the
 // third warpgroup gives the row groups 40 each: 2 x 208 + 88 = 3 x 168.  A row thread holds a
 // tile's 128 scores; at 168 it would spill 560 bytes.
@@ -50,8 +50,11 @@ constexpr float kLazyMax = 8.f;
 
 // A block: rows row0 .. row0 + nrows - 1 (row r: query token tok0 + r / G, q head h G + r % G)
 // over positions [lo, hi) of table row `tab`, whose length is len.
-struct TileBlk {
-    int tab, tok0, row0, nrows, lo, hi, len, kind;
+// A varlen row's query i sits at position pos0 + i.
+struct __align__(16) TileBlk {
+    int tok0, row0, nrows, kind;
+    int lo, hi, tab, len;
+    int pos0, pad[3];
 };
 enum { kOwn = 0, kPrefix = 1, kSuffix = 2 };  // varlen; shared: the group's prefix, a sequence's own tokens
 
@@ -223,7 +226,8 @@ __global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(const TileArgs 
             k.hi = k.len;
             if (k.kind == kOwn) {
                 const int i0 = k.row0 / G, i1 = (k.row0 + k.nrows - 1) / G;
-                const int pos0 = k.len - n + i0, pos1 = k.len - n + i1;
+                k.pos0 = k.len - n;
+                const int pos0 = k.pos0 + i0, pos1 = k.pos0 + i1;
                 if (a.causal) {
                     k.hi = pos1 + 1;
                     if (a.prefix_lens) k.hi = max(k.hi, min(a.prefix_lens[e], k.len));
@@ -345,25 +349,59 @@ struct TileSmem {
     static constexpr uint32_t kSlot = kTileTok * D * 2;  // K or V of one tile
     static constexpr uint32_t kQ = 128 * D * 2;          // 128 rows
     static constexpr int kSlots = D == 128 ? 5 : 10;
+    static constexpr int kRuns = 4;                        // run descriptors in flight
     static constexpr uint32_t q = 0;
     static constexpr uint32_t ring = 2 * kQ;
-    static constexpr uint32_t ml = ring + kSlots * kSlot;  // [2 runs][2][128] floats
-    static constexpr uint32_t bars = ml + 2 * 2 * 128 * 4;
-    static constexpr int kBars = 2 * kSlots + 2 * 6 + 2;
+    static constexpr uint32_t ml = ring + kSlots * kSlot;  // [2][128] floats
+    static constexpr uint32_t runs = ml + 2 * 128 * 4;     // [kRuns] x 48 bytes
+    static constexpr uint32_t bars = runs + kRuns * 48;
+    static constexpr int kBars = 2 * kSlots + 2 * kRuns + 2 * 7 + 8 + 1;
     static constexpr uint32_t misc = bars + kBars * 8;
     static constexpr uint32_t total = misc + 16;
 };
 
+// A run as the producer hands it to the other warps (in shared memory): n tiles of a
+// block's rows (n = 0: no more runs), tile j from position 128 (tile0 - j).  The last
+// positions come first: a causal row's largest scores, with a distance bias above all, lie
+// near its own position, so the running maximum seldom moves after the first tile.
+struct __align__(16) RunDesc {
+    int tok0, row0, nrows, h;
+    int lo, hi, tile0, n;
+    int tab, len, pos0, flags;  // flags: kind, 4: the whole unit, 8: its first tiles
+};
+
 // Bounded wait of a whole warp: each lane tests on its own, one vote at the end (the
-// result is warp-uniform); gives up once another warp did.
+// result is warp-uniform); gives up once another warp did.  The warp that gives up first
+// raises the status (tile_give_up), at the end of its role and not here, which keeps the
+// code of a wait short.
 __device__ __forceinline__ bool tile_wait(uint64_t *bar, uint32_t parity, volatile int *abort) {
     bool ok = mbar_try_wait(bar, parity);
+#pragma unroll 1
     for (unsigned i = 0; !ok && i < kSuspendTries; ++i) {
         if (*abort) break;
         ok = mbar_try_wait_suspend(bar, parity, kSuspendNs);
-        if (!ok && i + 1 == kSuspendTries) raise_status(GOLLEK_STATUS_TIMEOUT);
     }
     return __all_sync(0xffffffffu, ok);
+}
+__device__ __forceinline__ void tile_give_up(volatile int *abort) {
+    if (*abort == 0) raise_status(GOLLEK_STATUS_TIMEOUT);
+    *abort = 1;
+}
+
+// x / d for 0 <= x < 2^31: the magic's quotient is at most one too large.
+__device__ __forceinline__ unsigned div_magic(int d) { return d == 1 ? 0u : 0xFFFFFFFFu / d + 1; }
+__device__ __forceinline__ int fast_div(int x, int d, unsigned magic) {
+    int q = d == 1 ? x : static_cast<int>(__umulhi(x, magic));
+    return q * d > x ? q - 1 : q;
+}
+
+// A value the compiler cannot reason about.  Loops test their run-wide conditions through it:
+// left to itself the compiler copies each loop once per condition, and the kernel's 100 KB of
+// code then missed the instruction cache all the time.
+__device__ __forceinline__ bool opaque(bool x) {
+    int v = x;
+    asm volatile("" : "+r"(v));
+    return v != 0;
 }
 
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -412,7 +450,7 @@ struct PageLoc {
 
 // Ring positions, from the run's first, of K and V of tile j of n: a value product follows
 // the scores of the next tile, so V is copied behind the next K and waits less for its use.
-__device__ __forceinline__ int k_at(int j) { return j == 0 ? 0 : 2 * j - 1; }
+
 __device__ __forceinline__ int v_at(int j, int n) { return j == n - 1 ? 2 * n - 1 : 2 * j + 2; }
 
 template <typename T, int D>
@@ -423,40 +461,46 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     constexpr int kBf16 = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
     const AttnArgs &a = p.a;
     extern __shared__ __align__(1024) uint8_t tile_smem[];
-    uint8_t *smem = tile_smem;
-    const uint32_t q_s = smem_u32(smem + L::q);
-    uint8_t *ring = smem + L::ring;
-    float *sm_ml = reinterpret_cast<float *>(smem + L::ml);
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::bars);
+    uint8_t *ring = tile_smem + L::ring;
+    float *sm_ml = reinterpret_cast<float *>(tile_smem + L::ml);
+    RunDesc *runs = reinterpret_cast<RunDesc *>(tile_smem + L::runs);
+    uint64_t *full = reinterpret_cast<uint64_t *>(tile_smem + L::bars);
     uint64_t *empty = full + NS;
-    uint64_t *s_full = empty + NS;  // [2] scores in tensor memory (and every earlier MMA done)
-    uint64_t *p_full = s_full + 2;  // [2] probabilities in tensor memory (V cleared, O rescaled)
-    uint64_t *o_full = p_full + 2;  // [2] a run's last value MMA of the group done
-    uint64_t *o_free = o_full + 2;  // [2] O read
-    uint64_t *q_full = o_free + 2;  // [2] q staged in buffer 0, 1
-    uint64_t *ml_full = q_full + 2; // group 1's (m, l) handed over
-    uint64_t *p_half = ml_full + 1; // [2] probabilities of the tile's first 64 positions
-    uint64_t *drained = p_half + 2;
-    volatile int *abort = reinterpret_cast<volatile int *>(smem + L::misc);
-    uint32_t *sm_tmem = reinterpret_cast<uint32_t *>(smem + L::misc + 4);
+    uint64_t *run_full = empty + NS;           // [kRuns] descriptor written
+    uint64_t *run_free = run_full + L::kRuns;  // [kRuns] descriptor read by the 10 warps that use it
+    uint64_t *s_full = run_free + L::kRuns;    // [2] scores in tensor memory (and every earlier MMA done)
+    uint64_t *p_full = s_full + 2;             // [2] probabilities in tensor memory (V cleared, O rescaled)
+    uint64_t *o_full = p_full + 2;             // [2] a run's last value MMA of the group done
+    uint64_t *o_free = o_full + 2;             // [2] O read
+    uint64_t *q_full = o_free + 2;             // [2] q staged in buffer 0, 1
+    uint64_t *q_free = q_full + 2;             // [2] q buffer read by both issuers
+    uint64_t *drained = q_free + 2;            // [2] an issuer's MMAs done
+    uint64_t *turn = drained + 2;              // [2][4] group t's warp may use the exponent pipe
+    uint64_t *ml_full = turn + 8;              // group 1's (m, l) handed over
+    volatile int *abort = reinterpret_cast<volatile int *>(tile_smem + L::misc);
+    uint32_t *sm_tmem = reinterpret_cast<uint32_t *>(tile_smem + L::misc + 4);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int G = a.num_q_heads / a.num_kv_heads;
     if (tid == 0) {
         for (int i = 0; i < NS; ++i) {
             mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
+            mbar_init(&empty[i], 2);
+        }
+        for (int i = 0; i < L::kRuns; ++i) {
+            mbar_init(&run_full[i], 1);
+            mbar_init(&run_free[i], 10);
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&s_full[t], 1);
-            mbar_init(&p_half[t], 4);
             mbar_init(&p_full[t], 4);
             mbar_init(&o_full[t], 1);
             mbar_init(&o_free[t], 4);
             mbar_init(&q_full[t], 4);
+            mbar_init(&q_free[t], 2);
+            mbar_init(&drained[t], 1);
         }
+        for (int i = 0; i < 8; ++i) mbar_init(&turn[i], 1);
         mbar_init(ml_full, 4);
-        mbar_init(drained, 1);
         fence_barrier_init();
         *abort = 0;
     }
@@ -472,325 +516,411 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *sm_tmem;
-    pdl_wait();  // the plan is complete
+    auto wait = [&](uint64_t *bar, uint32_t phase) { return tile_wait(bar, phase & 1, abort); };
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kAuxRegs));
-        RunIter it;
-        it.begin(p, blockIdx.x);
-        TileRun r;
         if (warp == 9) {
             // ===================================================================== producer
-            // Tiles of all runs in one line, the page lookups two tiles ahead of the copies (so a run's
-            // first pages are known before the last ones of the run in front have a slot).
+            // Walks the runs, hands their descriptors out and copies their tiles; the page lookups go
+            // two tiles ahead of the copies, across runs.
+            pdl_wait();  // the plan is complete
+            RunIter it;
+            it.begin(p, blockIdx.x);
+            TileRun r{};
             struct Step {
                 PageLoc loc;
                 bool live, first, last;
             };
-            const int R = a.block_size < 16 ? a.block_size : 16, per = 16 / R;
+            const int R = a.block_size < 16 ? a.block_size : 16;
+            const unsigned bs_magic = div_magic(a.block_size);
             const int *bt = nullptr;
-            int t = 0, tb = 0, ta = 0;
-            auto step = [&]() {
-                Step s{{-1, -1}, false, false, false};
-                if (t >= tb) {
-                    if (!it.next(p, r)) return s;
+            int t = 0, tb = 0, ta = 0, nrun = 0;
+            int slot = 0, copies = 0;
+            uint32_t ph = 1;
+            bool ok = true, more = true;
+            Step s0{{-1, -1}, false, false, false}, s1 = s0;
+            PageLoc before{-1, -1};
+            // ring order of a run: K0, K1, V0, K2, V1, ... V(n-1) (v_at).  The first two rounds only fill
+            // the look-ahead; each part of the code stands here once, to keep it short.
+#pragma unroll 1
+            for (int round = 0; ok && (round < 2 || s0.live); ++round) {
+                Step s2{{-1, -1}, false, false, false};
+                if (t >= tb && more) {
+                    // the next run: its descriptor for the other warps, its table
+                    more = it.next(p, r);
+                    const int at = nrun % L::kRuns;
+                    if (nrun >= L::kRuns) ok = wait(&run_free[at], nrun / L::kRuns - 1);
+                    if (lane == 0 && ok) {
+                        RunDesc &d = runs[at];
+                        d.tok0 = r.b.tok0;
+                        d.row0 = r.b.row0;
+                        d.nrows = r.b.nrows;
+                        d.h = r.h;
+                        d.lo = r.b.lo;
+                        d.hi = r.b.hi;
+                        d.tile0 = r.b.lo / kTileTok + r.tb - 1;
+                        d.n = more ? r.tb - r.ta : 0;
+                        d.tab = r.b.tab;
+                        d.len = r.b.len;
+                        d.pos0 = r.b.pos0;
+                        d.flags = r.b.kind | (r.ta == 0 && r.tb == r.n ? 4 : 0) | (r.ta == 0 ? 8 : 0);
+                        mbar_arrive(&run_full[at]);
+                    }
+                    __syncwarp();
+                    ++nrun;
                     bt = r.b.kind == kPrefix ? a.prefix_tables + static_cast<long long>(r.b.tab) * a.max_pblocks
                                              : a.block_tables + static_cast<long long>(r.b.tab) * a.max_blocks;
                     t = ta = r.ta;
-                    tb = r.tb;
+                    tb = more ? r.tb : r.ta;
                 }
-                s.live = true;
-                s.first = t == ta;
-                s.last = t == tb - 1;
-                // pool rows / 8 of the lane's box(es); -1: nothing to load there
-                const int pos = (r.b.lo / kTileTok + t) * kTileTok + lane * 16;
-                auto row8 = [&](int at) {
-                    if (lane >= 8 || at >= r.b.hi || at + R <= r.b.lo) return -1;
-                    const int pg = at / a.block_size;
-                    int e = __ldg(bt + pg);
-                    if (e < 0 || (a.num_blocks > 0 && e >= a.num_blocks)) {
-                        raise_status(GOLLEK_STATUS_BAD_BLOCK_ID);
-                        e = 0;
+                if (t < tb) {
+                    s2.live = true;
+                    s2.first = t == ta;
+                    s2.last = t == tb - 1;
+                    // pool rows / 8 of the lane's box(es); -1: nothing to load there
+                    int at = (r.b.lo / kTileTok + tb - 1 - (t - ta)) * kTileTok + lane * 16;
+#pragma unroll 1
+                    for (int k = 0; k < 16; k += R, at += R) {
+                        if (lane >= 8 || at >= r.b.hi || at + R <= r.b.lo) continue;
+                        const int pg = fast_div(at, a.block_size, bs_magic);
+                        int e = __ldg(bt + pg);
+                        if (e < 0 || (a.num_blocks > 0 && e >= a.num_blocks)) {
+                            raise_status(GOLLEK_STATUS_BAD_BLOCK_ID);
+                            e = 0;
+                        }
+                        const int at8 = static_cast<int>((e * p.page_rows + static_cast<long long>(r.h) * a.block_size +
+                                                          (at - pg * a.block_size)) >> 3);
+                        if (k == 0)
+                            s2.loc.row0 = at8;
+                        else
+                            s2.loc.row1 = at8;
                     }
-                    return static_cast<int>((e * p.page_rows + static_cast<long long>(r.h) * a.block_size +
-                                             (at - pg * a.block_size)) >> 3);
-                };
-                s.loc.row0 = row8(pos);
-                if (per == 2) s.loc.row1 = row8(pos + R);
-                ++t;
-                return s;
-            };
-            int c = 0;  // ring position
-            auto copy = [&](const PageLoc &l, const CUtensorMap *map) {
-                const int slot = c % NS;
-                if (c >= NS && !tile_wait(&empty[slot], (c / NS - 1) & 1, abort)) return false;
-                const unsigned boxes = (l.row0 >= 0) + (l.row1 >= 0);
-                const uint32_t bytes = __reduce_add_sync(0xffffffffu, boxes) * R * D * 2;
-                if (lane == 0) mbar_arrive_expect_tx(&full[slot], bytes);
-                __syncwarp();
-                uint8_t *dst = ring + slot * L::kSlot + lane * (16 * D * 2);
-                if (l.row0 >= 0) tma_load_4d(dst, map, 0, 0, 0, l.row0, &full[slot]);
-                if (l.row1 >= 0) tma_load_4d(dst + R * D * 2, map, 0, 0, 0, l.row1, &full[slot]);
-                ++c;
-                return true;
-            };
-            // ring order of a run: K0, K1, V0, K2, V1, ... V(n-1) (k_at, v_at)
-            bool ok = true;
-            Step s0 = step(), s1 = step();
-            PageLoc before{-1, -1};
-            while (ok && s0.live) {
-                const Step s2 = step();
-                ok = copy(s0.loc, &tm_k);
-                if (ok && !s0.first) ok = copy(before, &tm_v);
-                if (ok && s0.last) ok = copy(s0.loc, &tm_v);
+                    __syncwarp();
+                    ++t;
+                }
+                // K of this tile, V of the tile before it in the run, V of the run's last tile
+#pragma unroll 1
+                for (int w = 0; w < 3 && s0.live && ok; ++w) {
+                    if ((w == 1 && s0.first) || (w == 2 && !s0.last)) continue;
+                    const PageLoc l = w == 1 ? before : s0.loc;
+                    if (copies >= NS) ok = wait(&empty[slot], ph);
+                    if (!ok) break;
+                    const unsigned boxes = (l.row0 >= 0) + (l.row1 >= 0);
+                    const uint32_t bytes = __reduce_add_sync(0xffffffffu, boxes) * R * D * 2;
+                    if (lane == 0) mbar_arrive_expect_tx(&full[slot], bytes);
+                    __syncwarp();
+                    uint8_t *dst = ring + slot * L::kSlot + lane * (16 * D * 2);
+                    const CUtensorMap *map = w ? &tm_v : &tm_k;
+                    if (l.row0 >= 0) tma_load_4d(dst, map, 0, 0, 0, l.row0, &full[slot]);
+                    if (l.row1 >= 0) tma_load_4d(dst + 8 * D * 2, map, 0, 0, 0, l.row1, &full[slot]);
+                    ++copies;
+                    if (++slot == NS) {
+                        slot = 0;
+                        ph ^= 1;
+                    }
+                }
                 before = s0.loc;
                 s0 = s1;
                 s1 = s2;
             }
-            if (!ok && lane == 0) *abort = 1;
+            if (!ok && lane == 0) tile_give_up(abort);
             // every copy issued lands before the shared memory is released
             if (lane == 0)
-                for (int k = max(0, c - NS); k < c; ++k) mbar_wait(&full[k % NS], (k / NS) & 1);
+                for (int k = max(0, copies - NS); k < copies; ++k) mbar_wait(&full[k % NS], (k / NS) & 1);
             __syncwarp();
-        } else if (warp == 8) {
-            // ===================================================================== MMA issuer
-            // The whole warp walks the tiles with warp-uniform values (so descriptors stay in uniform
-            // registers) and one elected lane issues: a lane that computed descriptors on its own took
-            // 2,300 cycles for the 16 MMAs of a step that run in about 1,000.
+        } else if (warp != 11) {
+            // ===================================================================== MMA issuers
+            // Warp 8 issues group 0's MMAs, warp 10 group 1's: what one waits for does not hold the
+            // other up.  The warp walks its steps with warp-uniform values (descriptors stay in uniform
+            // registers) and one elected lane issues.
+            const int t = warp == 10;
             constexpr uint32_t id_s = umma_idesc_16bit(128, kTileTok, kBf16, 0, 0);
             constexpr uint32_t id_o = umma_idesc_16bit(128, D, kBf16, 0, 1);
-            const uint64_t q_desc = umma_desc_sw128(q_s, 16, 1024);
+            const uint64_t q_desc = umma_desc_sw128(smem_u32(tile_smem + L::q), 16, 1024);
             const uint64_t k_desc = umma_desc_sw128(smem_u32(ring), 16, 16 * D);
             const uint64_t v_desc = umma_desc_sw128(smem_u32(ring), 1024, 16 * D);
+            const uint32_t t_s = tmem + 128 * t, t_o = tmem + 256 + 128 * t;
             const bool leader = elect_one();
-            int c0 = 0;                   // ring position of the run's first K
-            int pp[2] = {0, 0};           // probabilities taken from group t so far
-            int ou[2] = {0, 0};           // runs that used O of group t so far
-            int qu[2] = {0, 0};           // fills of q buffer t consumed so far
-            int qb = 1;                   // q buffer of the last small block; 1 after a large one
+            int slot = 0;      // next ring slot and its phase
+            uint32_t ring_ph = 0;
+            uint32_t pp = 0;   // phase of the next probabilities
+            int ou = 0;        // runs that used this group's O so far
+            uint32_t qph = 0;  // bit b: phase of the next fill of q buffer b
+            int qb = 1;        // q buffer of the last small block; 1 after a large one
             bool ok = true;
-            auto wait = [&](uint64_t *bar, uint32_t par) { return tile_wait(bar, par, abort); };
-            auto commit = [&](uint64_t *bar) {
-                if (leader) umma_commit(bar);
-            };
-            auto score = [&](int t, int buf, int c) {
-                const int slot = __shfl_sync(0xffffffffu, c % NS, 0);
-                const uint64_t qd = q_desc + buf * (L::kQ >> 4), kd = k_desc + slot * (L::kSlot >> 4);
-                const uint32_t d = tmem + 128 * t;
-                if (leader) {
-#pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk)
-                        umma_f16(d, qd + (kk >> 2) * (16384 >> 4) + (kk & 3) * 2, kd + (kk >> 2) * (1024 >> 4) + (kk & 3) * 2,
-                                 id_s, kk > 0);
-                    umma_commit(&s_full[t]);
-                }
-            };
-            // O += P V of group t with V of ring position c, in two halves as P arrives; O is free
-            // first (its last user's run has read it)
-            auto value = [&](int t, int c, bool first) {
-                const int slot = __shfl_sync(0xffffffffu, c % NS, 0);
-                const uint64_t vd = v_desc + slot * (L::kSlot >> 4);
-                const uint32_t d = tmem + 256 + 128 * t, pa = tmem + 128 * t;
-                if (first && ou[t] > 0 && !wait(&o_free[t], (ou[t] - 1) & 1)) return false;
-                if (!wait(&full[slot], (c / NS) & 1)) return false;
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    if (!wait(half ? &p_full[t] : &p_half[t], pp[t] & 1)) return false;
-                    tc_fence_after();
-                    if (leader) {
-#pragma unroll
-                        for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-                            umma_f16_ts(d, pa + 8 * kk, vd + kk * (32 * D >> 4), id_o, !(first && kk == 0));
-                    }
-                }
-                ++pp[t];
-                return true;
-            };
-            while (ok && it.next(p, r)) {
-                const int n = r.tb - r.ta;
-                if (r.b.nrows > 128) {
-                    // tile j: the values of j - 1 and the scores of j of each group in turn
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) ok = ok && wait(&q_full[t], qu[t]++ & 1);
-                    for (int j = 0; ok && j <= n; ++j) {
-                        const int ck = c0 + k_at(j), cv = c0 + v_at(j - 1, n);
-                        if (j < n) ok = wait(&full[ck % NS], (ck / NS) & 1);
-#pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-                            if (!ok) break;
-                            if (j > 0) {
-                                ok = value(t, cv, j == 1);
-                                if (!ok) break;
-                                if (j == n) commit(&o_full[t]);
-                            }
+#pragma unroll 1
+            for (int run = 0;; ++run) {
+                const int at = run % L::kRuns;
+                ok = wait(&run_full[at], run / L::kRuns);
+                if (!ok) break;
+                const int n = __shfl_sync(0xffffffffu, runs[at].n, 0);
+                const bool large = __shfl_sync(0xffffffffu, runs[at].nrows, 0) > 128;
+                if (leader) mbar_arrive(&run_free[at]);
+                if (n == 0) break;
+                // Large block: step j has the scores of tile j and the values of tile j - 1.  Small block:
+                // the scores of tile j and the values of j - 2, both of group j & 1; the other issuer only
+                // follows the ring's phases.
+                const int lag = large ? 1 : 2;
+                const bool used = large || t == 0 || n > 1;
+                qb = large ? 1 : (qb ^ 1);
+                const int qbuf = large ? t : qb;
+                ok = wait(&q_full[qbuf], qph >> qbuf);
+                const uint32_t other = qph >> (t ^ 1);  // large: phase of the other group's q
+                qph ^= large ? 3 : 1 << qbuf;
+                const uint64_t qd = q_desc + qbuf * (L::kQ >> 4);
+#pragma unroll 1
+                for (int j = 0; ok && j < n + lag; ++j) {
+                    const bool big = opaque(large);
+                    const bool own = big || (j & 1) == t;
+                    // ring order: K_j, V_j-1 (large), V_j-2, K_j (small)
+                    const bool has_k = j < n, has_v = j >= lag;
+                    int ks = 0, vs = 0;
+                    uint32_t kp = 0, vp = 0;
+                    auto take = [&](int &s, uint32_t &ph) {
+                        s = slot;
+                        ph = ring_ph;
+                        if (++slot == NS) {
+                            slot = 0;
+                            ring_ph ^= 1;
+                        }
+                    };
+                    if (big && has_k) take(ks, kp);
+                    if (has_v) take(vs, vp);
+                    if (!big && has_k) take(ks, kp);
+                    const uint64_t vd = v_desc + vs * (L::kSlot >> 4);
+                    const uint64_t kd = k_desc + ks * (L::kSlot >> 4);
+                    // Between the last probabilities and the next scores' issue a row group waits, so what
+                    // can be done before or after is.  (A small block's K comes last: its V slot is freed
+                    // without waiting for it.)
+                    if (big && has_k) ok = wait(&full[ks], kp);
+                    if (has_v) {
+                        ok = ok && wait(&full[vs], vp);
+                        if (own) {
+                            const bool first = j - lag < (big ? 1 : 2);
+                            if (first && ou > 0) ok = ok && wait(&o_free[t], ou - 1);
+                            ok = ok && wait(&p_full[t], pp);
                             tc_fence_after();
-                            if (j < n) score(t, t, ck);
-                        }
-                        if (!ok) break;
-                        if (j > 0) commit(&empty[cv % NS]);
-                        if (j < n) commit(&empty[ck % NS]);
-                    }
-                    ++ou[0];
-                    ++ou[1];
-                    qb = 1;
-                } else {
-                    // tile j belongs to group j & 1: its scores follow the values of j - 2
-                    qb ^= 1;
-                    ok = qb ? wait(&q_full[1], qu[1]++ & 1) : wait(&q_full[0], qu[0]++ & 1);
-                    for (int j0 = 0; ok && j0 < n + 2; j0 += 2) {
+                            if (ok && leader) {
 #pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-                            const int j = j0 + t;
-                            if (!ok) break;
-                            if (j >= 2 && j - 2 < n) {
-                                const int cv = c0 + v_at(j - 2, n);
-                                ok = value(t, cv, j - 2 < 2);
-                                if (!ok) break;
-                                if (j >= n) commit(&o_full[t]);
-                                commit(&empty[cv % NS]);
+                                for (int kk = 0; kk < kTileTok / 16; ++kk)
+                                    umma_f16_ts(t_o, t_s + 8 * kk, vd + kk * (32 * D >> 4), id_o, !(first && kk == 0));
                             }
-                            if (j < n) {
-                                const int ck = c0 + k_at(j);
-                                ok = wait(&full[ck % NS], (ck / NS) & 1);
-                                if (!ok) break;
-                                tc_fence_after();
-                                score(t, qb, ck);
-                                commit(&empty[ck % NS]);
+                            pp ^= 1;
+                            if (!big && ok && leader) {  // both arrivals of the slot
+                                umma_commit(&empty[vs]);
+                                umma_commit(&empty[vs]);
                             }
                         }
                     }
-                    ++ou[0];
-                    if (n > 1) ++ou[1];
+                    if (!big && has_k) ok = ok && wait(&full[ks], kp);
+                    if (!ok) break;
+                    if (own) {
+                        if (has_k) {
+                            tc_fence_after();
+                            if (leader) {
+#pragma unroll
+                                for (int kk = 0; kk < D / 16; ++kk)
+                                    umma_f16(t_s, qd + (kk >> 2) * (16384 >> 4) + (kk & 3) * 2,
+                                             kd + (kk >> 2) * (1024 >> 4) + (kk & 3) * 2, id_s, kk > 0);
+                                umma_commit(&s_full[t]);
+                                umma_commit(&empty[ks]);
+                                if (!big) umma_commit(&empty[ks]);
+                                if (j + lag >= n) umma_commit(&q_free[qbuf]);  // the group's last scores
+                            }
+                            if (big && j + 1 == n) {
+                                // the other group's buffer waits for both issuers
+                                ok = wait(&q_full[t ^ 1], other);
+                                if (ok && leader) mbar_arrive(&q_free[t ^ 1]);
+                            }
+                        }
+                        if (has_v && leader) {
+                            if (big) umma_commit(&empty[vs]);
+                            if (j >= n) umma_commit(&o_full[t]);  // the group's last tile
+                        }
+                    }
                 }
-                c0 += 2 * n;
+                if (!ok) break;
+                if (used)
+                    ++ou;
+                else if (leader)
+                    mbar_arrive(&q_free[qbuf]);
             }
-            if (!ok && lane == 0) *abort = 1;
+            if (!ok && lane == 0) tile_give_up(abort);
             // every MMA issued has completed before tensor memory and shared memory go
             if (leader) {
-                umma_commit(drained);
-                mbar_wait(drained, 0);
+                umma_commit(&drained[t]);
+                mbar_wait(&drained[t], 0);
             }
             __syncwarp();
         }
     } else {
         // ===================================================================== row groups
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs));
-        RunIter it;
-        it.begin(p, blockIdx.x);
-        TileRun r;
+        const int G = a.num_q_heads / a.num_kv_heads;
+        const unsigned g_magic = div_magic(G);
         const int t = warp >> 2;           // group
         const int row = tid & 127;         // row of the group = tensor-memory lane
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
         const uint32_t t_s = tmem + 128 * t + lanes, t_o = tmem + 256 + 128 * t + lanes;
-        const bool cap = a.soft_cap > 0.f, biased = a.slopes != nullptr;
-        const bool scaled = cap || biased || !(a.q_scale > 0.f);  // scores enter the exponent domain early
-        const float f = scaled ? 1.f : a.q_scale;
-        const float cap1 = cap ? 2.f * kLog2e * a.q_scale / a.soft_cap : 0.f, cap2 = a.soft_cap * kLog2e;
-        int c0 = 0, sn = 0;
-        int qb = 0;                        // small blocks: q buffer (0 behind a large block, then in turn)
+        int c0 = 0, sn = 0;                // ring position of the run's first K; this group's tiles so far
+        int qb = 1;                        // q buffer of the last small block; 1 after a large one
         int ou[2] = {0, 0};                // runs that used O of group 0, 1 so far
         int mln = 0;                       // small blocks of more than one tile so far
-        auto wait = [&](uint64_t *bar, int phase) { return tile_wait(bar, phase & 1, abort); };
+        int turns = 0;                     // tiles of large blocks so far
+        int fills[2] = {0, 0};             // of each q buffer so far, by either group
+        bool ok = true;
 
-        // 128 rows of q from row `first` of the run's block into buffer `buf`
-        auto fill = [&](const TileRun &u, int buf, int first) {
-            constexpr int CH = D / 8;  // 16-byte chunks of a row
-            const uint32_t dst = q_s + buf * L::kQ;
-            const int live = min(u.b.nrows - first, 128);
-#pragma unroll 8
-            for (int k = 0; k < CH; ++k) {
-                const int i = row + 128 * k, rr = i / CH, ch = i % CH;
-                if (rr >= live) continue;
-                const int rho = u.b.row0 + first + rr;
-                const long long tok = u.b.tok0 + rho / G;
-                const uint4 *src = reinterpret_cast<const uint4 *>(
-                    reinterpret_cast<const T *>(a.q) + (tok * a.num_q_heads + u.h * G + rho % G) * D);
-                sts_u4(dst + (ch >> 3) * 16384 + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4), __ldg(src + ch));
+        // The q of run `next`: of a large block group t fills buffer t, of a small one group 0 the buffer
+        // that the small block in front did not use.  A buffer is free once both issuers are through
+        // with its last contents.
+        auto fill_q = [&](int next) {
+            const int at = next % L::kRuns;
+            if (!(ok = wait(&run_full[at], next / L::kRuns))) return;
+            const RunDesc *d = &runs[at];
+            if (d->n == 0) return;
+            const bool large = d->nrows > 128;
+            const int buf = large ? t : qb ^ 1;
+            if (large || t == 0) {
+                const int before = buf ? fills[1] : fills[0];
+                if (before > 0 && !(ok = wait(&q_free[buf], before - 1))) return;
+                constexpr int CH = D / 8;  // 16-byte chunks of a row
+                const int first = large ? 128 * t : 0, live = min(d->nrows - first, 128), rho0 = d->row0 + first;
+                const T *q0 = reinterpret_cast<const T *>(a.q) + (static_cast<long long>(d->tok0) * a.num_q_heads + d->h * G) * D;
+                const uint32_t dst = smem_u32(tile_smem + L::q) + buf * L::kQ;
+                // a thread's chunks are one column of rows row / CH, + 128 / CH, ...; eight loads in flight
+                const int ch = row % CH;
+#pragma unroll 1
+                for (int k0 = 0; k0 < CH; k0 += 8) {
+                    const int r0 = row / CH + k0 * (128 / CH);
+                    if (r0 >= live) break;
+                    uint4 v[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int rho = rho0 + min(r0 + k * (128 / CH), live - 1), tok = fast_div(rho, G, g_magic);
+                        v[k] = __ldg(reinterpret_cast<const uint4 *>(
+                                         q0 + (static_cast<long long>(tok) * a.num_q_heads + (rho - tok * G)) * D) + ch);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int rr = r0 + k * (128 / CH);
+                        if (rr < live) sts_u4(dst + (ch >> 3) * 16384 + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4), v[k]);
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[buf]);
             }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full[buf]);
+            fills[0] += large || buf == 0;
+            fills[1] += large || buf == 1;
         };
 
-        // Bias, cap and mask of the tile at position t0: S becomes the score in the exponent domain
-        // (scaled), -inf outside columns [jlo, jhi).
-        auto rewrite = [&](int t0, int jlo, int jhi, bool masked, float slope, int pos) {
+        // The tile at position t0 of a row that a cap, a mask or a bias with two signs touches: S becomes
+        // the score in the exponent domain, -inf outside columns [jlo, jhi).
+        auto rewrite = [&](int t0, int jlo, int jhi, float slope, int pos) {
+            const bool cap = a.soft_cap > 0.f;
+            const float cap1 = cap ? 2.f * kLog2e * a.q_scale / a.soft_cap : 0.f, cap2 = a.soft_cap * kLog2e;
 #pragma unroll 1
-            for (int k = 0; k < 128; k += 32) {
-                float v[32];
-                tmem_ld<32>(t_s + k, v);
+            for (int k = 0; k < 128; k += 16) {
+                float v[16];
+                tmem_ld<16>(t_s + k, v);
                 tmem_wait_ld();
-                if (cap) {
+                if (opaque(cap)) {
                     // cap tanh(y) = cap - 2 cap / (1 + e^2y): absolute error about 2^-22 cap
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
+                    for (int i = 0; i < 16; ++i)
                         v[i] = fmaf(-2.f * cap2, __fdividef(1.f, 1.f + fast_exp2(v[i] * cap1)), cap2);
-                } else if (scaled) {
+                } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] *= a.q_scale;
+                    for (int i = 0; i < 16; ++i) v[i] *= a.q_scale;
                 }
-                if (biased) {
-                    const float d0 = static_cast<float>(t0 + k - pos);
+                const float d0 = static_cast<float>(t0 + k - pos);
+                uint32_t w[16];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = fmaf(-slope, fabsf(d0 + static_cast<float>(i)), v[i]);
+                for (int i = 0; i < 16; ++i) {
+                    const float x = fmaf(-slope, fabsf(d0 + static_cast<float>(i)), v[i]);
+                    w[i] = __float_as_uint((i >= jlo - k && i < jhi - k) ? x : -INFINITY);
                 }
-                if (masked) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = (i >= jlo - k && i < jhi - k) ? v[i] : -INFINITY;
-                }
-                tmem_st32(t_s + k, v);
+                tmem_st16(t_s + k, w);
             }
             tmem_wait_st();
         };
+        // One pass over the tile's scores: x = S f + c + se column - that is, scale, bias and reference
+        // in one or two operations -, P = 2^x packed into pk, its sum and the largest x.
+        uint32_t pk[64];
+        auto probs = [&](auto biased, float f, float c, float se, float &sum, float &top) {
+            constexpr bool BIAS = decltype(biased)::value;
+            const float2 ff = make_float2(f, f), step = make_float2(2.f * se, 2.f * se);
+            float2 acc = make_float2(0.f, 0.f);
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float v[2][32];
+            tmem_ld<32>(t_s, v[0]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float2 cc = make_float2(c, c);
+                if constexpr (BIAS) cc = make_float2(fmaf(se, 32.f * k, c), fmaf(se, 32.f * k + 1.f, c));
+                tmem_wait_ld();
+                if (k < 3) tmem_ld<32>(t_s + 32 * k + 32, v[(k + 1) & 1]);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float2 x = fma2(make_float2(v[k & 1][2 * i], v[k & 1][2 * i + 1]), ff, cc);
+                    if constexpr (BIAS) cc = add2(cc, step);
+                    mx[i & 3] = fmaxf(mx[i & 3], fmaxf(x.x, x.y));
+                    x.x = fast_exp2(x.x);
+                    x.y = fast_exp2(x.y);
+                    acc = add2(acc, x);
+                    pk[16 * k + i] = pack2<T>(x.x, x.y);
+                }
+            }
+            sum = acc.x + acc.y;
+            top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        };
 
-        bool ok = true;
-        bool have = it.next(p, r);
-        if (have) {
-            if (r.b.nrows > 128)
-                fill(r, t, 128 * t);
-            else if (t == 0)
-                fill(r, 0, 0);
-        }
-        while (have) {
-            const int n = r.tb - r.ta;
-            const bool big = r.b.nrows > 128;
-            TileRun u = r;  // the next run
-            const bool more = it.next(p, u);
-            const bool ubig = more && u.b.nrows > 128;
-            const int qn = big ? 0 : (qb ^ 1);
+#pragma unroll 1
+        for (int run = -1;; ++run) {  // -1: only fetches the first run's q
+            RunDesc d{};
+            if (run >= 0) {
+                const int at = run % L::kRuns;
+                if (!(ok = wait(&run_full[at], run / L::kRuns))) break;
+                d = runs[at];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&run_free[at]);
+                if (d.n == 0) break;
+            }
+            const int n = d.n;
+            const bool big = d.nrows > 128;
+            if (run >= 0) qb = big ? 1 : qb ^ 1;
             const int ri = big ? 128 * t + row : row;  // row of the block
-            const bool live = ri < r.b.nrows;
+            const bool live = ri < d.nrows;
             // the row's query, its positions [lo, hi) and its bias
             long long out_row = 0;
             int lo = 0, hi = 0, pos = 0;
             float slope = 0.f;
             if (live) {
-                const int rho = r.b.row0 + ri, i = rho / G, head = r.h * G + rho % G;
-                out_row = static_cast<long long>(r.b.tok0 + i) * a.num_q_heads + head;
-                lo = r.b.lo;
-                hi = r.b.hi;
-                if (r.b.kind == kOwn) {
-                    int q0, nq;
-                    seq_rows(a, r.b.tab, q0, nq);
-                    pos = r.b.len - nq + i;
-                    row_range(a, r.b.tab, q0 + i, pos, r.b.len, lo, hi);
-                    if (biased) slope = a.slopes[head] * kLog2e;
+                const int rho = d.row0 + ri, i = fast_div(rho, G, g_magic), head = d.h * G + (rho - i * G);
+                out_row = static_cast<long long>(d.tok0 + i) * a.num_q_heads + head;
+                lo = d.lo;
+                hi = d.hi;
+                if ((d.flags & 3) == kOwn) {
+                    pos = d.pos0 + i;
+                    row_range(a, d.tab, d.tok0 + i, pos, d.len, lo, hi);
+                    if (a.slopes) slope = a.slopes[head] * kLog2e;
                 }
             }
             const bool warp_live = __any_sync(0xffffffffu, live);
-            const int tile0 = r.b.lo / kTileTok + r.ta;
             float m = -INFINITY, l = 0.f;
-
-            for (int j = big ? 0 : t; j < n; j += big ? 1 : 2) {
-                const int t0 = (tile0 + j) * kTileTok;
+            const int j0 = big ? 0 : t, dj = big ? 1 : 2;
+#pragma unroll 1
+            for (int j = j0; j < n; j += dj) {
+                const int t0 = (d.tile0 - j) * kTileTok;
                 const int jlo = lo - t0, jhi = hi - t0;  // visible columns [jlo, jhi)
                 ok = wait(&s_full[t], sn++);
                 if (!ok) break;
                 tc_fence_after();
                 // V rows that no row of the block attends are cleared (a zero probability does not
-                // cancel a NaN): by group 0 for both groups, or by the tile's own group
-                const int vlo = r.b.lo - t0, vhi = r.b.hi - t0;
-                if ((vlo > 0 || vhi < kTileTok) && (t == 0 || !big)) {
+                // cancel a NaN), by each group that uses the tile
+                const int vlo = d.lo - t0, vhi = d.hi - t0;
+                if (__builtin_expect(vlo > 0 || vhi < kTileTok, 0)) {
                     const int cv = c0 + v_at(j, n);
                     ok = wait(&full[cv % NS], cv / NS);
                     if (!ok) break;
@@ -800,116 +930,84 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         if (tok < vlo || tok >= vhi) sts_u4(vt + kv_chunk_off<D>(tok, i % (D / 8)), make_uint4(0, 0, 0, 0));
                     }
                     fence_proxy_async_smem();
+                    __syncwarp();
                 }
-                // Short loops: the code of a tile has to fit the instruction cache closest to the warp
-                // (fully unrolled over the 128 columns it ran a third slower).
-                float ref = 0.f;
-                if (warp_live) {
-                    // bias, cap and mask, where a tile has any: the scores are rewritten in place
-                    const bool masked = __any_sync(0xffffffffu, live && (jlo > 0 || jhi < kTileTok));
-                    if (scaled || masked) rewrite(t0, jlo, jhi, masked, slope, pos);
-                    // pass 1: the row's largest score
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    float va[16], vb[16];
-                    auto largest = [&](const float (&v)[16]) {
-#pragma unroll
-                        for (int i = 0; i < 16; i += 8)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(v[i + e], v[i + e + 4]));
-                    };
-                    tmem_ld<16>(t_s, va);
-#pragma unroll 1
-                    for (int k = 0; k < 128; k += 32) {
-                        tmem_wait_ld();
-                        tmem_ld<16>(t_s + k + 16, vb);
-                        largest(va);
-                        tmem_wait_ld();
-                        tmem_ld<16>(t_s + (k + 32 & 127), va);  // the last one reads the first columns for pass 2
-                        largest(vb);
+                // Large blocks: the two groups' warps on one SM sub-partition take turns, so that one's
+                // exponentials run under the other's products.  Left alone most CTAs fell into step:
+                // both computed, then both waited.
+                if (opaque(big)) {
+                    if (turns + t > 0) ok = wait(&turn[4 * t + (warp & 3)], turns + t - 1);
+                    if (!ok) break;
+                    ++turns;
+                }
+                if (opaque(warp_live)) {
+                    // The bias is linear in the column where the row's visible columns lie on one side of its
+                    // own position.
+                    const bool behind = jhi <= pos + 1 - t0, ahead = jlo >= pos - t0;
+                    const bool odd = live && (jlo > 0 || jhi < kTileTok || (slope != 0.f && !behind && !ahead));
+                    const bool special = __any_sync(0xffffffffu, odd) || a.soft_cap > 0.f;
+                    float f = a.q_scale, se = behind ? slope : -slope;
+                    if (__builtin_expect(special, 0)) {
+                        rewrite(t0, jlo, jhi, slope, pos);
+                        f = 1.f;
+                        se = 0.f;
                     }
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
-                    const bool move = live && (m == -INFINITY ? top > -INFINITY : top > m + kLazyMax);
-                    if (__any_sync(0xffffffffu, move)) {
-                        const float mn = move ? top : m;
+                    const float base = se * static_cast<float>(t0 - pos);
+                    float sum, top;
+#pragma unroll 1
+                    for (;;) {
+                        // P against the row's reference; where a score passes it by more than 2^kLazyMax (or
+                        // the row has none yet) the reference moves, O follows, and the pass is repeated
+                        const float c = base - (m == -INFINITY ? 0.f : m);
+                        if (a.slopes)
+                            probs(std::true_type{}, f, c, se, sum, top);
+                        else
+                            probs(std::false_type{}, f, c, se, sum, top);
+                        const bool move = live && (m == -INFINITY ? top > -INFINITY : top > kLazyMax);
+                        if (__builtin_expect(!__any_sync(0xffffffffu, move), 1)) break;
+                        const float mn = !move ? m : m == -INFINITY ? top : m + top;
                         const float alpha = (mn == m || m == -INFINITY) ? 1.f : fast_exp2(m - mn);
                         m = mn;
                         l *= alpha;
                         // the scores' commit covers the group's earlier value MMAs: O is at rest
                         if (__any_sync(0xffffffffu, alpha != 1.f)) {
-                            tmem_wait_ld();
 #pragma unroll 1
-                            for (int k = 0; k < D / 32; ++k) {
-                                float o[32];
-                                tmem_ld<32>(t_o + 32 * k, o);
+                            for (int k = 0; k < D; k += 16) {
+                                float o[16];
+                                tmem_ld<16>(t_o + k, o);
                                 tmem_wait_ld();
+                                uint32_t w[16];
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) o[i] *= alpha;
-                                tmem_st32(t_o + 32 * k, o);
+                                for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(o[i] * alpha);
+                                tmem_st16(t_o + k, w);
                             }
                         }
                     }
-                    ref = m == -INFINITY ? 0.f : m;
-                    // pass 2: P = 2^(x - m) over the columns read already, and its sum; the value MMA of
-                    // the first 64 positions starts while the others are computed
-                    float2 sum = make_float2(0.f, 0.f);
-                    const float2 ff = make_float2(f, f), rr = make_float2(-ref, -ref);
-                    auto probs = [&](const float (&v)[16], uint32_t (&pk)[16], int at) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            float2 x = fma2(make_float2(v[2 * i], v[2 * i + 1]), ff, rr);
-                            x.x = fast_exp2(x.x);
-                            x.y = fast_exp2(x.y);
-                            sum = add2(sum, x);
-                            pk[at + i] = pack2<T>(x.x, x.y);
-                        }
-                    };
-#pragma unroll 1
-                    for (int k = 0; k < 128; k += 32) {
-                        uint32_t pk[16];
-                        tmem_wait_ld();
-                        tmem_ld<16>(t_s + k + 16, vb);
-                        probs(va, pk, 0);
-                        tmem_wait_ld();
-                        if (k < 96) tmem_ld<16>(t_s + k + 32, va);
-                        probs(vb, pk, 8);
-                        tmem_st16(t_s + (k >> 1), pk);
-                        if (k == 32) {
-                            tmem_wait_st();
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&p_half[t]);
-                        }
-                    }
+                    l += sum;
+                    if (opaque(big) && lane == 0) mbar_arrive(&turn[4 * (t ^ 1) + (warp & 3)]);
+                    tmem_st32(t_s, reinterpret_cast<const float *>(pk));
+                    tmem_st32(t_s + 32, reinterpret_cast<const float *>(pk + 32));
                     tmem_wait_st();
-                    l += sum.x + sum.y;
-                } else if (lane == 0) {
-                    mbar_arrive(&p_half[t]);
+                } else if (opaque(big) && lane == 0) {
+                    mbar_arrive(&turn[4 * (t ^ 1) + (warp & 3)]);
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[t]);
-                // this tile's scores came behind every score of the run in front: its q buffer is free
-                if (j == 0 && t == 0 && more && !big && !ubig) fill(u, qn, 0);
             }
             if (!ok) break;
-
-            // The next run's q.  Behind a small run, both groups read one buffer: a large run's fills
-            // wait for the end (`late`), a small one's took the other buffer after the first tile.
-            const bool late = !big && ubig;
-            if (more && big) {
-                if (ubig)
-                    fill(u, t, 128 * t);
-                else if (t == 0)
-                    fill(u, 0, 0);
-            }
+            fill_q(run + 1);  // the next run's q, under this run's last products
+            if (!ok) break;
+            if (run < 0) continue;
 
             // ------------------------------------------------ end of the run
-            const bool whole = r.ta == 0 && r.tb == r.n;
             const bool two = !big && n > 1;  // both groups hold a part of each row
             if (two && t == 1) {
-                float *ml = sm_ml + (mln & 1) * 256;  // group 0 of the run before the last has read it
-                ml[row] = m;
-                ml[128 + row] = l;
+                // group 0 has read what was there before (it freed O of group 1 behind that)
+                if (ou[1] > 0) ok = wait(&o_free[1], ou[1] - 1);
+                if (!ok) break;
+                sm_ml[row] = m;
+                sm_ml[128 + row] = l;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(ml_full);
             }
@@ -917,10 +1015,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 ok = wait(&o_full[t], ou[t]);
                 float fa = 1.f, fb = 0.f;
                 if (ok && two) {
-                    ok = wait(&o_full[1], ou[1]) && wait(ml_full, mln);
+                    // group 1's (m, l) first: by then it is through with its part of the runs in front, so
+                    // that the phase of o_full[1] waited for next is this run's
+                    ok = wait(ml_full, mln) && wait(&o_full[1], ou[1]);
                     if (ok) {
-                        const float *ml = sm_ml + (mln & 1) * 256;
-                        const float mb = ml[row], lb = ml[128 + row];
+                        const float mb = sm_ml[row], lb = sm_ml[128 + row];
                         const float mm = fmaxf(m, mb);
                         fa = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : fast_exp2(m - mm);
                         fb = mb == -INFINITY ? (lb == 0.f ? 0.f : 1.f) : fast_exp2(mb - mm);
@@ -932,49 +1031,47 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 tc_fence_after();
                 if (warp_live) {
                     const float inv = l == 0.f ? 0.f : 1.f / l;  // a NaN stays one
-                    const bool direct = whole && r.b.kind == kOwn;
+                    const bool whole = d.flags & 4, direct = whole && (d.flags & 3) == kOwn;
                     // where a partial state goes: the CTA's slot, or the row's place of a whole unit
                     float *st_o = nullptr;
                     if (!direct && live) {
                         if (whole) {
-                            const long long at = (r.b.kind == kSuffix ? static_cast<long long>(a.total_q) * a.num_q_heads : 0) + out_row;
-                            p.ml[at] = make_float2(m, l);
-                            st_o = p.acc + at * D;
+                            const long long to = ((d.flags & 3) == kSuffix ? static_cast<long long>(a.total_q) * a.num_q_heads : 0) + out_row;
+                            p.ml[to] = make_float2(m, l);
+                            st_o = p.acc + to * D;
                         } else {
-                            float *slot = p.slots + (static_cast<size_t>(blockIdx.x) * 2 + (r.ta == 0 ? 1 : 0)) * (kBlkRows * (D + 2));
-                            slot[ri] = m;
-                            slot[kBlkRows + ri] = l;
-                            st_o = slot + 2 * kBlkRows + ri * D;
+                            float *ps = p.slots + (static_cast<size_t>(blockIdx.x) * 2 + (d.flags >> 3 & 1)) * (kBlkRows * (D + 2));
+                            ps[ri] = m;
+                            ps[kBlkRows + ri] = l;
+                            st_o = ps + 2 * kBlkRows + ri * D;
                         }
                     }
+                    T *out = reinterpret_cast<T *>(a.out) + out_row * D;
                     __syncwarp();
 #pragma unroll 1
-                    for (int k = 0; k < D / 32; ++k) {
-                        float o[32];
-                        tmem_ld<32>(t_o + 32 * k, o);
-                        if (two) {
-                            float ob[32];
-                            tmem_ld<32>(t_o + 128 + 32 * k, ob);
+                    for (int k = 0; k < D; k += 16) {
+                        float o[16];
+                        tmem_ld<16>(t_o + k, o);
+                        if (opaque(two)) {
+                            float ob[16];
+                            tmem_ld<16>(t_o + 128 + k, ob);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = fmaf(o[i], fa, ob[i] * fb);
+                            for (int i = 0; i < 16; ++i) o[i] = fmaf(o[i], fa, ob[i] * fb);
                         } else {
                             tmem_wait_ld();
                         }
-                        if (live && direct) {
-                            uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + out_row * D + 32 * k);
+                        if (opaque(live && direct)) {
+                            uint32_t w[8];
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                uint32_t w[4];
+                            for (int e = 0; e < 8; ++e) w[e] = l == 0.f ? 0u : pack2<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
+                            uint4 *dst = reinterpret_cast<uint4 *>(out + k);
+                            dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                            dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                        } else if (opaque(live)) {
+                            float4 *dst = reinterpret_cast<float4 *>(st_o + k);
 #pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    w[e] = l == 0.f ? 0u : pack2<T>(o[8 * q + 2 * e] * inv, o[8 * q + 2 * e + 1] * inv);
-                                dst[q] = make_uint4(w[0], w[1], w[2], w[3]);
-                            }
-                        } else if (live) {
-                            float4 *dst = reinterpret_cast<float4 *>(st_o + 32 * k);
-#pragma unroll
-                            for (int q = 0; q < 8; ++q) dst[q] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+                            for (int q = 0; q < 4; ++q) dst[q] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
                         }
                         __syncwarp();  // the next tensor-memory load is the whole warp's
                     }
@@ -986,24 +1083,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     if (two) mbar_arrive(&o_free[1]);
                 }
             }
-            if (more && late) {
-                if (t == 1) {
-                    // every score MMA of this run is done
-                    ok = wait(&o_full[0], ou[0]);
-                    if (ok && two) ok = wait(&o_full[1], ou[1]);
-                    if (!ok) break;
-                }
-                fill(u, t, 128 * t);
-            }
             if (two) ++mln;
             ++ou[0];
             if (big || two) ++ou[1];
             c0 += 2 * n;
-            qb = qn;
-            r = u;
-            have = more;
         }
-        if (!ok && lane == 0) *abort = 1;
+        if (!ok && lane == 0) tile_give_up(abort);
     }
 
     // ---------------------------------------------------------------- teardown

@@ -157,7 +157,7 @@ int launch_tile(AttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
     p.entities = a.num_groups + a.num_seqs;
     const TileWs w = tile_ws(tile_entities(a.num_groups, a.num_seqs), tile_rows(a.total_q, G, shared),
                              static_cast<long long>(a.total_q) * a.num_q_heads, a.head_dim, shared);
-    if (w.max_blocks > (1LL << 30)) return fail(GOLLEK_ERR_UNSUPPORTED, "too many query rows for one call");
+    if (w.max_blocks > (1LL << 22)) return fail(GOLLEK_ERR_UNSUPPORTED, "too many query rows for one call");
     int dev = 0;
     GK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
     if (!ws) {
