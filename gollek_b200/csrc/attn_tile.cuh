@@ -56,6 +56,7 @@ struct __align__(16) TileBlk {
     int lo, hi, tab, len;
     int pos0, pad[3];
 };
+enum { kPlain = 0, kBias = 1, kCap = 2 };
 enum { kOwn = 0, kPrefix = 1, kSuffix = 2 };  // varlen; shared: the group's prefix, a sequence's own tokens
 
 struct PlanHead {
@@ -411,6 +412,14 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
         : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)), "l"(reinterpret_cast<uint64_t &>(c)));
     return d;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t &>(d))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return d;
+}
+__device__ __forceinline__ float2 pair(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 d;
     asm("add.rn.f32x2 %0, %1, %2;"
@@ -453,7 +462,10 @@ struct PageLoc {
 
 __device__ __forceinline__ int v_at(int j, int n) { return j == n - 1 ? 2 * n - 1 : 2 * j + 2; }
 
-template <typename T, int D>
+// FEAT: what is done to the scores besides scale and mask (kPlain, kBias: distance bias,
+// kCap: soft-cap, with or without bias); separate kernels, so that each one's code stays
+// short.
+template <typename T, int D, int FEAT>
 __global__ void __launch_bounds__(kTileThreads, 1)
     attn_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const TileArgs p) {
     using L = TileSmem<D>;
@@ -659,8 +671,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 if (leader) mbar_arrive(&run_free[at]);
                 if (n == 0) break;
                 // Large block: step j has the scores of tile j and the values of tile j - 1.  Small block:
-                // the scores of tile j and the values of j - 2, both of group j & 1; the other issuer only
-                // follows the ring's phases.
+                // the scores of tile j and the values of j - 2, both of group j & 1.  The other issuer follows
+                // the ring and frees the slots too: left out, it could fall behind by more than a turn of
+                // the ring (runs of one tile need it for nothing) and take one phase for another.
                 const int lag = large ? 1 : 2;
                 const bool used = large || t == 0 || n > 1;
                 qb = large ? 1 : (qb ^ 1);
@@ -707,10 +720,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                     umma_f16_ts(t_o, t_s + 8 * kk, vd + kk * (32 * D >> 4), id_o, !(first && kk == 0));
                             }
                             pp ^= 1;
-                            if (!big && ok && leader) {  // both arrivals of the slot
-                                umma_commit(&empty[vs]);
-                                umma_commit(&empty[vs]);
-                            }
+                            if (!big && ok && leader) umma_commit(&empty[vs]);
+                        } else if (ok && leader) {
+                            mbar_arrive(&empty[vs]);
                         }
                     }
                     if (!big && has_k) ok = ok && wait(&full[ks], kp);
@@ -725,7 +737,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                              kd + (kk >> 2) * (1024 >> 4) + (kk & 3) * 2, id_s, kk > 0);
                                 umma_commit(&s_full[t]);
                                 umma_commit(&empty[ks]);
-                                if (!big) umma_commit(&empty[ks]);
                                 if (j + lag >= n) umma_commit(&q_free[qbuf]);  // the group's last scores
                             }
                             if (big && j + 1 == n) {
@@ -738,6 +749,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                             if (big) umma_commit(&empty[vs]);
                             if (j >= n) umma_commit(&o_full[t]);  // the group's last tile
                         }
+                    } else if (has_k && leader) {
+                        mbar_arrive(&empty[ks]);
                     }
                 }
                 if (!ok) break;
@@ -768,26 +781,26 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         int ou[2] = {0, 0};                // runs that used O of group 0, 1 so far
         int mln = 0;                       // small blocks of more than one tile so far
         int turns = 0;                     // tiles of large blocks so far
-        int fills[2] = {0, 0};             // of each q buffer so far, by either group
+        int fills = 0;                     // of this group's q buffer so far
         bool ok = true;
 
-        // The q of run `next`: of a large block group t fills buffer t, of a small one group 0 the buffer
-        // that the small block in front did not use.  A buffer is free once both issuers are through
-        // with its last contents.
+        // The q of run `next`: group t fills buffer t, with its own rows of a large block, or with those of
+        // a small one whose turn that buffer is.  A buffer is free once both issuers are through with
+        // its last contents; its own group alone waits for that, every time, so that no phase is
+        // mistaken for another.
         auto fill_q = [&](int next) {
             const int at = next % L::kRuns;
             if (!(ok = wait(&run_full[at], next / L::kRuns))) return;
             const RunDesc *d = &runs[at];
             if (d->n == 0) return;
             const bool large = d->nrows > 128;
-            const int buf = large ? t : qb ^ 1;
-            if (large || t == 0) {
-                const int before = buf ? fills[1] : fills[0];
-                if (before > 0 && !(ok = wait(&q_free[buf], before - 1))) return;
+            if (large || t == (qb ^ 1)) {
+                if (fills > 0 && !(ok = wait(&q_free[t], fills - 1))) return;
+                ++fills;
                 constexpr int CH = D / 8;  // 16-byte chunks of a row
                 const int first = large ? 128 * t : 0, live = min(d->nrows - first, 128), rho0 = d->row0 + first;
                 const T *q0 = reinterpret_cast<const T *>(a.q) + (static_cast<long long>(d->tok0) * a.num_q_heads + d->h * G) * D;
-                const uint32_t dst = smem_u32(tile_smem + L::q) + buf * L::kQ;
+                const uint32_t dst = smem_u32(tile_smem + L::q) + t * L::kQ;
                 // a thread's chunks are one column of rows row / CH, + 128 / CH, ...; eight loads in flight
                 const int ch = row % CH;
 #pragma unroll 1
@@ -809,62 +822,77 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full[buf]);
+                if (lane == 0) mbar_arrive(&q_full[t]);
             }
-            fills[0] += large || buf == 0;
-            fills[1] += large || buf == 1;
         };
 
-        // The tile at position t0 of a row that a cap, a mask or a bias with two signs touches: S becomes
-        // the score in the exponent domain, -inf outside columns [jlo, jhi).
-        auto rewrite = [&](int t0, int jlo, int jhi, float slope, int pos) {
-            const bool cap = a.soft_cap > 0.f;
-            const float cap1 = cap ? 2.f * kLog2e * a.q_scale / a.soft_cap : 0.f, cap2 = a.soft_cap * kLog2e;
-#pragma unroll 1
-            for (int k = 0; k < 128; k += 16) {
-                float v[16];
-                tmem_ld<16>(t_s + k, v);
-                tmem_wait_ld();
-                if (opaque(cap)) {
-                    // cap tanh(y) = cap - 2 cap / (1 + e^2y): absolute error about 2^-22 cap
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        v[i] = fmaf(-2.f * cap2, __fdividef(1.f, 1.f + fast_exp2(v[i] * cap1)), cap2);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) v[i] *= a.q_scale;
-                }
-                const float d0 = static_cast<float>(t0 + k - pos);
-                uint32_t w[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float x = fmaf(-slope, fabsf(d0 + static_cast<float>(i)), v[i]);
-                    w[i] = __float_as_uint((i >= jlo - k && i < jhi - k) ? x : -INFINITY);
-                }
-                tmem_st16(t_s + k, w);
-            }
-            tmem_wait_st();
-        };
-        // One pass over the tile's scores: x = S f + c + se column - that is, scale, bias and reference
-        // in one or two operations -, P = 2^x packed into pk, its sum and the largest x.
+        // One pass over a tile's scores: x, the score in the exponent domain less the row's reference,
+        // P = 2^x packed into pk, its sum and the largest x.  GEN false: every column is visible and the
+        // bias is linear in the column (se of either sign; c = bias at column 0 - reference).  GEN true:
+        // -inf outside columns [jlo, jhi), bias -se |d0 + column| (c = -reference).
         uint32_t pk[64];
-        auto probs = [&](auto biased, float f, float c, float se, float &sum, float &top) {
-            constexpr bool BIAS = decltype(biased)::value;
-            const float2 ff = make_float2(f, f), step = make_float2(2.f * se, 2.f * se);
+        const float cap1 = FEAT == kCap ? a.q_scale / a.soft_cap : 0.f, cap2 = a.soft_cap * kLog2e;
+        auto probs = [&](auto general, float c, float se, float d0, int jlo, int jhi, float &sum, float &top) {
+            constexpr bool GEN = decltype(general)::value;
+            const float2 ff = make_float2(a.q_scale, a.q_scale), step = make_float2(2.f * se, 2.f * se);
             float2 acc = make_float2(0.f, 0.f);
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
             float v[2][32];
             tmem_ld<32>(t_s, v[0]);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                float2 cc = make_float2(c, c);
-                if constexpr (BIAS) cc = make_float2(fmaf(se, 32.f * k, c), fmaf(se, 32.f * k + 1.f, c));
+                float(&w)[32] = v[k & 1];
+                [[maybe_unused]] float2 cc = make_float2(c, c);
+                if constexpr (FEAT != kPlain && !GEN) cc = make_float2(fmaf(se, 32.f * k, c), fmaf(se, 32.f * k + 1.f, c));
+                [[maybe_unused]] unsigned seen = ~0u;
+                if constexpr (GEN) {
+                    const int l0 = jlo - 32 * k, h0 = jhi - 32 * k;
+                    seen = h0 >= 32 ? ~0u : h0 <= 0 ? 0u : (1u << h0) - 1;
+                    if (l0 > 0) seen = l0 >= 32 ? 0u : seen & (~0u << l0);
+                }
                 tmem_wait_ld();
                 if (k < 3) tmem_ld<32>(t_s + 32 * k + 32, v[(k + 1) & 1]);
+                if constexpr (FEAT == kCap) {
+                    // cap tanh(y), y = score / cap: on the FMA pipe where |y| <= 1/2 in the whole warp
+                    // (the usual case: caps are several times the scores), an odd polynomial of relative
+                    // error below 2^-22; else cap - 2 cap / (1 + e^2y), two exponent-pipe operations
+                    float big_y = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float2 y = mul2(make_float2(w[2 * i], w[2 * i + 1]), make_float2(cap1, cap1));
+                        w[2 * i] = y.x;
+                        w[2 * i + 1] = y.y;
+                        big_y = fmaxf(big_y, fmaxf(fabsf(y.x), fabsf(y.y)));
+                    }
+                    if (__any_sync(0xffffffffu, !(big_y <= 0.5f))) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            w[i] = fmaf(-2.f, __fdividef(1.f, 1.f + fast_exp2(w[i] * (2.f * kLog2e))), 1.f);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float2 y = make_float2(w[2 * i], w[2 * i + 1]), y2 = mul2(y, y);
+                            float2 q = fma2(y2, pair(0.01724149100482f), pair(-0.05304549261928f));
+                            q = fma2(q, y2, pair(0.13325878977776f));
+                            q = fma2(q, y2, pair(-0.33333143591881f));
+                            q = fma2(mul2(q, y2), y, y);
+                            w[2 * i] = q.x;
+                            w[2 * i + 1] = q.y;
+                        }
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    float2 x = fma2(make_float2(v[k & 1][2 * i], v[k & 1][2 * i + 1]), ff, cc);
-                    if constexpr (BIAS) cc = add2(cc, step);
+                    if constexpr (FEAT != kPlain && GEN) {
+                        const float col = static_cast<float>(32 * k + 2 * i);
+                        cc = make_float2(fmaf(-se, fabsf(d0 + col), c), fmaf(-se, fabsf(d0 + (col + 1.f)), c));
+                    }
+                    float2 x = fma2(make_float2(w[2 * i], w[2 * i + 1]), FEAT == kCap ? make_float2(cap2, cap2) : ff, cc);
+                    if constexpr (FEAT != kPlain && !GEN) cc = add2(cc, step);
+                    if constexpr (GEN) {
+                        x.x = (seen >> (2 * i) & 1) ? x.x : -INFINITY;
+                        x.y = (seen >> (2 * i + 1) & 1) ? x.y : -INFINITY;
+                    }
                     mx[i & 3] = fmaxf(mx[i & 3], fmaxf(x.x, x.y));
                     x.x = fast_exp2(x.x);
                     x.y = fast_exp2(x.y);
@@ -904,7 +932,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 if ((d.flags & 3) == kOwn) {
                     pos = d.pos0 + i;
                     row_range(a, d.tab, d.tok0 + i, pos, d.len, lo, hi);
-                    if (a.slopes) slope = a.slopes[head] * kLog2e;
+                    if (FEAT != kPlain && a.slopes) slope = a.slopes[head] * kLog2e;
                 }
             }
             const bool warp_live = __any_sync(0xffffffffu, live);
@@ -944,27 +972,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     // The bias is linear in the column where the row's visible columns lie on one side of its
                     // own position.
                     const bool behind = jhi <= pos + 1 - t0, ahead = jlo >= pos - t0;
-                    const bool odd = live && (jlo > 0 || jhi < kTileTok || (slope != 0.f && !behind && !ahead));
-                    const bool special = __any_sync(0xffffffffu, odd) || a.soft_cap > 0.f;
-                    float f = a.q_scale, se = behind ? slope : -slope;
-                    if (__builtin_expect(special, 0)) {
-                        rewrite(t0, jlo, jhi, slope, pos);
-                        f = 1.f;
-                        se = 0.f;
-                    }
-                    const float base = se * static_cast<float>(t0 - pos);
+                    const bool general = __any_sync(0xffffffffu, live && (jlo > 0 || jhi < kTileTok ||
+                                                                          (FEAT != kPlain && slope != 0.f && !behind && !ahead)));
+                    const float d0 = static_cast<float>(t0 - pos), se = general || behind ? slope : -slope;
+                    const float base = FEAT != kPlain && !general ? se * d0 : 0.f;
                     float sum, top;
 #pragma unroll 1
-                    for (;;) {
+                    for (int tries = 0;; ++tries) {
                         // P against the row's reference; where a score passes it by more than 2^kLazyMax (or
                         // the row has none yet) the reference moves, O follows, and the pass is repeated
+                        // (twice at most: a reference so large that its own rounding exceeds 2^kLazyMax, some
+                        // 10^8, might never settle)
                         const float c = base - (m == -INFINITY ? 0.f : m);
-                        if (a.slopes)
-                            probs(std::true_type{}, f, c, se, sum, top);
+                        if (general)
+                            probs(std::true_type{}, c, se, d0, jlo, jhi, sum, top);
                         else
-                            probs(std::false_type{}, f, c, se, sum, top);
+                            probs(std::false_type{}, c, se, d0, jlo, jhi, sum, top);
                         const bool move = live && (m == -INFINITY ? top > -INFINITY : top > kLazyMax);
-                        if (__builtin_expect(!__any_sync(0xffffffffu, move), 1)) break;
+                        if (__builtin_expect(tries == 2 || !__any_sync(0xffffffffu, move), 1)) break;
                         const float mn = !move ? m : m == -INFINITY ? top : m + top;
                         const float alpha = (mn == m || m == -INFINITY) ? 1.f : fast_exp2(m - mn);
                         m = mn;
@@ -1049,29 +1074,32 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     T *out = reinterpret_cast<T *>(a.out) + out_row * D;
                     __syncwarp();
 #pragma unroll 1
-                    for (int k = 0; k < D; k += 16) {
-                        float o[16];
-                        tmem_ld<16>(t_o + k, o);
+                    for (int k = 0; k < D; k += 32) {
+                        float o[32];
+                        tmem_ld<32>(t_o + k, o);
                         if (opaque(two)) {
-                            float ob[16];
-                            tmem_ld<16>(t_o + 128 + k, ob);
+                            float ob[32];
+                            tmem_ld<32>(t_o + 128 + k, ob);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = fmaf(o[i], fa, ob[i] * fb);
+                            for (int i = 0; i < 32; ++i) o[i] = fmaf(o[i], fa, ob[i] * fb);
                         } else {
                             tmem_wait_ld();
                         }
                         if (opaque(live && direct)) {
-                            uint32_t w[8];
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) w[e] = l == 0.f ? 0u : pack2<T>(o[2 * e] * inv, o[2 * e + 1] * inv);
                             uint4 *dst = reinterpret_cast<uint4 *>(out + k);
-                            dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                            dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    w[e] = l == 0.f ? 0u : pack2<T>(o[8 * q + 2 * e] * inv, o[8 * q + 2 * e + 1] * inv);
+                                dst[q] = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
                         } else if (opaque(live)) {
                             float4 *dst = reinterpret_cast<float4 *>(st_o + k);
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) dst[q] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+                            for (int q = 0; q < 8; ++q) dst[q] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
                         }
                         __syncwarp();  // the next tensor-memory load is the whole warp's
                     }

@@ -133,7 +133,9 @@ int launch_dependent(const void *fn, dim3 grid, int threads, size_t smem, cudaSt
 template <typename T, int D>
 int launch_tile_as(TileArgs &p, const CUtensorMap &tmk, const CUtensorMap &tmv, cudaStream_t st) {
     const AttnArgs &a = p.a;
-    const void *fn = reinterpret_cast<const void *>(&attn_tile_kernel<T, D>);
+    const void *fn = a.soft_cap > 0.f ? reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kCap>)
+                     : a.slopes       ? reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kBias>)
+                                      : reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kPlain>);
     GK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, TileSmem<D>::total), "cudaFuncSetAttribute");
     tile_plan_kernel<<<1, kPlanThreads, 0, st>>>(p);
     GK_CUDA(cudaGetLastError(), "tile_plan_kernel launch");

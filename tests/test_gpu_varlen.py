@@ -64,11 +64,13 @@ def run_varlen(dev, q, pool, tables, cu, ctx, qkind, out=None, **kw):
 
 
 def check_varlen(dev, case, qkind, **kw):
+    from gollek_b200 import ops
     q, pool, tables, cu, ctx = case
     scale = 1 / math.sqrt(q.shape[2])
     out = torch.full(q.shape, 7.0, dtype=DT[qkind], device=dev)
     got = run_varlen(dev, q, pool, tables, cu, ctx, qkind, out=out, **kw).double().cpu().numpy()
     want = R.varlen(q, pool, tables, cu, ctx, scale, **kw)
+    assert ops.device_status(dev.index or 0) == 0
     outside = np.isnan(want).any(axis=(1, 2))
     assert (got[outside] == 7.0).all(), "rows in no sequence were written"
     most = float(np.max(np.abs(kw["slopes"]))) * float(ctx.max()) if kw.get("slopes") is not None else 0.0
@@ -171,6 +173,19 @@ def test_long_contexts_split_over_the_gpu(cuda_device, ctx, new, kind, qkind):
     check_varlen(cuda_device, case, qkind, slopes=SLOPES(8) / 64)
 
 
+@pytest.mark.parametrize("hq,hkv,window,cap", [(32, 8, 1024, 30.0), (8, 8, 0, 0.0), (12, 4, 200, 0.0), (64, 2, 0, 4.0)])
+def test_large_and_small_blocks_in_turn(cuda_device, hq, hkv, window, cap):
+    """Blocks of more and of fewer than 128 rows, of many tiles and of one, behind one another in every order: what the
+    warps of a block hand each other may not be mistaken for the next block's."""
+    rng = np.random.default_rng(60)
+    for rep in range(3):
+        n = 24
+        ctx = np.where(rng.random(n) < 0.5, rng.integers(1, 128, n), rng.integers(128, 2000, n))
+        new = np.where(rng.random(n) < 0.5, 1, np.minimum(ctx, rng.integers(1, 300, n)))
+        case = varlen_case(ctx, new, hq, hkv, 128, 16, "bf16", "bf16", 61 + rep, window=window)
+        check_varlen(cuda_device, case, "bf16", window=window, cap=cap)
+
+
 def test_one_layer_of_a_pool(cuda_device):
     """page_stride: a layer of a [block][layer][...] pool, through a view of it."""
     from gollek_b200 import ops
@@ -236,10 +251,12 @@ def run_shared(dev, case, qkind, cap=0.0, **kw):
 
 
 def check_shared(dev, case, qkind, cap=0.0):
+    from gollek_b200 import ops
     q, pool, pt, plens, starts, t, ctx = case
     scale = 1 / math.sqrt(q.shape[2])
     got = run_shared(dev, case, qkind, cap).double().cpu().numpy()
     want = R.shared_prefix(q, pool, pt, plens, starts, t, ctx, scale, cap)
+    assert ops.device_status(dev.index or 0) == 0
     tol = R.bound(want, q, pool, scale, qkind, p_kind=None if qkind == "f32" else qkind, cap=cap)
     err = np.abs(got - want)
     assert np.isfinite(got).all()
