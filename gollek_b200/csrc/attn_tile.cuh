@@ -43,9 +43,11 @@ constexpr int kRunCostTiles = 2;      // start-up of a run (q, pipeline fill, ou
 constexpr int kMaxTileCtas = 160;
 constexpr int kTileThreads = 384;     // 8 row warps, 2 MMA issuers, 1 producer, 1 idle
 // Registers: launched with 168 a thread (384 x 168 = 64,512 of the SM's 65,536), of which the
-// third warpgroup gives the row groups 40 each: 2 x 208 + 88 = 3 x 168.  A row thread holds a
+// third warpgroup gives the row groups 32 each: 2 x 200 + 104 = 3 x 168.  A row thread holds a
 // tile's 128 scores; at 168 it would spill 560 bytes.
-constexpr int kRowRegs = 208, kAuxRegs = 88;
+constexpr int kRowRegs = 200, kAuxRegs = 104;
+// int8 caches: a fourth warpgroup converts; 512 threads launched with 128 registers.
+constexpr int kTileThreadsQ8 = 512, kAuxRegsQ8 = 56;
 constexpr float kLazyMax = 8.f;
 
 // A block: rows row0 .. row0 + nrows - 1 (row r: query token tok0 + r / G, q head h G + r % G)
@@ -345,18 +347,26 @@ struct RunIter {
 
 // ---------------------------------------------------------------------------- tile kernel
 
-template <int D>
+// Q8: int8 caches.  Their tiles land as bytes in a ring of their own, four converter warps
+// turn them into bf16 tiles (exact: integers below 2^8), and the scales, which enter the
+// scores and the probabilities, are kept by tile: with 3 + 3 slots the copies are never
+// more than 5 tiles ahead of a tile in use.
+template <int D, bool Q8>
 struct TileSmem {
     static constexpr uint32_t kSlot = kTileTok * D * 2;  // K or V of one tile
     static constexpr uint32_t kQ = 128 * D * 2;          // 128 rows
-    static constexpr int kSlots = D == 128 ? 5 : 10;
+    static constexpr int kSlots = (Q8 ? 3 : 5) * (128 / D);
+    static constexpr int kRaw = Q8 ? 3 * (128 / D) : 0;  // int8 tiles in flight
+    static constexpr int kScales = Q8 ? 8 * (128 / D) : 0;  // tiles whose scales are kept
     static constexpr int kRuns = 4;                        // run descriptors in flight
     static constexpr uint32_t q = 0;
     static constexpr uint32_t ring = 2 * kQ;
-    static constexpr uint32_t ml = ring + kSlots * kSlot;  // [2][128] floats
+    static constexpr uint32_t raw = ring + kSlots * kSlot;   // [kRaw][128][D] bytes
+    static constexpr uint32_t scales = raw + kRaw * (kSlot / 2);  // [kScales][K, V][128] floats
+    static constexpr uint32_t ml = scales + kScales * 1024;  // [2][128] floats
     static constexpr uint32_t runs = ml + 2 * 128 * 4;     // [kRuns] x 48 bytes
     static constexpr uint32_t bars = runs + kRuns * 48;
-    static constexpr int kBars = 2 * kSlots + 2 * kRuns + 2 * 7 + 8 + 1;
+    static constexpr int kBars = 2 * kSlots + 2 * kRaw + 2 * kRuns + 2 * 7 + 8 + 1;
     static constexpr uint32_t misc = bars + kBars * 8;
     static constexpr uint32_t total = misc + 16;
 };
@@ -436,6 +446,16 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
         "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc));
 }
 
+// Two bytes of w (SEL: a prmt selector that puts each below a byte of 0x43) as signed
+// integers in bf16.
+template <unsigned SEL>
+__device__ __forceinline__ uint32_t byte_pair(uint32_t w) {
+    const uint32_t x = __byte_perm(w, 0x43434343u, SEL);
+    uint32_t a = x & 0xFF7FFF7Fu, b = x & 0xFF80FF80u, d;
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
 // One lane of the converged warp, always the same.
 __device__ __forceinline__ bool elect_one() {
     uint32_t ok;
@@ -454,7 +474,13 @@ __device__ __forceinline__ uint32_t kv_chunk_off(int tok, int ch) {
 // Page lookups and TMA boxes of a run's tiles: lane g < 8 owns the 16 positions 16 g .. of
 // each tile (one box; two of 8 rows where pages hold 8).
 struct PageLoc {
-    int row0, row1;  // first pool row of the box / 8, or -1
+    int row0, row1;  // first pool row of the box (16-bit caches: / 8), or -1
+};
+// int8 caches: also the box's scales - where they are, or, one per page, what they are.
+struct PageLocQ8 {
+    int row0, row1;
+    long long sc0, sc1;
+    float ks0, vs0, ks1, vs1;
 };
 
 // Ring positions, from the run's first, of K and V of tile j of n: a value product follows
@@ -465,10 +491,10 @@ __device__ __forceinline__ int v_at(int j, int n) { return j == n - 1 ? 2 * n - 
 // FEAT: what is done to the scores besides scale and mask (kPlain, kBias: distance bias,
 // kCap: soft-cap, with or without bias); separate kernels, so that each one's code stays
 // short.
-template <typename T, int D, int FEAT>
-__global__ void __launch_bounds__(kTileThreads, 1)
+template <typename T, int D, int FEAT, bool Q8>
+__global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
     attn_tile_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const TileArgs p) {
-    using L = TileSmem<D>;
+    using L = TileSmem<D, Q8>;
     constexpr int NS = L::kSlots;
     constexpr int kBf16 = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
     const AttnArgs &a = p.a;
@@ -478,8 +504,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     RunDesc *runs = reinterpret_cast<RunDesc *>(tile_smem + L::runs);
     uint64_t *full = reinterpret_cast<uint64_t *>(tile_smem + L::bars);
     uint64_t *empty = full + NS;
-    uint64_t *run_full = empty + NS;           // [kRuns] descriptor written
-    uint64_t *run_free = run_full + L::kRuns;  // [kRuns] descriptor read by the 10 warps that use it
+    uint64_t *raw_full = empty + NS;           // [kRaw] bytes of a tile (and, with K, its scales)
+    uint64_t *raw_free = raw_full + L::kRaw;   // [kRaw] converted
+    uint64_t *run_full = raw_free + L::kRaw;   // [kRuns] descriptor written
+    uint64_t *run_free = run_full + L::kRuns;  // [kRuns] descriptor read by the 10 (Q8: 14) warps that use it
     uint64_t *s_full = run_free + L::kRuns;    // [2] scores in tensor memory (and every earlier MMA done)
     uint64_t *p_full = s_full + 2;             // [2] probabilities in tensor memory (V cleared, O rescaled)
     uint64_t *o_full = p_full + 2;             // [2] a run's last value MMA of the group done
@@ -495,12 +523,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < NS; ++i) {
-            mbar_init(&full[i], 1);
+            mbar_init(&full[i], Q8 ? 4 : 1);
             mbar_init(&empty[i], 2);
+        }
+        for (int i = 0; i < L::kRaw; ++i) {
+            mbar_init(&raw_full[i], 1);
+            mbar_init(&raw_free[i], 4);
         }
         for (int i = 0; i < L::kRuns; ++i) {
             mbar_init(&run_full[i], 1);
-            mbar_init(&run_free[i], 10);
+            mbar_init(&run_free[i], Q8 ? 14 : 10);
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&s_full[t], 1);
@@ -531,7 +563,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     auto wait = [&](uint64_t *bar, uint32_t phase) { return tile_wait(bar, phase & 1, abort); };
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kAuxRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q8 ? kAuxRegsQ8 : kAuxRegs));
         if (warp == 9) {
             // ===================================================================== producer
             // Walks the runs, hands their descriptors out and copies their tiles; the page lookups go
@@ -540,8 +572,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             RunIter it;
             it.begin(p, blockIdx.x);
             TileRun r{};
+            using Loc = std::conditional_t<Q8, PageLocQ8, PageLoc>;
             struct Step {
-                PageLoc loc;
+                Loc loc;
                 bool live, first, last;
             };
             const int R = a.block_size < 16 ? a.block_size : 16;
@@ -552,7 +585,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             uint32_t ph = 1;
             bool ok = true, more = true;
             Step s0{{-1, -1}, false, false, false}, s1 = s0;
-            PageLoc before{-1, -1};
+            Loc before{-1, -1};
+            [[maybe_unused]] int sc_slot = 0;  // scales of the tile copied next
+            [[maybe_unused]] const bool page_scales = a.scale_token_stride == 0;
             // ring order of a run: K0, K1, V0, K2, V1, ... V(n-1) (v_at).  The first two rounds only fill
             // the look-ahead; each part of the code stands here once, to keep it short.
 #pragma unroll 1
@@ -601,8 +636,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                             raise_status(GOLLEK_STATUS_BAD_BLOCK_ID);
                             e = 0;
                         }
-                        const int at8 = static_cast<int>((e * p.page_rows + static_cast<long long>(r.h) * a.block_size +
-                                                          (at - pg * a.block_size)) >> 3);
+                        const int off = at - pg * a.block_size;
+                        const long long first = e * p.page_rows + static_cast<long long>(r.h) * a.block_size + off;
+                        if constexpr (Q8) {
+                            const long long so = e * a.scale_page_stride + r.h * a.scale_head_stride + off * a.scale_token_stride;
+                            if (k == 0)
+                                s2.loc.sc0 = so;
+                            else
+                                s2.loc.sc1 = so;
+                            if (page_scales) {
+                                (k == 0 ? s2.loc.ks0 : s2.loc.ks1) = __ldg(a.k_scales + so);
+                                (k == 0 ? s2.loc.vs0 : s2.loc.vs1) = __ldg(a.v_scales + so);
+                            }
+                        }
+                        const int at8 = static_cast<int>(Q8 ? first : first >> 3);
                         if (k == 0)
                             s2.loc.row0 = at8;
                         else
@@ -615,19 +662,52 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll 1
                 for (int w = 0; w < 3 && s0.live && ok; ++w) {
                     if ((w == 1 && s0.first) || (w == 2 && !s0.last)) continue;
-                    const PageLoc l = w == 1 ? before : s0.loc;
-                    if (copies >= NS) ok = wait(&empty[slot], ph);
+                    const Loc l = w == 1 ? before : s0.loc;
+                    constexpr int kRing = Q8 ? L::kRaw : NS;
+                    uint64_t *const r_full = Q8 ? raw_full : full, *const r_free = Q8 ? raw_free : empty;
+                    if (copies >= kRing) ok = wait(&r_free[slot], ph);
                     if (!ok) break;
                     const unsigned boxes = (l.row0 >= 0) + (l.row1 >= 0);
-                    const uint32_t bytes = __reduce_add_sync(0xffffffffu, boxes) * R * D * 2;
-                    if (lane == 0) mbar_arrive_expect_tx(&full[slot], bytes);
+                    constexpr int kRowBytes = Q8 ? D : 2 * D;
+                    uint32_t bytes = __reduce_add_sync(0xffffffffu, boxes) * R * kRowBytes;
+                    if constexpr (Q8) {
+                        // with K: both scales of the tile, 16 positions a lane
+                        if (w == 0 && !page_scales) bytes += __reduce_add_sync(0xffffffffu, boxes) * R * 8;
+                        if (w == 0 && page_scales && lane < 8) {
+                            float *sk = reinterpret_cast<float *>(tile_smem + L::scales) + sc_slot * 256 + lane * 16;
+                            for (int i = 0; i < 16; ++i) {
+                                sk[i] = i < R ? l.ks0 : l.ks1;
+                                sk[128 + i] = i < R ? l.vs0 : l.vs1;
+                            }
+                        }
+                        __syncwarp();
+                    }
+                    if (lane == 0) mbar_arrive_expect_tx(&r_full[slot], bytes);
                     __syncwarp();
-                    uint8_t *dst = ring + slot * L::kSlot + lane * (16 * D * 2);
                     const CUtensorMap *map = w ? &tm_v : &tm_k;
-                    if (l.row0 >= 0) tma_load_4d(dst, map, 0, 0, 0, l.row0, &full[slot]);
-                    if (l.row1 >= 0) tma_load_4d(dst + 8 * D * 2, map, 0, 0, 0, l.row1, &full[slot]);
+                    if constexpr (Q8) {
+                        uint8_t *dst = tile_smem + L::raw + slot * (L::kSlot / 2) + lane * (16 * D);
+                        if (l.row0 >= 0) tma_load_2d(dst, map, 0, l.row0, &r_full[slot]);
+                        if (l.row1 >= 0) tma_load_2d(dst + 8 * D, map, 0, l.row1, &r_full[slot]);
+                        if (w == 0 && !page_scales) {
+                            float *sk = reinterpret_cast<float *>(tile_smem + L::scales) + sc_slot * 256 + lane * 16;
+                            if (l.row0 >= 0) {
+                                bulk_load(sk, a.k_scales + l.sc0, R * 4, &r_full[slot]);
+                                bulk_load(sk + 128, a.v_scales + l.sc0, R * 4, &r_full[slot]);
+                            }
+                            if (l.row1 >= 0) {
+                                bulk_load(sk + 8, a.k_scales + l.sc1, R * 4, &r_full[slot]);
+                                bulk_load(sk + 136, a.v_scales + l.sc1, R * 4, &r_full[slot]);
+                            }
+                        }
+                        if (w == 0) sc_slot = sc_slot + 1 == L::kScales ? 0 : sc_slot + 1;
+                    } else {
+                        uint8_t *dst = ring + slot * L::kSlot + lane * (16 * D * 2);
+                        if (l.row0 >= 0) tma_load_4d(dst, map, 0, 0, 0, l.row0, &r_full[slot]);
+                        if (l.row1 >= 0) tma_load_4d(dst + 8 * D * 2, map, 0, 0, 0, l.row1, &r_full[slot]);
+                    }
                     ++copies;
-                    if (++slot == NS) {
+                    if (++slot == kRing) {
                         slot = 0;
                         ph ^= 1;
                     }
@@ -639,9 +719,71 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (!ok && lane == 0) tile_give_up(abort);
             // every copy issued lands before the shared memory is released
             if (lane == 0)
-                for (int k = max(0, copies - NS); k < copies; ++k) mbar_wait(&full[k % NS], (k / NS) & 1);
+                for (int n = Q8 ? L::kRaw : NS, k = max(0, copies - n); k < copies; ++k)
+                    mbar_wait(Q8 ? &raw_full[k % n] : &full[k % n], (k / n) & 1);
             __syncwarp();
-        } else if (warp != 11) {
+        } else if (Q8 && warp >= 12) {
+            // ===================================================================== converters
+            // Copies of the ring in order: 128 x D bytes to bf16 in the operand layout, 16 bytes a thread at a
+            // time.  0x4300 | u is bf16 128 + u for u < 128, and 0x4300 | sign bit is 128 or 256: their
+            // difference is the signed byte, without the conversion pipe that the exponentials use.
+            if constexpr (Q8) {
+                const int me = tid - 384;
+                int rs = 0, bs = 0;
+                uint32_t rph = 0, bph = 1;
+                bool ok = true;
+#pragma unroll 1
+                for (int run = 0; ok; ++run) {
+                    const int at = run % L::kRuns;
+                    if (!(ok = wait(&run_full[at], run / L::kRuns))) break;
+                    const int n = runs[at].n;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&run_free[at]);
+                    if (n == 0) break;
+#pragma unroll 1
+                    for (int c = 0; c < 2 * n; ++c) {
+                        ok = wait(&raw_full[rs], rph) && wait(&empty[bs], bph);
+                        if (!ok) break;
+                        const uint32_t src = smem_u32(tile_smem + L::raw) + rs * (L::kSlot / 2);
+                        const uint32_t dst = smem_u32(ring) + bs * L::kSlot;
+                        constexpr int C = D / 16;  // 16-byte pieces of a row
+#pragma unroll 4
+                        for (int i = me; i < kTileTok * C; i += 128) {
+                            const int tok = i / C, pc = i % C;
+                            const uint4 w = lds_u4(src + i * 16);
+                            uint32_t o[8];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const uint32_t x = k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w;
+                                o[2 * k] = byte_pair<0x4140>(x);
+                                o[2 * k + 1] = byte_pair<0x4342>(x);
+                            }
+                            // the upper half of a row's threads stores its second chunk first: no two of eight
+                            // lanes meet in a bank
+                            const bool swap = pc >= C / 2;
+                            const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+                            sts_u4(dst + kv_chunk_off<D>(tok, 2 * pc + swap), swap ? hi : lo);
+                            sts_u4(dst + kv_chunk_off<D>(tok, 2 * pc + !swap), swap ? lo : hi);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            mbar_arrive(&full[bs]);
+                            mbar_arrive(&raw_free[rs]);
+                        }
+                        if (++rs == L::kRaw) {
+                            rs = 0;
+                            rph ^= 1;
+                        }
+                        if (++bs == NS) {
+                            bs = 0;
+                            bph ^= 1;
+                        }
+                    }
+                }
+                if (!ok && lane == 0) tile_give_up(abort);
+            }
+        } else if (warp == 8 || warp == 10) {
             // ===================================================================== MMA issuers
             // Warp 8 issues group 0's MMAs, warp 10 group 1's: what one waits for does not hold the
             // other up.  The warp walks its steps with warp-uniform values (descriptors stay in uniform
@@ -777,6 +919,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
         const uint32_t t_s = tmem + 128 * t + lanes, t_o = tmem + 256 + 128 * t + lanes;
         int c0 = 0, sn = 0;                // ring position of the run's first K; this group's tiles so far
+        [[maybe_unused]] int sc0 = 0;      // scales of the run's first tile
         int qb = 1;                        // q buffer of the last small block; 1 after a large one
         int ou[2] = {0, 0};                // runs that used O of group 0, 1 so far
         int mln = 0;                       // small blocks of more than one tile so far
@@ -832,7 +975,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         // -inf outside columns [jlo, jhi), bias -se |d0 + column| (c = -reference).
         uint32_t pk[64];
         const float cap1 = FEAT == kCap ? a.q_scale / a.soft_cap : 0.f, cap2 = a.soft_cap * kLog2e;
-        auto probs = [&](auto general, float c, float se, float d0, int jlo, int jhi, float &sum, float &top) {
+        auto probs = [&](auto general, float c, float se, float d0, int jlo, int jhi, const float *scales, float &sum, float &top) {
             constexpr bool GEN = decltype(general)::value;
             const float2 ff = make_float2(a.q_scale, a.q_scale), step = make_float2(2.f * se, 2.f * se);
             float2 acc = make_float2(0.f, 0.f);
@@ -852,6 +995,15 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 }
                 tmem_wait_ld();
                 if (k < 3) tmem_ld<32>(t_s + 32 * k + 32, v[(k + 1) & 1]);
+                if constexpr (Q8) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float4 s4 = *reinterpret_cast<const float4 *>(scales + 32 * k + 4 * i);
+                        const float2 a2 = mul2(make_float2(w[4 * i], w[4 * i + 1]), make_float2(s4.x, s4.y));
+                        const float2 b2 = mul2(make_float2(w[4 * i + 2], w[4 * i + 3]), make_float2(s4.z, s4.w));
+                        w[4 * i] = a2.x, w[4 * i + 1] = a2.y, w[4 * i + 2] = b2.x, w[4 * i + 3] = b2.y;
+                    }
+                }
                 if constexpr (FEAT == kCap) {
                     // cap tanh(y), y = score / cap: on the FMA pipe where |y| <= 1/2 in the whole warp
                     // (the usual case: caps are several times the scores), an odd polynomial of relative
@@ -897,6 +1049,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     x.x = fast_exp2(x.x);
                     x.y = fast_exp2(x.y);
                     acc = add2(acc, x);
+                    if constexpr (Q8) {
+                        // the value scale, 0 where nothing is seen (scales there may be anything)
+                        const float2 s2 = *reinterpret_cast<const float2 *>(scales + 128 + 32 * k + 2 * i);
+                        if constexpr (GEN) {
+                            x.x = (seen >> (2 * i) & 1) ? x.x * s2.x : 0.f;
+                            x.y = (seen >> (2 * i + 1) & 1) ? x.y * s2.y : 0.f;
+                        } else {
+                            x = mul2(x, s2);
+                        }
+                    }
                     pk[16 * k + i] = pack2<T>(x.x, x.y);
                 }
             }
@@ -948,7 +1110,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 // V rows that no row of the block attends are cleared (a zero probability does not
                 // cancel a NaN), by each group that uses the tile
                 const int vlo = d.lo - t0, vhi = d.hi - t0;
-                if (__builtin_expect(vlo > 0 || vhi < kTileTok, 0)) {
+                if (!Q8 && __builtin_expect(vlo > 0 || vhi < kTileTok, 0)) {  // int8: integers are finite
                     const int cv = c0 + v_at(j, n);
                     ok = wait(&full[cv % NS], cv / NS);
                     if (!ok) break;
@@ -976,6 +1138,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                                                           (FEAT != kPlain && slope != 0.f && !behind && !ahead)));
                     const float d0 = static_cast<float>(t0 - pos), se = general || behind ? slope : -slope;
                     const float base = FEAT != kPlain && !general ? se * d0 : 0.f;
+                    const float *scales = nullptr;
+                    if constexpr (Q8)
+                        scales = reinterpret_cast<const float *>(tile_smem + L::scales) + (sc0 + j) % L::kScales * 256;
                     float sum, top;
 #pragma unroll 1
                     for (int tries = 0;; ++tries) {
@@ -985,9 +1150,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         // 10^8, might never settle)
                         const float c = base - (m == -INFINITY ? 0.f : m);
                         if (general)
-                            probs(std::true_type{}, c, se, d0, jlo, jhi, sum, top);
+                            probs(std::true_type{}, c, se, d0, jlo, jhi, scales, sum, top);
                         else
-                            probs(std::false_type{}, c, se, d0, jlo, jhi, sum, top);
+                            probs(std::false_type{}, c, se, d0, jlo, jhi, scales, sum, top);
                         const bool move = live && (m == -INFINITY ? top > -INFINITY : top > kLazyMax);
                         if (__builtin_expect(tries == 2 || !__any_sync(0xffffffffu, move), 1)) break;
                         const float mn = !move ? m : m == -INFINITY ? top : m + top;
@@ -1115,6 +1280,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             ++ou[0];
             if (big || two) ++ou[1];
             c0 += 2 * n;
+            if constexpr (Q8) sc0 = (sc0 + n) % L::kScales;
         }
         if (!ok && lane == 0) tile_give_up(abort);
     }

@@ -78,10 +78,20 @@ int launch_generic(AttnArgs &a, cudaStream_t st) {
     return GOLLEK_OK;
 }
 
-// Whether the tile kernel takes the call: 16-bit pool and q of one type, head_dim 64 or 128,
-// pages of 8 or a multiple of 16 tokens in whole 8-row groups, 16-byte aligned tensors.
+// Whether the tile kernel takes the call: 16-bit pool and q of one type, or int8 pool and
+// bf16 q (one scale per page and head, or the scales of a page's tokens behind one another);
+// head_dim 64 or 128, pages of 8 or a multiple of 16 tokens in whole 8-row groups, 16-byte
+// aligned tensors.
 bool tile_takes(const AttnArgs &a) {
-    if (a.q_dtype != a.kv_dtype || (a.kv_dtype != GOLLEK_DTYPE_BF16 && a.kv_dtype != GOLLEK_DTYPE_F16)) return false;
+    if (a.kv_dtype == GOLLEK_DTYPE_I8) {
+        if (a.q_dtype != GOLLEK_DTYPE_BF16) return false;
+        if (a.scale_token_stride != 0 &&
+            (a.scale_token_stride != 1 || ((a.scale_page_stride | a.scale_head_stride) & 3) || !aligned16(a.k_scales) ||
+             !aligned16(a.v_scales)))
+            return false;
+    } else if (a.q_dtype != a.kv_dtype || (a.kv_dtype != GOLLEK_DTYPE_BF16 && a.kv_dtype != GOLLEK_DTYPE_F16)) {
+        return false;
+    }
     if (a.head_dim != 64 && a.head_dim != 128) return false;
     if (a.block_size != 8 && a.block_size % 16 != 0) return false;
     if (a.page_stride % (8 * a.head_dim) != 0) return false;
@@ -113,6 +123,21 @@ int encode_tile_map(CUtensorMap *m, const void *base, int kv_dtype, int D, long 
     return GOLLEK_OK;
 }
 
+// 2-D map over a pool of int8 rows; a box is box_rows whole rows, behind one another.
+int encode_byte_map(CUtensorMap *m, const void *base, int D, long long rows, int box_rows) {
+    auto enc = encode_fn();
+    if (!enc) return fail(GOLLEK_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled unavailable");
+    cuuint64_t dims[2] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows)};
+    cuuint64_t strides[1] = {static_cast<cuuint64_t>(D)};
+    cuuint32_t box[2] = {static_cast<cuuint32_t>(D), static_cast<cuuint32_t>(box_rows)};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(GOLLEK_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return GOLLEK_OK;
+}
+
 // A launch that may begin before the kernel in front of it has ended (that kernel's results are
 // read behind griddepcontrol.wait).
 int launch_dependent(const void *fn, dim3 grid, int threads, size_t smem, cudaStream_t st, void **args, const char *what) {
@@ -130,17 +155,19 @@ int launch_dependent(const void *fn, dim3 grid, int threads, size_t smem, cudaSt
     return GOLLEK_OK;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool Q8 = false>
 int launch_tile_as(TileArgs &p, const CUtensorMap &tmk, const CUtensorMap &tmv, cudaStream_t st) {
     const AttnArgs &a = p.a;
-    const void *fn = a.soft_cap > 0.f ? reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kCap>)
-                     : a.slopes       ? reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kBias>)
-                                      : reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kPlain>);
-    GK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, TileSmem<D>::total), "cudaFuncSetAttribute");
+    constexpr uint32_t smem = TileSmem<D, Q8>::total;
+    static_assert(smem <= 227 * 1024, "shared memory of the tile kernel");
+    const void *fn = a.soft_cap > 0.f ? reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kCap, Q8>)
+                     : a.slopes       ? reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kBias, Q8>)
+                                      : reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kPlain, Q8>);
+    GK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute");
     tile_plan_kernel<<<1, kPlanThreads, 0, st>>>(p);
     GK_CUDA(cudaGetLastError(), "tile_plan_kernel launch");
     void *args[] = {const_cast<CUtensorMap *>(&tmk), const_cast<CUtensorMap *>(&tmv), &p};
-    int rc = launch_dependent(fn, dim3(p.grid), kTileThreads, TileSmem<D>::total, st, args, "attn_tile_kernel launch");
+    int rc = launch_dependent(fn, dim3(p.grid), Q8 ? kTileThreadsQ8 : kTileThreads, smem, st, args, "attn_tile_kernel launch");
     if (rc) return rc;
     void *margs[] = {&p};
     if (a.num_groups == 0)
@@ -184,10 +211,17 @@ int launch_tile(AttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
     const long long rows = a.num_blocks > 0 ? a.num_blocks * p.page_rows : (1LL << 31) - 8;
     const int box = std::min(a.block_size, 16);
     CUtensorMap tmk, tmv;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a.kv_dtype == GOLLEK_DTYPE_I8) {
+        int rc = encode_byte_map(&tmk, a.k, a.head_dim, rows, box);
+        if (!rc) rc = encode_byte_map(&tmv, a.v, a.head_dim, rows, box);
+        if (rc) return rc;
+        return a.head_dim == 128 ? launch_tile_as<__nv_bfloat16, 128, true>(p, tmk, tmv, st)
+                                 : launch_tile_as<__nv_bfloat16, 64, true>(p, tmk, tmv, st);
+    }
     int rc = encode_tile_map(&tmk, a.k, a.kv_dtype, a.head_dim, rows, box);
     if (!rc) rc = encode_tile_map(&tmv, a.v, a.kv_dtype, a.head_dim, rows, box);
     if (rc) return rc;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool bf16 = a.kv_dtype == GOLLEK_DTYPE_BF16;
     if (a.head_dim == 128)
         return bf16 ? launch_tile_as<__nv_bfloat16, 128>(p, tmk, tmv, st) : launch_tile_as<__half, 128>(p, tmk, tmv, st);
