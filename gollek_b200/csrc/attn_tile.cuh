@@ -42,13 +42,11 @@ constexpr int kBlkRows = 256;
 constexpr int kRunCostTiles = 2;      // start-up of a run (q, pipeline fill, output), in tiles
 constexpr int kMaxTileCtas = 160;
 constexpr int kTileThreads = 384;     // 8 row warps, 2 MMA issuers, 1 producer, 1 idle
-// Registers: launched with 168 a thread (384 x 168 = 64,512 of the SM's 65,536), of which the
-// third warpgroup gives the row groups 32 each: 2 x 200 + 104 = 3 x 168.  A row thread holds a
-// tile's 128 scores; at 168 it would spill 560 bytes.
-constexpr int kRowRegs = 200, kAuxRegs = 104;
-// int8 caches: a fourth warpgroup converts; 512 threads launched with 128 registers.
-constexpr int kTileThreadsQ8 = 512, kAuxRegsQ8 = 56;
-constexpr float kLazyMax = 8.f;
+constexpr int kTileThreadsQ8 = 512;   // int8 caches: a fourth warpgroup converts
+// Scores may pass their row's reference by this much (log2 units) before it moves: P stays far
+// below the largest number of its type, and sums of it below fp32's.
+template <typename T>
+constexpr float kLazyMax = std::is_same<T, __half>::value ? 12.f : 64.f;
 
 // A block: rows row0 .. row0 + nrows - 1 (row r: query token tok0 + r / G, q head h G + r % G)
 // over positions [lo, hi) of table row `tab`, whose length is len.
@@ -363,7 +361,8 @@ struct TileSmem {
     static constexpr uint32_t ring = 2 * kQ;
     static constexpr uint32_t raw = ring + kSlots * kSlot;   // [kRaw][128][D] bytes
     static constexpr uint32_t scales = raw + kRaw * (kSlot / 2);  // [kScales][K, V][128] floats
-    static constexpr uint32_t ml = scales + kScales * 1024;  // [2][128] floats
+    static constexpr uint32_t ones = scales + kScales * 1024;  // Q8: [128] floats of 1
+    static constexpr uint32_t ml = ones + (Q8 ? 512 : 0);  // [2][128] floats
     static constexpr uint32_t runs = ml + 2 * 128 * 4;     // [kRuns] x 48 bytes
     static constexpr uint32_t bars = runs + kRuns * 48;
     static constexpr int kBars = 2 * kSlots + 2 * kRaw + 2 * kRuns + 2 * 7 + 8 + 1;
@@ -383,14 +382,23 @@ struct __align__(16) RunDesc {
 
 // Bounded wait of a whole warp: each lane tests on its own, one vote at the end (the
 // result is warp-uniform); gives up once another warp did.  The warp that gives up first
-// raises the status (tile_give_up), at the end of its role and not here, which keeps the
-// code of a wait short.
-__device__ __forceinline__ bool tile_wait(uint64_t *bar, uint32_t parity, volatile int *abort) {
-    bool ok = mbar_try_wait(bar, parity);
+// raises the status (tile_give_up) at the end of its role.  One copy of the code for all
+// waits: see opaque() on why size matters here.
+__device__ __noinline__ bool tile_wait(uint32_t bar, uint32_t parity, uint32_t abort) {
+    bool ok = false;
 #pragma unroll 1
     for (unsigned i = 0; !ok && i < kSuspendTries; ++i) {
-        if (*abort) break;
-        ok = mbar_try_wait_suspend(bar, parity, kSuspendNs);
+        uint32_t done, gone;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%2], %3, %5;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t"
+            "ld.volatile.shared.u32 %1, [%4];\n\t}"
+            : "=r"(done), "=r"(gone)
+            : "r"(bar), "r"(parity), "r"(abort), "r"(kSuspendNs)
+            : "memory");
+        ok = done != 0;
+        if (gone) break;
     }
     return __all_sync(0xffffffffu, ok);
 }
@@ -453,6 +461,17 @@ __device__ __forceinline__ uint32_t byte_pair(uint32_t w) {
     const uint32_t x = __byte_perm(w, 0x43434343u, SEL);
     uint32_t a = x & 0xFF7FFF7Fu, b = x & 0xFF80FF80u, d;
     asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
+// A packed pair times a packed pair.
+template <typename T>
+__device__ __forceinline__ uint32_t scale_pair(uint32_t x, uint32_t by) {
+    uint32_t d;
+    if constexpr (std::is_same<T, __half>::value)
+        asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(by));
+    else
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(by));
     return d;
 }
 
@@ -548,6 +567,7 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
         fence_barrier_init();
         *abort = 0;
     }
+    if (Q8 && tid < 128) reinterpret_cast<float *>(tile_smem + L::ones)[tid] = 1.f;
     if (warp == 9 && lane == 0) {
         prefetch_tensormap(&tm_k);
         prefetch_tensormap(&tm_v);
@@ -560,10 +580,10 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *sm_tmem;
-    auto wait = [&](uint64_t *bar, uint32_t phase) { return tile_wait(bar, phase & 1, abort); };
+    const uint32_t abort_s = smem_u32(tile_smem + L::misc);
+    auto wait = [&](uint64_t *bar, uint32_t phase) { return tile_wait(smem_u32(bar), phase & 1, abort_s); };
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q8 ? kAuxRegsQ8 : kAuxRegs));
         if (warp == 9) {
             // ===================================================================== producer
             // Walks the runs, hands their descriptors out and copies their tiles; the page lookups go
@@ -911,7 +931,6 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
         }
     } else {
         // ===================================================================== row groups
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRowRegs));
         const int G = a.num_q_heads / a.num_kv_heads;
         const unsigned g_magic = div_magic(G);
         const int t = warp >> 2;           // group
@@ -969,39 +988,20 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
             }
         };
 
-        // One pass over a tile's scores: x, the score in the exponent domain less the row's reference,
-        // P = 2^x packed into pk, its sum and the largest x.  GEN false: every column is visible and the
-        // bias is linear in the column (se of either sign; c = bias at column 0 - reference).  GEN true:
-        // -inf outside columns [jlo, jhi), bias -se |d0 + column| (c = -reference).
-        uint32_t pk[64];
+        // rewrite: where a cap, a mask or a bias of both signs asks for more than probs does, S becomes the
+        // score in the exponent domain first, -inf outside columns [jlo, jhi).
         const float cap1 = FEAT == kCap ? a.q_scale / a.soft_cap : 0.f, cap2 = a.soft_cap * kLog2e;
-        auto probs = [&](auto general, float c, float se, float d0, int jlo, int jhi, const float *scales, float &sum, float &top) {
-            constexpr bool GEN = decltype(general)::value;
-            const float2 ff = make_float2(a.q_scale, a.q_scale), step = make_float2(2.f * se, 2.f * se);
-            float2 acc = make_float2(0.f, 0.f);
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            float v[2][32];
-            tmem_ld<32>(t_s, v[0]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float(&w)[32] = v[k & 1];
-                [[maybe_unused]] float2 cc = make_float2(c, c);
-                if constexpr (FEAT != kPlain && !GEN) cc = make_float2(fmaf(se, 32.f * k, c), fmaf(se, 32.f * k + 1.f, c));
-                [[maybe_unused]] unsigned seen = ~0u;
-                if constexpr (GEN) {
-                    const int l0 = jlo - 32 * k, h0 = jhi - 32 * k;
-                    seen = h0 >= 32 ? ~0u : h0 <= 0 ? 0u : (1u << h0) - 1;
-                    if (l0 > 0) seen = l0 >= 32 ? 0u : seen & (~0u << l0);
-                }
+        auto rewrite = [&](float slope, float d0, int jlo, int jhi, const float *scales) {
+#pragma unroll 1
+            for (int k = 0; k < 128; k += 32) {
+                float w[32];
+                tmem_ld<32>(t_s + k, w);
                 tmem_wait_ld();
-                if (k < 3) tmem_ld<32>(t_s + 32 * k + 32, v[(k + 1) & 1]);
                 if constexpr (Q8) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float4 s4 = *reinterpret_cast<const float4 *>(scales + 32 * k + 4 * i);
-                        const float2 a2 = mul2(make_float2(w[4 * i], w[4 * i + 1]), make_float2(s4.x, s4.y));
-                        const float2 b2 = mul2(make_float2(w[4 * i + 2], w[4 * i + 3]), make_float2(s4.z, s4.w));
-                        w[4 * i] = a2.x, w[4 * i + 1] = a2.y, w[4 * i + 2] = b2.x, w[4 * i + 3] = b2.y;
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 s4 = *reinterpret_cast<const float4 *>(scales + k + i);
+                        w[i] *= s4.x, w[i + 1] *= s4.y, w[i + 2] *= s4.z, w[i + 3] *= s4.w;
                     }
                 }
                 if constexpr (FEAT == kCap) {
@@ -1010,11 +1010,9 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
                     // error below 2^-22; else cap - 2 cap / (1 + e^2y), two exponent-pipe operations
                     float big_y = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float2 y = mul2(make_float2(w[2 * i], w[2 * i + 1]), make_float2(cap1, cap1));
-                        w[2 * i] = y.x;
-                        w[2 * i + 1] = y.y;
-                        big_y = fmaxf(big_y, fmaxf(fabsf(y.x), fabsf(y.y)));
+                    for (int i = 0; i < 32; ++i) {
+                        w[i] *= cap1;
+                        big_y = fmaxf(big_y, fabsf(w[i]));
                     }
                     if (__any_sync(0xffffffffu, !(big_y <= 0.5f))) {
 #pragma unroll
@@ -1022,48 +1020,125 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
                             w[i] = fmaf(-2.f, __fdividef(1.f, 1.f + fast_exp2(w[i] * (2.f * kLog2e))), 1.f);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float2 y = make_float2(w[2 * i], w[2 * i + 1]), y2 = mul2(y, y);
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 y = make_float2(w[i], w[i + 1]), y2 = mul2(y, y);
                             float2 q = fma2(y2, pair(0.01724149100482f), pair(-0.05304549261928f));
                             q = fma2(q, y2, pair(0.13325878977776f));
                             q = fma2(q, y2, pair(-0.33333143591881f));
                             q = fma2(mul2(q, y2), y, y);
-                            w[2 * i] = q.x;
-                            w[2 * i + 1] = q.y;
+                            w[i] = q.x;
+                            w[i + 1] = q.y;
                         }
                     }
                 }
+                const float f = FEAT == kCap ? cap2 : a.q_scale;
+                const int l0 = jlo - k, h0 = jhi - k;
+                unsigned seen = h0 >= 32 ? ~0u : h0 <= 0 ? 0u : (1u << h0) - 1;
+                if (l0 > 0) seen = l0 >= 32 ? 0u : seen & (~0u << l0);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    if constexpr (FEAT != kPlain && GEN) {
-                        const float col = static_cast<float>(32 * k + 2 * i);
-                        cc = make_float2(fmaf(-se, fabsf(d0 + col), c), fmaf(-se, fabsf(d0 + (col + 1.f)), c));
-                    }
-                    float2 x = fma2(make_float2(w[2 * i], w[2 * i + 1]), FEAT == kCap ? make_float2(cap2, cap2) : ff, cc);
-                    if constexpr (FEAT != kPlain && !GEN) cc = add2(cc, step);
-                    if constexpr (GEN) {
-                        x.x = (seen >> (2 * i) & 1) ? x.x : -INFINITY;
-                        x.y = (seen >> (2 * i + 1) & 1) ? x.y : -INFINITY;
-                    }
-                    mx[i & 3] = fmaxf(mx[i & 3], fmaxf(x.x, x.y));
-                    x.x = fast_exp2(x.x);
-                    x.y = fast_exp2(x.y);
+                for (int i = 0; i < 32; ++i) {
+                    float x = w[i] * f;
+                    if constexpr (FEAT != kPlain) x = fmaf(-slope, fabsf(d0 + static_cast<float>(k + i)), x);
+                    w[i] = (seen >> i & 1) ? x : -INFINITY;
+                }
+                tmem_st32(t_s + k, w);
+            }
+            tmem_wait_st();
+        };
+        float m = -INFINITY, l = 0.f;  // the row's reference (exponent domain) and sum in this run
+        // The reference rises by `by` (an integer where the row had one, so that all but m scale
+        // exactly), and what stands relative to it follows: l, the sum so far, the columns of P stored
+        // already and O (fresh: the group has none in this run yet; what stands there may be another
+        // run's that group 0 is still reading).
+        auto raise = [&](bool move, float top, float2 &acc, int stored, bool fresh) {
+            const float by = !move || m == -INFINITY ? 0.f : ceilf(top), alpha = fast_exp2(-by);
+            m = !move ? m : m == -INFINITY ? top : m + by;
+            if (!__any_sync(0xffffffffu, by != 0.f)) return;
+            l *= alpha;
+            acc.x *= alpha;
+            acc.y *= alpha;
+            const uint32_t a2 = pack2<T>(alpha, alpha);
+            tmem_wait_ld();
+            tmem_wait_st();
+#pragma unroll 1
+            for (int k = fresh ? D : 0; k < D + stored; k += 8) {
+                // the scores' commit covers the group's earlier value MMAs: O is at rest
+                const bool is_o = k < D;
+                const uint32_t at = is_o ? t_o + k : t_s + (k - D);
+                float o[8];
+                tmem_ld<8>(at, o);
+                tmem_wait_ld();
+                uint32_t w[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    w[i] = is_o ? __float_as_uint(o[i] * alpha) : scale_pair<T>(__float_as_uint(o[i]), a2);
+                tmem_st8(at, w);
+            }
+            tmem_wait_st();
+        };
+        // One pass over a tile's scores: x = S f + c + se column - m (c: bias at column 0), P = 2^x over the
+        // columns read already, and its sum.  S is read once, since reading it takes about as long as
+        // the exponentials.
+        auto probs = [&](float f, float c, float se, const float *scales_k, const float *scales_v, bool live, bool fresh) {
+            constexpr int W = Q8 ? 16 : 32;  // columns at a time, the next ones' load under way
+            float2 acc = make_float2(0.f, 0.f);
+            float wa[W], wb[W];
+            auto part = [&](float(&w)[W], int col) {
+                float2 cc = pair(c - (m == -INFINITY ? 0.f : m));
+                if constexpr (FEAT == kBias) {
+                    cc.x = fmaf(se, static_cast<float>(col), cc.x);
+                    cc.y = cc.x + se;
+                }
+                float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < W; i += 2) {
+                    float2 ff = pair(f);
+                    if constexpr (Q8) ff = mul2(ff, *reinterpret_cast<const float2 *>(scales_k + col + i));
+                    const float2 x = fma2(make_float2(w[i], w[i + 1]), ff, cc);
+                    if constexpr (FEAT == kBias) cc = add2(cc, pair(2.f * se));
+                    w[i] = x.x;
+                    w[i + 1] = x.y;
+                    mx[i / 2 & 1] = fmaxf(mx[i / 2 & 1], fmaxf(x.x, x.y));
+                }
+                const float top = fmaxf(mx[0], mx[1]);
+                const bool move = live && (m == -INFINITY ? top > -INFINITY : top > kLazyMax<T>);
+                if (__builtin_expect(__any_sync(0xffffffffu, move), 0)) {
+                    const float was = m == -INFINITY ? 0.f : m;
+                    raise(move, top, acc, col / 2, fresh);
+                    const float down = was - (m == -INFINITY ? 0.f : m);
+#pragma unroll
+                    for (int i = 0; i < W; ++i) w[i] += down;
+                }
+                uint32_t pk[W / 2];
+#pragma unroll
+                for (int i = 0; i < W; i += 2) {
+                    float2 x = make_float2(fast_exp2(w[i]), fast_exp2(w[i + 1]));
                     acc = add2(acc, x);
                     if constexpr (Q8) {
-                        // the value scale, 0 where nothing is seen (scales there may be anything)
-                        const float2 s2 = *reinterpret_cast<const float2 *>(scales + 128 + 32 * k + 2 * i);
-                        if constexpr (GEN) {
-                            x.x = (seen >> (2 * i) & 1) ? x.x * s2.x : 0.f;
-                            x.y = (seen >> (2 * i + 1) & 1) ? x.y * s2.y : 0.f;
-                        } else {
-                            x = mul2(x, s2);
-                        }
+                        // times the value's scale; where nothing is seen (P = 0) that may be anything
+                        const float2 s2 = *reinterpret_cast<const float2 *>(scales_v + col + i);
+                        x.x = x.x == 0.f ? 0.f : x.x * s2.x;
+                        x.y = x.y == 0.f ? 0.f : x.y * s2.y;
                     }
-                    pk[16 * k + i] = pack2<T>(x.x, x.y);
+                    pk[i / 2] = pack2<T>(x.x, x.y);
                 }
+                if constexpr (W == 32)
+                    tmem_st16(t_s + (col >> 1), pk);
+                else
+                    tmem_st8(t_s + (col >> 1), pk);
+            };
+            tmem_ld<W>(t_s, wa);
+#pragma unroll 1
+            for (int k = 0; k < 128; k += 2 * W) {
+                tmem_wait_ld();
+                tmem_ld<W>(t_s + k + W, wb);
+                part(wa, k);
+                tmem_wait_ld();
+                tmem_ld<W>(t_s + (k + 2 * W & 127), wa);  // the last round's is not used
+                part(wb, k + W);
             }
-            sum = acc.x + acc.y;
-            top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            tmem_wait_ld();
+            l += acc.x + acc.y;
         };
 
 #pragma unroll 1
@@ -1098,7 +1173,8 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
                 }
             }
             const bool warp_live = __any_sync(0xffffffffu, live);
-            float m = -INFINITY, l = 0.f;
+            m = -INFINITY;
+            l = 0.f;
             const int j0 = big ? 0 : t, dj = big ? 1 : 2;
 #pragma unroll 1
             for (int j = j0; j < n; j += dj) {
@@ -1122,65 +1198,36 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
                     fence_proxy_async_smem();
                     __syncwarp();
                 }
+                float f = a.q_scale, se = 0.f, base = 0.f;
+                [[maybe_unused]] const float *scales = nullptr, *scales_k = nullptr;
+                if constexpr (Q8)
+                    scales_k = scales = reinterpret_cast<const float *>(tile_smem + L::scales) + (sc0 + j) % L::kScales * 256;
+                if (opaque(warp_live)) {
+                    // The bias is linear in the column where the row's visible columns lie on one side of its
+                    // own position.
+                    const bool behind = jhi <= pos + 1 - t0, ahead = jlo >= pos - t0;
+                    const bool odd = live && (jlo > 0 || jhi < kTileTok || (FEAT == kBias && slope != 0.f && !behind && !ahead));
+                    const float d0 = static_cast<float>(t0 - pos);
+                    if (FEAT == kCap || __any_sync(0xffffffffu, odd)) {
+                        rewrite(slope, d0, jlo, jhi, scales);
+                        f = 1.f;
+                        scales_k = reinterpret_cast<const float *>(tile_smem + L::ones);  // applied already
+                    } else if (FEAT == kBias) {
+                        se = behind ? slope : -slope;
+                        base = se * d0;
+                    }
+                }
                 // Large blocks: the two groups' warps on one SM sub-partition take turns, so that one's
-                // exponentials run under the other's products.  Left alone most CTAs fell into step:
-                // both computed, then both waited.
+                // exponentials run under the other's products.  Left alone most CTAs fell into step: both
+                // computed, then both waited.
                 if (opaque(big)) {
                     if (turns + t > 0) ok = wait(&turn[4 * t + (warp & 3)], turns + t - 1);
                     if (!ok) break;
                     ++turns;
                 }
-                if (opaque(warp_live)) {
-                    // The bias is linear in the column where the row's visible columns lie on one side of its
-                    // own position.
-                    const bool behind = jhi <= pos + 1 - t0, ahead = jlo >= pos - t0;
-                    const bool general = __any_sync(0xffffffffu, live && (jlo > 0 || jhi < kTileTok ||
-                                                                          (FEAT != kPlain && slope != 0.f && !behind && !ahead)));
-                    const float d0 = static_cast<float>(t0 - pos), se = general || behind ? slope : -slope;
-                    const float base = FEAT != kPlain && !general ? se * d0 : 0.f;
-                    const float *scales = nullptr;
-                    if constexpr (Q8)
-                        scales = reinterpret_cast<const float *>(tile_smem + L::scales) + (sc0 + j) % L::kScales * 256;
-                    float sum, top;
-#pragma unroll 1
-                    for (int tries = 0;; ++tries) {
-                        // P against the row's reference; where a score passes it by more than 2^kLazyMax (or
-                        // the row has none yet) the reference moves, O follows, and the pass is repeated
-                        // (twice at most: a reference so large that its own rounding exceeds 2^kLazyMax, some
-                        // 10^8, might never settle)
-                        const float c = base - (m == -INFINITY ? 0.f : m);
-                        if (general)
-                            probs(std::true_type{}, c, se, d0, jlo, jhi, scales, sum, top);
-                        else
-                            probs(std::false_type{}, c, se, d0, jlo, jhi, scales, sum, top);
-                        const bool move = live && (m == -INFINITY ? top > -INFINITY : top > kLazyMax);
-                        if (__builtin_expect(tries == 2 || !__any_sync(0xffffffffu, move), 1)) break;
-                        const float mn = !move ? m : m == -INFINITY ? top : m + top;
-                        const float alpha = (mn == m || m == -INFINITY) ? 1.f : fast_exp2(m - mn);
-                        m = mn;
-                        l *= alpha;
-                        // the scores' commit covers the group's earlier value MMAs: O is at rest
-                        if (__any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll 1
-                            for (int k = 0; k < D; k += 16) {
-                                float o[16];
-                                tmem_ld<16>(t_o + k, o);
-                                tmem_wait_ld();
-                                uint32_t w[16];
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(o[i] * alpha);
-                                tmem_st16(t_o + k, w);
-                            }
-                        }
-                    }
-                    l += sum;
-                    if (opaque(big) && lane == 0) mbar_arrive(&turn[4 * (t ^ 1) + (warp & 3)]);
-                    tmem_st32(t_s, reinterpret_cast<const float *>(pk));
-                    tmem_st32(t_s + 32, reinterpret_cast<const float *>(pk + 32));
-                    tmem_wait_st();
-                } else if (opaque(big) && lane == 0) {
-                    mbar_arrive(&turn[4 * (t ^ 1) + (warp & 3)]);
-                }
+                if (opaque(warp_live)) probs(f, base, se, scales_k, scales + 128, live, j == j0);
+                if (opaque(big) && lane == 0) mbar_arrive(&turn[4 * (t ^ 1) + (warp & 3)]);
+                tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[t]);
