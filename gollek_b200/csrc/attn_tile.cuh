@@ -74,10 +74,10 @@ struct TileWs {
 
 __host__ __device__ inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-// Rows of all entities cut into blocks of 256: each entity leaves at most one short block.
-inline TileWs tile_ws(long long entities, long long rows, long long out_rows, int D, bool shared) {
+// Rows of all entities cut into blocks of blk_rows: each entity leaves at most one short block.
+inline TileWs tile_ws(long long entities, long long rows, int blk_rows, long long out_rows, int D, bool shared) {
     TileWs w;
-    w.max_blocks = rows / kBlkRows + entities;
+    w.max_blocks = rows / blk_rows + entities;
     size_t o = 256;
     w.blks = o;
     o = up256(o + w.max_blocks * sizeof(TileBlk));
@@ -105,6 +105,7 @@ struct TileArgs {
     float2 *ml;       // shared: [2][rows]
     float *acc;       // shared: [2][rows][D]
     int entities, grid, max_blocks;
+    int blk_rows;     // rows a block may have
     long long page_rows;
 };
 
@@ -175,7 +176,7 @@ __global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(const TileArgs 
                 check_group(a, e);
             else
                 check_seq(a, e - a.num_groups);
-            blocks = (static_cast<long long>(entity_tokens(a, e)) * G + kBlkRows - 1) / kBlkRows;
+            blocks = (static_cast<long long>(entity_tokens(a, e)) * G + p.blk_rows - 1) / p.blk_rows;
         }
         long long sum;
         const long long at = block_scan(blocks, sm_l, &sum);
@@ -221,8 +222,8 @@ __global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(const TileArgs 
                 k.len = clamp_len(a, a.context_lens[k.tab], a.max_blocks);
             }
             k.tok0 = first;
-            k.row0 = (b - p.ents[e]) * kBlkRows;
-            k.nrows = static_cast<int>(min(static_cast<long long>(n) * G - k.row0, static_cast<long long>(kBlkRows)));
+            k.row0 = (b - p.ents[e]) * p.blk_rows;
+            k.nrows = static_cast<int>(min(static_cast<long long>(n) * G - k.row0, static_cast<long long>(p.blk_rows)));
             k.lo = 0;
             k.hi = k.len;
             if (k.kind == kOwn) {
@@ -407,6 +408,12 @@ __device__ __forceinline__ void tile_give_up(volatile int *abort) {
     *abort = 1;
 }
 
+template <typename T>
+__device__ __forceinline__ void sts_u2(uint32_t addr, T v) {
+    static_assert(sizeof(T) == 2, "two bytes");
+    asm volatile("st.shared.b16 [%0], %1;" ::"r"(addr), "h"(reinterpret_cast<const unsigned short &>(v)) : "memory");
+}
+
 // x / d for 0 <= x < 2^31: the magic's quotient is at most one too large.
 __device__ __forceinline__ unsigned div_magic(int d) { return d == 1 ? 0u : 0xFFFFFFFFu / d + 1; }
 __device__ __forceinline__ int fast_div(int x, int d, unsigned magic) {
@@ -475,6 +482,32 @@ __device__ __forceinline__ uint32_t scale_pair(uint32_t x, uint32_t by) {
     return d;
 }
 
+// w = tanh(w), warp-collective: on the FMA pipe where |w| <= 1/2 in the whole warp (the usual
+// case: caps are several times the scores), an odd polynomial of relative error below 2^-22;
+// else 1 - 2 / (1 + e^2w), two exponent-pipe operations.
+template <int N>
+__device__ __forceinline__ void unit_cap(float (&w)[N]) {
+    float big = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) big = fmaxf(big, fabsf(w[i]));
+    if (__any_sync(0xffffffffu, !(big <= 0.5f))) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            w[i] = fmaf(-2.f, __fdividef(1.f, 1.f + fast_exp2(w[i] * (2.f * kLog2e))), 1.f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float2 y = make_float2(w[i], w[i + 1]), y2 = mul2(y, y);
+            float2 q = fma2(y2, pair(0.01724149100482f), pair(-0.05304549261928f));
+            q = fma2(q, y2, pair(0.13325878977776f));
+            q = fma2(q, y2, pair(-0.33333143591881f));
+            q = fma2(mul2(q, y2), y, y);
+            w[i] = q.x;
+            w[i + 1] = q.y;
+        }
+    }
+}
+
 // One lane of the converged warp, always the same.
 __device__ __forceinline__ bool elect_one() {
     uint32_t ok;
@@ -507,6 +540,284 @@ struct PageLocQ8 {
 
 __device__ __forceinline__ int v_at(int j, int n) { return j == n - 1 ? 2 * n - 1 : 2 * j + 2; }
 
+// What the producer, the converters and the other roles of a kernel share; L names the places.
+template <typename L>
+struct TilePipe {
+    uint8_t *smem;
+    RunDesc *runs;
+    uint64_t *full, *empty;        // [kSlots] tile in shared memory; read
+    uint64_t *raw_full, *raw_free; // [kRaw] bytes of a tile (and, with K, its scales); converted
+    uint64_t *run_full, *run_free; // [kRuns] descriptor written; read by the warps that use it
+    uint64_t *own;                 // the kernel's own barriers
+    volatile int *abort;
+
+    __device__ __forceinline__ explicit TilePipe(uint8_t *base) : smem(base) {
+        runs = reinterpret_cast<RunDesc *>(base + L::runs);
+        full = reinterpret_cast<uint64_t *>(base + L::bars);
+        empty = full + L::kSlots;
+        raw_full = empty + L::kSlots;
+        raw_free = raw_full + L::kRaw;
+        run_full = raw_free + L::kRaw;
+        run_free = run_full + L::kRuns;
+        own = run_free + L::kRuns;
+        abort = reinterpret_cast<volatile int *>(base + L::misc);
+    }
+    // by one thread; `fillers` arrive on full, `readers` on empty, `users` read a descriptor
+    __device__ __forceinline__ void init(int fillers, int readers, int users) const {
+        for (int i = 0; i < L::kSlots; ++i) {
+            mbar_init(&full[i], fillers);
+            mbar_init(&empty[i], readers);
+        }
+        for (int i = 0; i < L::kRaw; ++i) {
+            mbar_init(&raw_full[i], 1);
+            mbar_init(&raw_free[i], fillers);
+        }
+        for (int i = 0; i < L::kRuns; ++i) {
+            mbar_init(&run_full[i], 1);
+            mbar_init(&run_free[i], users);
+        }
+        *abort = 0;
+    }
+    __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t phase) const {
+        return tile_wait(smem_u32(bar), phase & 1, smem_u32(smem + L::misc));
+    }
+};
+
+// Walks the runs, hands their descriptors out and copies their tiles; the page lookups go
+// two tiles ahead of the copies, across runs.
+template <typename L, int D, bool Q8>
+__device__ __forceinline__ void tile_producer(const TileArgs &p, const TilePipe<L> &pipe, const CUtensorMap &tm_k,
+                                              const CUtensorMap &tm_v, int lane) {
+    constexpr int NS = L::kSlots;
+    const AttnArgs &a = p.a;
+    uint64_t *const full = pipe.full, *const empty = pipe.empty, *const run_full = pipe.run_full, *const run_free = pipe.run_free;
+    [[maybe_unused]] uint64_t *const raw_full = pipe.raw_full, *const raw_free = pipe.raw_free;
+    RunDesc *const runs = pipe.runs;
+    volatile int *const abort = pipe.abort;
+    auto wait = [&](uint64_t *bar, uint32_t phase) { return pipe.wait(bar, phase); };
+    pdl_wait();  // the plan is complete
+    RunIter it;
+    it.begin(p, blockIdx.x);
+    TileRun r{};
+    using Loc = std::conditional_t<Q8, PageLocQ8, PageLoc>;
+    struct Step {
+        Loc loc;
+        bool live, first, last;
+    };
+    const int R = a.block_size < 16 ? a.block_size : 16;
+    const unsigned bs_magic = div_magic(a.block_size);
+    const int *bt = nullptr;
+    int t = 0, tb = 0, ta = 0, nrun = 0;
+    int slot = 0, copies = 0;
+    uint32_t ph = 1;
+    bool ok = true, more = true;
+    Step s0{{-1, -1}, false, false, false}, s1 = s0;
+    Loc before{-1, -1};
+    [[maybe_unused]] int sc_slot = 0;  // scales of the tile copied next
+    [[maybe_unused]] const bool page_scales = a.scale_token_stride == 0;
+    // ring order of a run: K0, K1, V0, K2, V1, ... V(n-1) (v_at).  The first two rounds only fill
+    // the look-ahead; each part of the code stands here once, to keep it short.
+#pragma unroll 1
+    for (int round = 0; ok && (round < 2 || s0.live); ++round) {
+        Step s2{{-1, -1}, false, false, false};
+        if (t >= tb && more) {
+            // the next run: its descriptor for the other warps, its table
+            more = it.next(p, r);
+            const int at = nrun % L::kRuns;
+            if (nrun >= L::kRuns) ok = wait(&run_free[at], nrun / L::kRuns - 1);
+            if (lane == 0 && ok) {
+                RunDesc &d = runs[at];
+                d.tok0 = r.b.tok0;
+                d.row0 = r.b.row0;
+                d.nrows = r.b.nrows;
+                d.h = r.h;
+                d.lo = r.b.lo;
+                d.hi = r.b.hi;
+                d.tile0 = r.b.lo / kTileTok + r.tb - 1;
+                d.n = more ? r.tb - r.ta : 0;
+                d.tab = r.b.tab;
+                d.len = r.b.len;
+                d.pos0 = r.b.pos0;
+                d.flags = r.b.kind | (r.ta == 0 && r.tb == r.n ? 4 : 0) | (r.ta == 0 ? 8 : 0);
+                mbar_arrive(&run_full[at]);
+            }
+            __syncwarp();
+            ++nrun;
+            bt = r.b.kind == kPrefix ? a.prefix_tables + static_cast<long long>(r.b.tab) * a.max_pblocks
+                                     : a.block_tables + static_cast<long long>(r.b.tab) * a.max_blocks;
+            t = ta = r.ta;
+            tb = more ? r.tb : r.ta;
+        }
+        if (t < tb) {
+            s2.live = true;
+            s2.first = t == ta;
+            s2.last = t == tb - 1;
+            // pool rows / 8 of the lane's box(es); -1: nothing to load there
+            int at = (r.b.lo / kTileTok + tb - 1 - (t - ta)) * kTileTok + lane * 16;
+#pragma unroll 1
+            for (int k = 0; k < 16; k += R, at += R) {
+                if (lane >= 8 || at >= r.b.hi || at + R <= r.b.lo) continue;
+                const int pg = fast_div(at, a.block_size, bs_magic);
+                int e = __ldg(bt + pg);
+                if (e < 0 || (a.num_blocks > 0 && e >= a.num_blocks)) {
+                    raise_status(GOLLEK_STATUS_BAD_BLOCK_ID);
+                    e = 0;
+                }
+                const int off = at - pg * a.block_size;
+                const long long first = e * p.page_rows + static_cast<long long>(r.h) * a.block_size + off;
+                if constexpr (Q8) {
+                    const long long so = e * a.scale_page_stride + r.h * a.scale_head_stride + off * a.scale_token_stride;
+                    if (k == 0)
+                        s2.loc.sc0 = so;
+                    else
+                        s2.loc.sc1 = so;
+                    if (page_scales) {
+                        (k == 0 ? s2.loc.ks0 : s2.loc.ks1) = __ldg(a.k_scales + so);
+                        (k == 0 ? s2.loc.vs0 : s2.loc.vs1) = __ldg(a.v_scales + so);
+                    }
+                }
+                const int at8 = static_cast<int>(Q8 ? first : first >> 3);
+                if (k == 0)
+                    s2.loc.row0 = at8;
+                else
+                    s2.loc.row1 = at8;
+            }
+            __syncwarp();
+            ++t;
+        }
+        // K of this tile, V of the tile before it in the run, V of the run's last tile
+#pragma unroll 1
+        for (int w = 0; w < 3 && s0.live && ok; ++w) {
+            if ((w == 1 && s0.first) || (w == 2 && !s0.last)) continue;
+            const Loc l = w == 1 ? before : s0.loc;
+            constexpr int kRing = Q8 ? L::kRaw : NS;
+            uint64_t *const r_full = Q8 ? raw_full : full, *const r_free = Q8 ? raw_free : empty;
+            if (copies >= kRing) ok = wait(&r_free[slot], ph);
+            if (!ok) break;
+            const unsigned boxes = (l.row0 >= 0) + (l.row1 >= 0);
+            constexpr int kRowBytes = Q8 ? D : 2 * D;
+            uint32_t bytes = __reduce_add_sync(0xffffffffu, boxes) * R * kRowBytes;
+            if constexpr (Q8) {
+                // with K: both scales of the tile, 16 positions a lane
+                if (w == 0 && !page_scales) bytes += __reduce_add_sync(0xffffffffu, boxes) * R * 8;
+                if (w == 0 && page_scales && lane < 8) {
+                    float *sk = reinterpret_cast<float *>(pipe.smem + L::scales) + sc_slot * 256 + lane * 16;
+                    for (int i = 0; i < 16; ++i) {
+                        sk[i] = i < R ? l.ks0 : l.ks1;
+                        sk[128 + i] = i < R ? l.vs0 : l.vs1;
+                    }
+                }
+                __syncwarp();
+            }
+            if (lane == 0) mbar_arrive_expect_tx(&r_full[slot], bytes);
+            __syncwarp();
+            const CUtensorMap *map = w ? &tm_v : &tm_k;
+            if constexpr (Q8) {
+                uint8_t *dst = pipe.smem + L::raw + slot * (L::kSlot / 2) + lane * (16 * D);
+                if (l.row0 >= 0) tma_load_2d(dst, map, 0, l.row0, &r_full[slot]);
+                if (l.row1 >= 0) tma_load_2d(dst + 8 * D, map, 0, l.row1, &r_full[slot]);
+                if (w == 0 && !page_scales) {
+                    float *sk = reinterpret_cast<float *>(pipe.smem + L::scales) + sc_slot * 256 + lane * 16;
+                    if (l.row0 >= 0) {
+                        bulk_load(sk, a.k_scales + l.sc0, R * 4, &r_full[slot]);
+                        bulk_load(sk + 128, a.v_scales + l.sc0, R * 4, &r_full[slot]);
+                    }
+                    if (l.row1 >= 0) {
+                        bulk_load(sk + 8, a.k_scales + l.sc1, R * 4, &r_full[slot]);
+                        bulk_load(sk + 136, a.v_scales + l.sc1, R * 4, &r_full[slot]);
+                    }
+                }
+                if (w == 0) sc_slot = sc_slot + 1 == L::kScales ? 0 : sc_slot + 1;
+            } else {
+                uint8_t *dst = pipe.smem + L::ring + slot * L::kSlot + lane * (16 * D * 2);
+                if (l.row0 >= 0) tma_load_4d(dst, map, 0, 0, 0, l.row0, &r_full[slot]);
+                if (l.row1 >= 0) tma_load_4d(dst + 8 * D * 2, map, 0, 0, 0, l.row1, &r_full[slot]);
+            }
+            ++copies;
+            if (++slot == kRing) {
+                slot = 0;
+                ph ^= 1;
+            }
+        }
+        before = s0.loc;
+        s0 = s1;
+        s1 = s2;
+    }
+    if (!ok && lane == 0) tile_give_up(abort);
+    // every copy issued lands before the shared memory is released
+    if (lane == 0)
+        for (int n = Q8 ? L::kRaw : NS, k = max(0, copies - n); k < copies; ++k)
+            mbar_wait(Q8 ? &raw_full[k % n] : &full[k % n], (k / n) & 1);
+    __syncwarp();
+}
+
+// Copies of the ring in order: 128 x D bytes to bf16 in the operand layout, 16 bytes a thread at a
+// time.  0x4300 | u is bf16 128 + u for u < 128, and 0x4300 | sign bit is 128 or 256: their
+// difference is the signed byte, without the conversion pipe that the exponentials use.
+template <typename L, int D, int THREADS>
+__device__ __forceinline__ void tile_converter(const TilePipe<L> &pipe, int me) {
+    constexpr int NS = L::kSlots;
+    const int lane = me & 31;
+    uint64_t *const full = pipe.full, *const empty = pipe.empty, *const run_full = pipe.run_full, *const run_free = pipe.run_free;
+    uint64_t *const raw_full = pipe.raw_full, *const raw_free = pipe.raw_free;
+    RunDesc *const runs = pipe.runs;
+    volatile int *const abort = pipe.abort;
+    auto wait = [&](uint64_t *bar, uint32_t phase) { return pipe.wait(bar, phase); };
+    int rs = 0, bs = 0;
+    uint32_t rph = 0, bph = 1;
+    bool ok = true;
+#pragma unroll 1
+    for (int run = 0; ok; ++run) {
+        const int at = run % L::kRuns;
+        if (!(ok = wait(&run_full[at], run / L::kRuns))) break;
+        const int n = runs[at].n;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&run_free[at]);
+        if (n == 0) break;
+#pragma unroll 1
+        for (int c = 0; c < 2 * n; ++c) {
+            ok = wait(&raw_full[rs], rph) && wait(&empty[bs], bph);
+            if (!ok) break;
+            const uint32_t src = smem_u32(pipe.smem + L::raw) + rs * (L::kSlot / 2);
+            const uint32_t dst = smem_u32(pipe.smem + L::ring) + bs * L::kSlot;
+            constexpr int C = D / 16;  // 16-byte pieces of a row
+#pragma unroll 4
+            for (int i = me; i < kTileTok * C; i += THREADS) {
+                const int tok = i / C, pc = i % C;
+                const uint4 w = lds_u4(src + i * 16);
+                uint32_t o[8];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t x = k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w;
+                    o[2 * k] = byte_pair<0x4140>(x);
+                    o[2 * k + 1] = byte_pair<0x4342>(x);
+                }
+                // the upper half of a row's threads stores its second chunk first: no two of eight
+                // lanes meet in a bank
+                const bool swap = pc >= C / 2;
+                const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+                sts_u4(dst + kv_chunk_off<D>(tok, 2 * pc + swap), swap ? hi : lo);
+                sts_u4(dst + kv_chunk_off<D>(tok, 2 * pc + !swap), swap ? lo : hi);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&full[bs]);
+                mbar_arrive(&raw_free[rs]);
+            }
+            if (++rs == L::kRaw) {
+                rs = 0;
+                rph ^= 1;
+            }
+            if (++bs == NS) {
+                bs = 0;
+                bph ^= 1;
+            }
+        }
+    }
+    if (!ok && lane == 0) tile_give_up(abort);
+}
+
 // FEAT: what is done to the scores besides scale and mask (kPlain, kBias: distance bias,
 // kCap: soft-cap, with or without bias); separate kernels, so that each one's code stays
 // short.
@@ -520,14 +831,11 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
     extern __shared__ __align__(1024) uint8_t tile_smem[];
     uint8_t *ring = tile_smem + L::ring;
     float *sm_ml = reinterpret_cast<float *>(tile_smem + L::ml);
-    RunDesc *runs = reinterpret_cast<RunDesc *>(tile_smem + L::runs);
-    uint64_t *full = reinterpret_cast<uint64_t *>(tile_smem + L::bars);
-    uint64_t *empty = full + NS;
-    uint64_t *raw_full = empty + NS;           // [kRaw] bytes of a tile (and, with K, its scales)
-    uint64_t *raw_free = raw_full + L::kRaw;   // [kRaw] converted
-    uint64_t *run_full = raw_free + L::kRaw;   // [kRuns] descriptor written
-    uint64_t *run_free = run_full + L::kRuns;  // [kRuns] descriptor read by the 10 (Q8: 14) warps that use it
-    uint64_t *s_full = run_free + L::kRuns;    // [2] scores in tensor memory (and every earlier MMA done)
+    const TilePipe<L> pipe(tile_smem);
+    RunDesc *const runs = pipe.runs;
+    uint64_t *const full = pipe.full, *const empty = pipe.empty, *const run_full = pipe.run_full, *const run_free = pipe.run_free;
+    volatile int *const abort = pipe.abort;
+    uint64_t *s_full = pipe.own;               // [2] scores in tensor memory (and every earlier MMA done)
     uint64_t *p_full = s_full + 2;             // [2] probabilities in tensor memory (V cleared, O rescaled)
     uint64_t *o_full = p_full + 2;             // [2] a run's last value MMA of the group done
     uint64_t *o_free = o_full + 2;             // [2] O read
@@ -536,23 +844,11 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
     uint64_t *drained = q_free + 2;            // [2] an issuer's MMAs done
     uint64_t *turn = drained + 2;              // [2][4] group t's warp may use the exponent pipe
     uint64_t *ml_full = turn + 8;              // group 1's (m, l) handed over
-    volatile int *abort = reinterpret_cast<volatile int *>(tile_smem + L::misc);
     uint32_t *sm_tmem = reinterpret_cast<uint32_t *>(tile_smem + L::misc + 4);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        for (int i = 0; i < NS; ++i) {
-            mbar_init(&full[i], Q8 ? 4 : 1);
-            mbar_init(&empty[i], 2);
-        }
-        for (int i = 0; i < L::kRaw; ++i) {
-            mbar_init(&raw_full[i], 1);
-            mbar_init(&raw_free[i], 4);
-        }
-        for (int i = 0; i < L::kRuns; ++i) {
-            mbar_init(&run_full[i], 1);
-            mbar_init(&run_free[i], Q8 ? 14 : 10);
-        }
+        pipe.init(Q8 ? 4 : 1, 2, Q8 ? 14 : 10);
         for (int t = 0; t < 2; ++t) {
             mbar_init(&s_full[t], 1);
             mbar_init(&p_full[t], 4);
@@ -565,7 +861,6 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
         for (int i = 0; i < 8; ++i) mbar_init(&turn[i], 1);
         mbar_init(ml_full, 4);
         fence_barrier_init();
-        *abort = 0;
     }
     if (Q8 && tid < 128) reinterpret_cast<float *>(tile_smem + L::ones)[tid] = 1.f;
     if (warp == 9 && lane == 0) {
@@ -580,229 +875,15 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *sm_tmem;
-    const uint32_t abort_s = smem_u32(tile_smem + L::misc);
-    auto wait = [&](uint64_t *bar, uint32_t phase) { return tile_wait(smem_u32(bar), phase & 1, abort_s); };
+    auto wait = [&](uint64_t *bar, uint32_t phase) { return pipe.wait(bar, phase); };
 
     if (warp >= 8) {
         if (warp == 9) {
             // ===================================================================== producer
-            // Walks the runs, hands their descriptors out and copies their tiles; the page lookups go
-            // two tiles ahead of the copies, across runs.
-            pdl_wait();  // the plan is complete
-            RunIter it;
-            it.begin(p, blockIdx.x);
-            TileRun r{};
-            using Loc = std::conditional_t<Q8, PageLocQ8, PageLoc>;
-            struct Step {
-                Loc loc;
-                bool live, first, last;
-            };
-            const int R = a.block_size < 16 ? a.block_size : 16;
-            const unsigned bs_magic = div_magic(a.block_size);
-            const int *bt = nullptr;
-            int t = 0, tb = 0, ta = 0, nrun = 0;
-            int slot = 0, copies = 0;
-            uint32_t ph = 1;
-            bool ok = true, more = true;
-            Step s0{{-1, -1}, false, false, false}, s1 = s0;
-            Loc before{-1, -1};
-            [[maybe_unused]] int sc_slot = 0;  // scales of the tile copied next
-            [[maybe_unused]] const bool page_scales = a.scale_token_stride == 0;
-            // ring order of a run: K0, K1, V0, K2, V1, ... V(n-1) (v_at).  The first two rounds only fill
-            // the look-ahead; each part of the code stands here once, to keep it short.
-#pragma unroll 1
-            for (int round = 0; ok && (round < 2 || s0.live); ++round) {
-                Step s2{{-1, -1}, false, false, false};
-                if (t >= tb && more) {
-                    // the next run: its descriptor for the other warps, its table
-                    more = it.next(p, r);
-                    const int at = nrun % L::kRuns;
-                    if (nrun >= L::kRuns) ok = wait(&run_free[at], nrun / L::kRuns - 1);
-                    if (lane == 0 && ok) {
-                        RunDesc &d = runs[at];
-                        d.tok0 = r.b.tok0;
-                        d.row0 = r.b.row0;
-                        d.nrows = r.b.nrows;
-                        d.h = r.h;
-                        d.lo = r.b.lo;
-                        d.hi = r.b.hi;
-                        d.tile0 = r.b.lo / kTileTok + r.tb - 1;
-                        d.n = more ? r.tb - r.ta : 0;
-                        d.tab = r.b.tab;
-                        d.len = r.b.len;
-                        d.pos0 = r.b.pos0;
-                        d.flags = r.b.kind | (r.ta == 0 && r.tb == r.n ? 4 : 0) | (r.ta == 0 ? 8 : 0);
-                        mbar_arrive(&run_full[at]);
-                    }
-                    __syncwarp();
-                    ++nrun;
-                    bt = r.b.kind == kPrefix ? a.prefix_tables + static_cast<long long>(r.b.tab) * a.max_pblocks
-                                             : a.block_tables + static_cast<long long>(r.b.tab) * a.max_blocks;
-                    t = ta = r.ta;
-                    tb = more ? r.tb : r.ta;
-                }
-                if (t < tb) {
-                    s2.live = true;
-                    s2.first = t == ta;
-                    s2.last = t == tb - 1;
-                    // pool rows / 8 of the lane's box(es); -1: nothing to load there
-                    int at = (r.b.lo / kTileTok + tb - 1 - (t - ta)) * kTileTok + lane * 16;
-#pragma unroll 1
-                    for (int k = 0; k < 16; k += R, at += R) {
-                        if (lane >= 8 || at >= r.b.hi || at + R <= r.b.lo) continue;
-                        const int pg = fast_div(at, a.block_size, bs_magic);
-                        int e = __ldg(bt + pg);
-                        if (e < 0 || (a.num_blocks > 0 && e >= a.num_blocks)) {
-                            raise_status(GOLLEK_STATUS_BAD_BLOCK_ID);
-                            e = 0;
-                        }
-                        const int off = at - pg * a.block_size;
-                        const long long first = e * p.page_rows + static_cast<long long>(r.h) * a.block_size + off;
-                        if constexpr (Q8) {
-                            const long long so = e * a.scale_page_stride + r.h * a.scale_head_stride + off * a.scale_token_stride;
-                            if (k == 0)
-                                s2.loc.sc0 = so;
-                            else
-                                s2.loc.sc1 = so;
-                            if (page_scales) {
-                                (k == 0 ? s2.loc.ks0 : s2.loc.ks1) = __ldg(a.k_scales + so);
-                                (k == 0 ? s2.loc.vs0 : s2.loc.vs1) = __ldg(a.v_scales + so);
-                            }
-                        }
-                        const int at8 = static_cast<int>(Q8 ? first : first >> 3);
-                        if (k == 0)
-                            s2.loc.row0 = at8;
-                        else
-                            s2.loc.row1 = at8;
-                    }
-                    __syncwarp();
-                    ++t;
-                }
-                // K of this tile, V of the tile before it in the run, V of the run's last tile
-#pragma unroll 1
-                for (int w = 0; w < 3 && s0.live && ok; ++w) {
-                    if ((w == 1 && s0.first) || (w == 2 && !s0.last)) continue;
-                    const Loc l = w == 1 ? before : s0.loc;
-                    constexpr int kRing = Q8 ? L::kRaw : NS;
-                    uint64_t *const r_full = Q8 ? raw_full : full, *const r_free = Q8 ? raw_free : empty;
-                    if (copies >= kRing) ok = wait(&r_free[slot], ph);
-                    if (!ok) break;
-                    const unsigned boxes = (l.row0 >= 0) + (l.row1 >= 0);
-                    constexpr int kRowBytes = Q8 ? D : 2 * D;
-                    uint32_t bytes = __reduce_add_sync(0xffffffffu, boxes) * R * kRowBytes;
-                    if constexpr (Q8) {
-                        // with K: both scales of the tile, 16 positions a lane
-                        if (w == 0 && !page_scales) bytes += __reduce_add_sync(0xffffffffu, boxes) * R * 8;
-                        if (w == 0 && page_scales && lane < 8) {
-                            float *sk = reinterpret_cast<float *>(tile_smem + L::scales) + sc_slot * 256 + lane * 16;
-                            for (int i = 0; i < 16; ++i) {
-                                sk[i] = i < R ? l.ks0 : l.ks1;
-                                sk[128 + i] = i < R ? l.vs0 : l.vs1;
-                            }
-                        }
-                        __syncwarp();
-                    }
-                    if (lane == 0) mbar_arrive_expect_tx(&r_full[slot], bytes);
-                    __syncwarp();
-                    const CUtensorMap *map = w ? &tm_v : &tm_k;
-                    if constexpr (Q8) {
-                        uint8_t *dst = tile_smem + L::raw + slot * (L::kSlot / 2) + lane * (16 * D);
-                        if (l.row0 >= 0) tma_load_2d(dst, map, 0, l.row0, &r_full[slot]);
-                        if (l.row1 >= 0) tma_load_2d(dst + 8 * D, map, 0, l.row1, &r_full[slot]);
-                        if (w == 0 && !page_scales) {
-                            float *sk = reinterpret_cast<float *>(tile_smem + L::scales) + sc_slot * 256 + lane * 16;
-                            if (l.row0 >= 0) {
-                                bulk_load(sk, a.k_scales + l.sc0, R * 4, &r_full[slot]);
-                                bulk_load(sk + 128, a.v_scales + l.sc0, R * 4, &r_full[slot]);
-                            }
-                            if (l.row1 >= 0) {
-                                bulk_load(sk + 8, a.k_scales + l.sc1, R * 4, &r_full[slot]);
-                                bulk_load(sk + 136, a.v_scales + l.sc1, R * 4, &r_full[slot]);
-                            }
-                        }
-                        if (w == 0) sc_slot = sc_slot + 1 == L::kScales ? 0 : sc_slot + 1;
-                    } else {
-                        uint8_t *dst = ring + slot * L::kSlot + lane * (16 * D * 2);
-                        if (l.row0 >= 0) tma_load_4d(dst, map, 0, 0, 0, l.row0, &r_full[slot]);
-                        if (l.row1 >= 0) tma_load_4d(dst + 8 * D * 2, map, 0, 0, 0, l.row1, &r_full[slot]);
-                    }
-                    ++copies;
-                    if (++slot == kRing) {
-                        slot = 0;
-                        ph ^= 1;
-                    }
-                }
-                before = s0.loc;
-                s0 = s1;
-                s1 = s2;
-            }
-            if (!ok && lane == 0) tile_give_up(abort);
-            // every copy issued lands before the shared memory is released
-            if (lane == 0)
-                for (int n = Q8 ? L::kRaw : NS, k = max(0, copies - n); k < copies; ++k)
-                    mbar_wait(Q8 ? &raw_full[k % n] : &full[k % n], (k / n) & 1);
-            __syncwarp();
+            tile_producer<L, D, Q8>(p, pipe, tm_k, tm_v, lane);
         } else if (Q8 && warp >= 12) {
             // ===================================================================== converters
-            // Copies of the ring in order: 128 x D bytes to bf16 in the operand layout, 16 bytes a thread at a
-            // time.  0x4300 | u is bf16 128 + u for u < 128, and 0x4300 | sign bit is 128 or 256: their
-            // difference is the signed byte, without the conversion pipe that the exponentials use.
-            if constexpr (Q8) {
-                const int me = tid - 384;
-                int rs = 0, bs = 0;
-                uint32_t rph = 0, bph = 1;
-                bool ok = true;
-#pragma unroll 1
-                for (int run = 0; ok; ++run) {
-                    const int at = run % L::kRuns;
-                    if (!(ok = wait(&run_full[at], run / L::kRuns))) break;
-                    const int n = runs[at].n;
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&run_free[at]);
-                    if (n == 0) break;
-#pragma unroll 1
-                    for (int c = 0; c < 2 * n; ++c) {
-                        ok = wait(&raw_full[rs], rph) && wait(&empty[bs], bph);
-                        if (!ok) break;
-                        const uint32_t src = smem_u32(tile_smem + L::raw) + rs * (L::kSlot / 2);
-                        const uint32_t dst = smem_u32(ring) + bs * L::kSlot;
-                        constexpr int C = D / 16;  // 16-byte pieces of a row
-#pragma unroll 4
-                        for (int i = me; i < kTileTok * C; i += 128) {
-                            const int tok = i / C, pc = i % C;
-                            const uint4 w = lds_u4(src + i * 16);
-                            uint32_t o[8];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const uint32_t x = k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w;
-                                o[2 * k] = byte_pair<0x4140>(x);
-                                o[2 * k + 1] = byte_pair<0x4342>(x);
-                            }
-                            // the upper half of a row's threads stores its second chunk first: no two of eight
-                            // lanes meet in a bank
-                            const bool swap = pc >= C / 2;
-                            const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
-                            sts_u4(dst + kv_chunk_off<D>(tok, 2 * pc + swap), swap ? hi : lo);
-                            sts_u4(dst + kv_chunk_off<D>(tok, 2 * pc + !swap), swap ? lo : hi);
-                        }
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0) {
-                            mbar_arrive(&full[bs]);
-                            mbar_arrive(&raw_free[rs]);
-                        }
-                        if (++rs == L::kRaw) {
-                            rs = 0;
-                            rph ^= 1;
-                        }
-                        if (++bs == NS) {
-                            bs = 0;
-                            bph ^= 1;
-                        }
-                    }
-                }
-                if (!ok && lane == 0) tile_give_up(abort);
-            }
+            if constexpr (Q8) tile_converter<L, D, 128>(pipe, tid - 384);
         } else if (warp == 8 || warp == 10) {
             // ===================================================================== MMA issuers
             // Warp 8 issues group 0's MMAs, warp 10 group 1's: what one waits for does not hold the
@@ -1005,31 +1086,9 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
                     }
                 }
                 if constexpr (FEAT == kCap) {
-                    // cap tanh(y), y = score / cap: on the FMA pipe where |y| <= 1/2 in the whole warp
-                    // (the usual case: caps are several times the scores), an odd polynomial of relative
-                    // error below 2^-22; else cap - 2 cap / (1 + e^2y), two exponent-pipe operations
-                    float big_y = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        w[i] *= cap1;
-                        big_y = fmaxf(big_y, fabsf(w[i]));
-                    }
-                    if (__any_sync(0xffffffffu, !(big_y <= 0.5f))) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            w[i] = fmaf(-2.f, __fdividef(1.f, 1.f + fast_exp2(w[i] * (2.f * kLog2e))), 1.f);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float2 y = make_float2(w[i], w[i + 1]), y2 = mul2(y, y);
-                            float2 q = fma2(y2, pair(0.01724149100482f), pair(-0.05304549261928f));
-                            q = fma2(q, y2, pair(0.13325878977776f));
-                            q = fma2(q, y2, pair(-0.33333143591881f));
-                            q = fma2(mul2(q, y2), y, y);
-                            w[i] = q.x;
-                            w[i + 1] = q.y;
-                        }
-                    }
+                    for (int i = 0; i < 32; ++i) w[i] *= cap1;
+                    unit_cap(w);
                 }
                 const float f = FEAT == kCap ? cap2 : a.q_scale;
                 const int l0 = jlo - k, h0 = jhi - k;

@@ -2,6 +2,7 @@
 // cache read-back: argument checks, kernel selection and their C ABI (gollek_kernels.h).
 #include <algorithm>
 
+#include "attn_rows.cuh"
 #include "attn_tile.cuh"
 #include "host.cuh"
 #include "kv_gather.cuh"
@@ -138,6 +139,21 @@ int encode_byte_map(CUtensorMap *m, const void *base, int D, long long rows, int
     return GOLLEK_OK;
 }
 
+// Whether a varlen call goes to the kernel for few rows: its sequences have 16 rows at most on
+// average (a longer one is cut into blocks of 16, each of which reads its pages).
+bool few_rows(int num_groups, int num_seqs, int total_q, int G, int D) {
+    return num_groups == 0 && D == kFewD && G <= kFewRows && static_cast<long long>(total_q) * G <= static_cast<long long>(num_seqs) * kFewRows;
+}
+
+// The workspace of a call; *blk_rows receives the rows of its blocks.
+TileWs attn_ws(int num_groups, int num_seqs, int total_q, int hq, int hkv, int D, int *blk_rows) {
+    const int G = hq / hkv;
+    const bool shared = num_groups > 0;
+    *blk_rows = few_rows(num_groups, num_seqs, total_q, G, D) ? kFewRows : kBlkRows;
+    return tile_ws(tile_entities(num_groups, num_seqs), tile_rows(total_q, G, shared), *blk_rows,
+                   static_cast<long long>(total_q) * hq, D, shared);
+}
+
 // A launch that may begin before the kernel in front of it has ended (that kernel's results are
 // read behind griddepcontrol.wait).
 int launch_dependent(const void *fn, dim3 grid, int threads, size_t smem, cudaStream_t st, void **args, const char *what) {
@@ -158,16 +174,25 @@ int launch_dependent(const void *fn, dim3 grid, int threads, size_t smem, cudaSt
 template <typename T, int D, bool Q8 = false>
 int launch_tile_as(TileArgs &p, const CUtensorMap &tmk, const CUtensorMap &tmv, cudaStream_t st) {
     const AttnArgs &a = p.a;
-    constexpr uint32_t smem = TileSmem<D, Q8>::total;
-    static_assert(smem <= 227 * 1024, "shared memory of the tile kernel");
+    uint32_t smem = TileSmem<D, Q8>::total;
+    static_assert(TileSmem<D, Q8>::total <= 227 * 1024, "shared memory of the tile kernel");
     const void *fn = a.soft_cap > 0.f ? reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kCap, Q8>)
                      : a.slopes       ? reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kBias, Q8>)
                                       : reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kPlain, Q8>);
+    int threads = Q8 ? kTileThreadsQ8 : kTileThreads;
+    if constexpr (D == kFewD) {
+        static_assert(RowsSmem<Q8>::total <= 227 * 1024, "shared memory of the kernel for few rows");
+        if (p.blk_rows == kFewRows) {
+            smem = RowsSmem<Q8>::total;
+            fn = reinterpret_cast<const void *>(&attn_rows_kernel<T, Q8>);
+            threads = kRowsThreads + (Q8 ? kRowsConverters : 0);
+        }
+    }
     GK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute");
     tile_plan_kernel<<<1, kPlanThreads, 0, st>>>(p);
     GK_CUDA(cudaGetLastError(), "tile_plan_kernel launch");
     void *args[] = {const_cast<CUtensorMap *>(&tmk), const_cast<CUtensorMap *>(&tmv), &p};
-    int rc = launch_dependent(fn, dim3(p.grid), Q8 ? kTileThreadsQ8 : kTileThreads, smem, st, args, "attn_tile_kernel launch");
+    int rc = launch_dependent(fn, dim3(p.grid), threads, smem, st, args, "attn_tile_kernel launch");
     if (rc) return rc;
     void *margs[] = {&p};
     if (a.num_groups == 0)
@@ -180,12 +205,9 @@ int launch_tile_as(TileArgs &p, const CUtensorMap &tmk, const CUtensorMap &tmv, 
 }
 
 int launch_tile(AttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
-    const bool shared = a.num_groups > 0;
-    const int G = a.num_q_heads / a.num_kv_heads;
     TileArgs p{};
     p.entities = a.num_groups + a.num_seqs;
-    const TileWs w = tile_ws(tile_entities(a.num_groups, a.num_seqs), tile_rows(a.total_q, G, shared),
-                             static_cast<long long>(a.total_q) * a.num_q_heads, a.head_dim, shared);
+    const TileWs w = attn_ws(a.num_groups, a.num_seqs, a.total_q, a.num_q_heads, a.num_kv_heads, a.head_dim, &p.blk_rows);
     if (w.max_blocks > (1LL << 22)) return fail(GOLLEK_ERR_UNSUPPORTED, "too many query rows for one call");
     int dev = 0;
     GK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
@@ -235,8 +257,8 @@ int launch_attn(AttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
 
 size_t attn_workspace(int num_groups, int num_seqs, int total_q, int hq, int hkv, int D) {
     if (num_seqs <= 0 || total_q <= 0 || num_groups < 0 || hkv <= 0 || hq <= 0 || hq % hkv || D <= 0) return 0;
-    return tile_ws(tile_entities(num_groups, num_seqs), tile_rows(total_q, hq / hkv, num_groups > 0),
-                   static_cast<long long>(total_q) * hq, D, num_groups > 0).total;
+    int blk_rows;
+    return attn_ws(num_groups, num_seqs, total_q, hq, hkv, D, &blk_rows).total;
 }
 
 template <int KV>

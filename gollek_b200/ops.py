@@ -5,6 +5,7 @@ and the current torch stream; none has a CPU path.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -12,6 +13,7 @@ import torch
 from . import _lib
 from ._lib import BF16, F16, F32, I4, I8, check
 
+_FLOAT = (torch.float32, torch.bfloat16, torch.float16)
 _TORCH_DTYPE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, torch.int8: I8}
 
 
@@ -131,15 +133,14 @@ def kv_append(key, value, token_pos, block_tables, k_cache, v_cache, *, block_si
     check(rc)
 
 
-def _check(name, t, shape=None, dtype=None, device=None, optional=False, packed=True):
-    """Shape, type, device and layout of one argument of the functions below."""
+def _check(name, t, shape, dtype, device, packed=True):
+    """Shape (None: any size), type (None: any), device and layout of one argument; says what
+    is wrong with it."""
     if t is None:
-        if optional:
-            return
         raise ValueError(f"{name} is required")
-    if not t.is_cuda:
+    if t.device.type != "cuda":
         raise ValueError("gollek_b200 ops take CUDA tensors only (no CPU path)")
-    if device is not None and t.device != device:
+    if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not {device}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
@@ -149,6 +150,22 @@ def _check(name, t, shape=None, dtype=None, device=None, optional=False, packed=
                          f"not {tuple(t.shape)}")
     if packed and not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+
+
+def _check_vectors(device, rows):
+    """_check of 1-D arguments, (name, tensor, length, dtype) each, None tensors skipped: the
+    common case in as few Python steps as possible, since small calls wait for them."""
+    for name, t, n, dtype in rows:
+        if t is not None and not (t.dtype is dtype and t.shape == (n,) and t.device == device
+                                  and t.is_contiguous()):
+            _check(name, t, (n,), dtype, device)
+
+
+def _first(name, t, dims):
+    """The argument that fixes the device: a contiguous CUDA tensor of `dims` dimensions."""
+    if t is None or t.device.type != "cuda" or t.dim() != dims or not t.is_contiguous():
+        _check(name, t, (None,) * dims, None, None if t is None else t.device)
+    return t.device
 
 
 def _behind(t):
@@ -163,7 +180,8 @@ def _check_pool(k_cache, v_cache, k_scales, v_scales, scale_strides, num_kv_head
     pages (scales too) when that is given.  With page_stride the tensors are base pointers
     (one layer of a larger pool); without it they are whole and contiguous."""
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        _check(name, t, device=device, packed=not page_stride)
+        if t is None or t.device != device or not (page_stride or t.is_contiguous()):
+            _check(name, t, None, None, device, packed=not page_stride)
         if int4:
             if t.dtype not in (torch.uint8, torch.int8):
                 raise ValueError(f"an int4 {name} is a tensor of bytes, not {t.dtype}")
@@ -172,14 +190,16 @@ def _check_pool(k_cache, v_cache, k_scales, v_scales, scale_strides, num_kv_head
     if k_cache.dtype != v_cache.dtype:
         raise ValueError("k_cache and v_cache have different types")
     for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
-        _check(name, t, dtype=torch.float32, device=device, optional=True, packed=False)
+        if t is not None and (t.dtype is not torch.float32 or t.device != device):
+            _check(name, t, None, torch.float32, device, packed=False)
     if num_blocks > 0 and num_kv_heads > 0 and block_size > 0 and head_dim > 0:
         page = num_kv_heads * block_size * head_dim
         need = (num_blocks - 1) * (page_stride or page) + page
         for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-            if _behind(t) * (2 if int4 else 1) < need:
+            have = _behind(t) if page_stride else t.numel()
+            if have * (2 if int4 else 1) < need:
                 raise ValueError(f"{name} is smaller than {num_blocks} pages")
-        if int4 or k_cache.dtype == torch.int8:
+        if int4 or k_cache.dtype is torch.int8:
             sps, shs, sts = scale_strides
             last = (num_blocks - 1) * sps + (num_kv_heads - 1) * shs + (block_size - 1) * sts
             for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
@@ -216,12 +236,12 @@ def _scratch(need, workspace, device):
     """The caller's workspace (checked), or a fresh one from torch's allocator: stream
     ordered, and private to a captured graph."""
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    else:
-        _check("workspace", workspace, device=device)
-    return workspace, 0 if workspace is None else workspace.numel() * workspace.element_size()
+        return torch.empty(need, dtype=torch.uint8, device=device) if need else None, need
+    _check("workspace", workspace, None, None, device)
+    return workspace, workspace.numel() * workspace.element_size()
 
 
+@functools.lru_cache(maxsize=1024)
 def varlen_workspace_size(num_seqs, total_queries, num_q_heads, num_kv_heads, head_dim) -> int:
     return int(_lib.load().gollek_paged_attention_varlen_workspace_size(
         num_seqs, total_queries, num_q_heads, num_kv_heads, head_dim))
@@ -240,19 +260,21 @@ def paged_attention_varlen(q, k_cache, v_cache, block_tables, cu_seqlens_q, cont
     sequence's first positions visible to all its queries; token_starts [total] is the first
     position each query may attend.  Rows of `out` in no sequence are not written.
     """
-    _check("q", q, (None, None, None))
-    dev = q.device
+    dev = _first("q", q, 3)
     total, Hq, D = q.shape
-    if q.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    if q.dtype not in _FLOAT:
         raise ValueError(f"unsupported q dtype {q.dtype}")
     _check("block_tables", block_tables, (None, None), torch.int32, dev)
-    S = block_tables.shape[0]
-    _check("cu_seqlens_q", cu_seqlens_q, (S + 1,), torch.int32, dev)
-    _check("context_lens", context_lens, (S,), torch.int32, dev)
-    _check("alibi_slopes", alibi_slopes, (Hq,), torch.float32, dev, optional=True)
-    _check("prefix_lens", prefix_lens, (S,), torch.int32, dev, optional=True)
-    _check("token_starts", token_starts, (total,), torch.int32, dev, optional=True)
-    _check("out", out, tuple(q.shape), q.dtype, dev, optional=True)
+    S, width = block_tables.shape
+    _check_vectors(dev, (("cu_seqlens_q", cu_seqlens_q, S + 1, torch.int32),
+                         ("context_lens", context_lens, S, torch.int32),
+                         ("alibi_slopes", alibi_slopes, Hq, torch.float32),
+                         ("prefix_lens", prefix_lens, S, torch.int32),
+                         ("token_starts", token_starts, total, torch.int32)))
+    if cu_seqlens_q is None or context_lens is None:
+        raise ValueError("cu_seqlens_q and context_lens are required")
+    if out is not None:
+        _check("out", out, q.shape, q.dtype, dev)
     _check_pool(k_cache, v_cache, k_scales, v_scales, scale_strides, int(num_kv_heads), D,
                 int(block_size), int(num_blocks), int(page_stride), int4, dev)
     if scale is None:
@@ -268,13 +290,14 @@ def paged_attention_varlen(q, k_cache, v_cache, block_tables, cu_seqlens_q, cont
             _ptr(out), _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales), _ptr(v_scales),
             _ptr(block_tables), _ptr(cu_seqlens_q), _ptr(context_lens), _ptr(alibi_slopes),
             _ptr(prefix_lens), _ptr(token_starts), S, total, Hq, int(num_kv_heads), D,
-            int(block_size), block_tables.shape[1], int(num_blocks), int(page_stride),
+            int(block_size), width, int(num_blocks), int(page_stride),
             _TORCH_DTYPE[q.dtype], kv_dtype_code(k_cache, int4), int(sps), int(shs), int(sts),
             float(scale), float(soft_cap), int(sliding_window), int(bool(causal)), _ptr(ws),
             nbytes, st))
     return out
 
 
+@functools.lru_cache(maxsize=1024)
 def shared_prefix_workspace_size(num_groups, num_seqs, num_q_heads, num_kv_heads, head_dim) -> int:
     return int(_lib.load().gollek_paged_attention_shared_prefix_workspace_size(
         num_groups, num_seqs, num_q_heads, num_kv_heads, head_dim))
@@ -289,18 +312,20 @@ def paged_attention_shared_prefix(q, k_cache, v_cache, prefix_tables, prefix_len
     q [S, Hq, D] fp32/bf16/f16; sequences group_starts[g] .. group_starts[g+1] - 1 attend the
     prefix_lens[g] tokens of prefix_tables[g], read once for the group, and then their own
     context_lens[s] tokens."""
-    _check("q", q, (None, None, None))
-    dev = q.device
+    dev = _first("q", q, 3)
     S, Hq, D = q.shape
-    if q.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    if q.dtype not in _FLOAT:
         raise ValueError(f"unsupported q dtype {q.dtype}")
     _check("prefix_tables", prefix_tables, (None, None), torch.int32, dev)
     groups = prefix_tables.shape[0]
-    _check("prefix_lens", prefix_lens, (groups,), torch.int32, dev)
-    _check("group_starts", group_starts, (groups + 1,), torch.int32, dev)
     _check("block_tables", block_tables, (S, None), torch.int32, dev)
-    _check("context_lens", context_lens, (S,), torch.int32, dev)
-    _check("out", out, tuple(q.shape), q.dtype, dev, optional=True)
+    _check_vectors(dev, (("prefix_lens", prefix_lens, groups, torch.int32),
+                         ("group_starts", group_starts, groups + 1, torch.int32),
+                         ("context_lens", context_lens, S, torch.int32)))
+    if prefix_lens is None or group_starts is None or context_lens is None:
+        raise ValueError("prefix_lens, group_starts and context_lens are required")
+    if out is not None:
+        _check("out", out, q.shape, q.dtype, dev)
     _check_pool(k_cache, v_cache, k_scales, v_scales, scale_strides, int(num_kv_heads), D,
                 int(block_size), int(num_blocks), int(page_stride), int4, dev)
     if scale is None:
@@ -329,16 +354,18 @@ def kv_gather(k_cache, v_cache, token_pos, block_tables, *, num_kv_heads, head_d
     """Read rows of the cache back (gollek_kv_gather): (key, value), each [T, Hkv, head_dim] of
     `dtype` (fp32/bf16/f16), dequantised; row i is position token_pos[i] of sequence
     token_seq[i] (default: i)."""
-    _check("token_pos", token_pos, (None,), torch.int32)
-    dev = token_pos.device
+    dev = _first("token_pos", token_pos, 1)
     T = token_pos.shape[0]
-    _check("token_seq", token_seq, (T,), torch.int32, dev, optional=True)
+    _check_vectors(dev, (("token_pos", token_pos, T, torch.int32),
+                         ("token_seq", token_seq, T, torch.int32)))
     _check("block_tables", block_tables, (None, None), torch.int32, dev)
-    if dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    if dtype not in _FLOAT:
         raise ValueError(f"unsupported output dtype {dtype}")
     shape = (T, int(num_kv_heads), int(head_dim))
-    _check("key", key, shape, dtype, dev, optional=True)
-    _check("value", value, shape, dtype, dev, optional=True)
+    if key is not None:
+        _check("key", key, shape, dtype, dev)
+    if value is not None:
+        _check("value", value, shape, dtype, dev)
     _check_pool(k_cache, v_cache, k_scales, v_scales, scale_strides, int(num_kv_heads),
                 int(head_dim), int(block_size), int(num_blocks), int(page_stride), int4, dev)
     sps, shs, sts = scale_strides
