@@ -21,7 +21,7 @@ namespace gk {
 
 constexpr int kFewRows = 16;
 constexpr int kFewD = 128;             // the value product's M
-constexpr int kRowsThreads = 320;      // 8 row warps, the MMA issuer, the producer
+constexpr int kRowsThreads = 352;      // 8 row warps, the MMA issuer, 2 producers
 constexpr int kRowsConverters = 128;   // more for int8 caches
 
 template <bool Q8>
@@ -30,8 +30,8 @@ struct RowsSmem {
     static constexpr uint32_t kSlot = kTileTok * D * 2;
     static constexpr uint32_t kQ = kFewRows * D * 2;
     static constexpr uint32_t kP = kFewRows * kTileTok * 2;
-    static constexpr int kSlots = Q8 ? 3 : 6;
-    static constexpr int kRaw = Q8 ? 6 : 0;
+    static constexpr int kSlots = Q8 ? 4 : 6;
+    static constexpr int kRaw = Q8 ? 4 : 0;
     static constexpr int kScales = Q8 ? 8 : 0;  // copies are at most 5 tiles ahead of a tile in use
     static constexpr int kRuns = 4;
     static constexpr uint32_t q = 0;                              // [2]
@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kRowsThreads + (Q8 ? kRowsConverters : 0), 1)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         constexpr int conv = kRowsConverters / 32;
-        pipe.init(Q8 ? conv : 1, 1, 9 + (Q8 ? conv : 0));
+        pipe.init(Q8 ? conv : 2, 1, 9 + (Q8 ? conv : 0));
         for (int t = 0; t < 2; ++t) {
             mbar_init(&s_full[t], 1);
             mbar_init(&p_full[t], 4);
@@ -112,10 +112,13 @@ __global__ void __launch_bounds__(kRowsThreads + (Q8 ? kRowsConverters : 0), 1)
     const uint32_t tmem = *sm_tmem;
     auto wait = [&](uint64_t *bar, uint32_t phase) { return pipe.wait(bar, phase); };
 
-    if (warp == 9) {
-        tile_producer<L, D, Q8>(p, pipe, tm_k, tm_v, lane);
-    } else if (warp > 9) {
-        if constexpr (Q8) tile_converter<L, D, kRowsConverters>(pipe, tid - 320);
+    if (warp == 9 || warp == 10) {
+        tile_producer<L, D, Q8>(p, pipe, tm_k, tm_v, lane, warp - 9);
+    } else if (warp > 10) {
+        if constexpr (Q8) {
+            static_assert(L::kRaw == L::kSlots, "see tile_converter");
+            tile_converter<L, D, kRowsConverters, true>(pipe, tid - kRowsThreads);
+        }
     } else if (warp == 8) {
         // ===================================================================== MMA issuer
         // Tiles alternate between the groups; step j has the values of tile j - 2 and the scores of
@@ -300,6 +303,19 @@ __global__ void __launch_bounds__(kRowsThreads + (Q8 ? kRowsConverters : 0), 1)
                     if (!inside)
 #pragma unroll 4
                         for (int ch = 0; ch < D / 8; ++ch) sts_u4(vt + kv_chunk_off<D>(row, ch), make_uint4(0, 0, 0, 0));
+                }
+                if constexpr (Q8) {
+                    // V is this group's to convert (K the converter warps'): its slot is free, since the
+                    // scores' commit covers the MMAs four copies back
+                    const int cv = c0 + v_at(j, n);
+                    ok = wait(&empty[cv % NS], cv / NS - 1) && wait(&pipe.raw_full[cv % NS], cv / NS);
+                    if (!ok) break;
+                    convert_tile<D, 128>(smem_u32(tile_smem + L::raw) + cv % NS * (L::kSlot / 2), smem_u32(ring) + cv % NS * L::kSlot, row);
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(&full[cv % NS]);
+                        mbar_arrive(&pipe.raw_free[cv % NS]);
+                    }
                 }
                 float f = a.q_scale;
                 [[maybe_unused]] float fv = 1.f;

@@ -41,7 +41,7 @@ constexpr int kTileTok = 128;
 constexpr int kBlkRows = 256;
 constexpr int kRunCostTiles = 2;      // start-up of a run (q, pipeline fill, output), in tiles
 constexpr int kMaxTileCtas = 160;
-constexpr int kTileThreads = 384;     // 8 row warps, 2 MMA issuers, 1 producer, 1 idle
+constexpr int kTileThreads = 384;     // 8 row warps, 2 MMA issuers, 2 producers
 constexpr int kTileThreadsQ8 = 512;   // int8 caches: a fourth warpgroup converts
 // Scores may pass their row's reference by this much (log2 units) before it moves: P stays far
 // below the largest number of its type, and sums of it below fp32's.
@@ -414,6 +414,15 @@ __device__ __forceinline__ void sts_u2(uint32_t addr, T v) {
     asm volatile("st.shared.b16 [%0], %1;" ::"r"(addr), "h"(reinterpret_cast<const unsigned short &>(v)) : "memory");
 }
 
+// 16 bytes (4 bytes) of global memory into shared memory, asynchronously.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // x / d for 0 <= x < 2^31: the magic's quotient is at most one too large.
 __device__ __forceinline__ unsigned div_magic(int d) { return d == 1 ? 0u : 0xFFFFFFFFu / d + 1; }
 __device__ __forceinline__ int fast_div(int x, int d, unsigned magic) {
@@ -523,16 +532,19 @@ __device__ __forceinline__ uint32_t kv_chunk_off(int tok, int ch) {
     return static_cast<uint32_t>((tok >> 3) * (16 * D) + (ch >> 3) * 1024 + r8 * 128 + (((ch & 7) ^ r8) << 4));
 }
 
-// Page lookups and TMA boxes of a run's tiles: lane g < 8 owns the 16 positions 16 g .. of
-// each tile (one box; two of 8 rows where pages hold 8).
-struct PageLoc {
-    int row0, row1;  // first pool row of the box (16-bit caches: / 8), or -1
+// What lane g < 8 copies of the 16 positions 16 g .. of a tile: two halves of 8, in one page or
+// (pages of 8) in one each.  `entry`: the pages' table entries, looked up two tiles ahead;
+// resolved one tile ahead.
+struct PageEntry {
+    int e0, e1, off0, off1;  // off < 0: nothing to load there
+    int h;
 };
-// int8 caches: also the box's scales - where they are, or, one per page, what they are.
+struct PageLoc {
+    int row0, row1;  // first pool row of the half / 8, or -1
+};
+// int8 caches: the first row itself, and where the half's scales are.
 struct PageLocQ8 {
-    int row0, row1;
-    long long sc0, sc1;
-    float ks0, vs0, ks1, vs1;
+    long long row0, row1, sc0, sc1;
 };
 
 // Ring positions, from the run's first, of K and V of tile j of n: a value product follows
@@ -569,7 +581,7 @@ struct TilePipe {
             mbar_init(&empty[i], readers);
         }
         for (int i = 0; i < L::kRaw; ++i) {
-            mbar_init(&raw_full[i], 1);
+            mbar_init(&raw_full[i], 64);  // the producers' lanes
             mbar_init(&raw_free[i], fillers);
         }
         for (int i = 0; i < L::kRuns; ++i) {
@@ -578,7 +590,18 @@ struct TilePipe {
         }
         *abort = 0;
     }
+    // by a whole warp; the call is left to waits that have something to wait for (it takes some
+    // 350 clocks)
     __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t phase) const {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(smem_u32(bar)), "r"(phase & 1)
+            : "memory");
+        if (__all_sync(0xffffffffu, done)) return true;
         return tile_wait(smem_u32(bar), phase & 1, smem_u32(smem + L::misc));
     }
 };
@@ -587,7 +610,7 @@ struct TilePipe {
 // two tiles ahead of the copies, across runs.
 template <typename L, int D, bool Q8>
 __device__ __forceinline__ void tile_producer(const TileArgs &p, const TilePipe<L> &pipe, const CUtensorMap &tm_k,
-                                              const CUtensorMap &tm_v, int lane) {
+                                              const CUtensorMap &tm_v, int lane, int part) {
     constexpr int NS = L::kSlots;
     const AttnArgs &a = p.a;
     uint64_t *const full = pipe.full, *const empty = pipe.empty, *const run_full = pipe.run_full, *const run_free = pipe.run_free;
@@ -601,6 +624,7 @@ __device__ __forceinline__ void tile_producer(const TileArgs &p, const TilePipe<
     TileRun r{};
     using Loc = std::conditional_t<Q8, PageLocQ8, PageLoc>;
     struct Step {
+        PageEntry at;
         Loc loc;
         bool live, first, last;
     };
@@ -611,21 +635,20 @@ __device__ __forceinline__ void tile_producer(const TileArgs &p, const TilePipe<
     int slot = 0, copies = 0;
     uint32_t ph = 1;
     bool ok = true, more = true;
-    Step s0{{-1, -1}, false, false, false}, s1 = s0;
+    Step s0{{0, 0, -1, -1, 0}, {-1, -1}, false, false, false}, s1 = s0;
     Loc before{-1, -1};
     [[maybe_unused]] int sc_slot = 0;  // scales of the tile copied next
-    [[maybe_unused]] const bool page_scales = a.scale_token_stride == 0;
     // ring order of a run: K0, K1, V0, K2, V1, ... V(n-1) (v_at).  The first two rounds only fill
     // the look-ahead; each part of the code stands here once, to keep it short.
 #pragma unroll 1
     for (int round = 0; ok && (round < 2 || s0.live); ++round) {
-        Step s2{{-1, -1}, false, false, false};
+        Step s2{{0, 0, -1, -1, 0}, {-1, -1}, false, false, false};
         if (t >= tb && more) {
             // the next run: its descriptor for the other warps, its table
             more = it.next(p, r);
             const int at = nrun % L::kRuns;
             if (nrun >= L::kRuns) ok = wait(&run_free[at], nrun / L::kRuns - 1);
-            if (lane == 0 && ok) {
+            if (part == 0 && lane == 0 && ok) {
                 RunDesc &d = runs[at];
                 d.tok0 = r.b.tok0;
                 d.row0 = r.b.row0;
@@ -652,39 +675,39 @@ __device__ __forceinline__ void tile_producer(const TileArgs &p, const TilePipe<
             s2.live = true;
             s2.first = t == ta;
             s2.last = t == tb - 1;
-            // pool rows / 8 of the lane's box(es); -1: nothing to load there
-            int at = (r.b.lo / kTileTok + tb - 1 - (t - ta)) * kTileTok + lane * 16;
-#pragma unroll 1
-            for (int k = 0; k < 16; k += R, at += R) {
-                if (lane >= 8 || at >= r.b.hi || at + R <= r.b.lo) continue;
-                const int pg = fast_div(at, a.block_size, bs_magic);
-                int e = __ldg(bt + pg);
-                if (e < 0 || (a.num_blocks > 0 && e >= a.num_blocks)) {
-                    raise_status(GOLLEK_STATUS_BAD_BLOCK_ID);
-                    e = 0;
-                }
-                const int off = at - pg * a.block_size;
-                const long long first = e * p.page_rows + static_cast<long long>(r.h) * a.block_size + off;
-                if constexpr (Q8) {
-                    const long long so = e * a.scale_page_stride + r.h * a.scale_head_stride + off * a.scale_token_stride;
-                    if (k == 0)
-                        s2.loc.sc0 = so;
-                    else
-                        s2.loc.sc1 = so;
-                    if (page_scales) {
-                        (k == 0 ? s2.loc.ks0 : s2.loc.ks1) = __ldg(a.k_scales + so);
-                        (k == 0 ? s2.loc.vs0 : s2.loc.vs1) = __ldg(a.v_scales + so);
-                    }
-                }
-                const int at8 = static_cast<int>(Q8 ? first : first >> 3);
-                if (k == 0)
-                    s2.loc.row0 = at8;
-                else
-                    s2.loc.row1 = at8;
+            const int at = (r.b.lo / kTileTok + tb - 1 - (t - ta)) * kTileTok + lane * 16;
+            s2.at.h = r.h;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int p0 = at + 8 * k;  // a page of 16 positions or more is copied 16 at a time
+                if (lane >> 2 != part || (R == 16 ? at >= r.b.hi || at + 16 <= r.b.lo : p0 >= r.b.hi || p0 + 8 <= r.b.lo)) continue;
+                const int pg = fast_div(p0, a.block_size, bs_magic);
+                (k ? s2.at.off1 : s2.at.off0) = p0 - pg * a.block_size;
+                if (k == 0 || R == 8) (k ? s2.at.e1 : s2.at.e0) = __ldg(bt + pg);
             }
             __syncwarp();
             ++t;
         }
+        // the next tile's entries, here by now, to rows
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            int e = k == 0 || R == 16 ? s1.at.e0 : s1.at.e1;
+            const int off = k ? s1.at.off1 : s1.at.off0;
+            if (off < 0) continue;
+            if (e < 0 || (a.num_blocks > 0 && e >= a.num_blocks)) {
+                raise_status(GOLLEK_STATUS_BAD_BLOCK_ID);
+                e = 0;
+            }
+            const long long first = e * p.page_rows + static_cast<long long>(s1.at.h) * a.block_size + off;
+            if constexpr (Q8) {
+                const long long so = e * a.scale_page_stride + s1.at.h * a.scale_head_stride + off * a.scale_token_stride;
+                (k ? s1.loc.row1 : s1.loc.row0) = first;
+                (k ? s1.loc.sc1 : s1.loc.sc0) = so;
+            } else if (k == 0 || R == 8) {
+                (k ? s1.loc.row1 : s1.loc.row0) = static_cast<int>(first >> 3);
+            }
+        }
+        __syncwarp();
         // K of this tile, V of the tile before it in the run, V of the run's last tile
 #pragma unroll 1
         for (int w = 0; w < 3 && s0.live && ok; ++w) {
@@ -694,41 +717,45 @@ __device__ __forceinline__ void tile_producer(const TileArgs &p, const TilePipe<
             uint64_t *const r_full = Q8 ? raw_full : full, *const r_free = Q8 ? raw_free : empty;
             if (copies >= kRing) ok = wait(&r_free[slot], ph);
             if (!ok) break;
-            const unsigned boxes = (l.row0 >= 0) + (l.row1 >= 0);
-            constexpr int kRowBytes = Q8 ? D : 2 * D;
-            uint32_t bytes = __reduce_add_sync(0xffffffffu, boxes) * R * kRowBytes;
             if constexpr (Q8) {
-                // with K: both scales of the tile, 16 positions a lane
-                if (w == 0 && !page_scales) bytes += __reduce_add_sync(0xffffffffu, boxes) * R * 8;
-                if (w == 0 && page_scales && lane < 8) {
-                    float *sk = reinterpret_cast<float *>(pipe.smem + L::scales) + sc_slot * 256 + lane * 16;
-                    for (int i = 0; i < 16; ++i) {
-                        sk[i] = i < R ? l.ks0 : l.ks1;
-                        sk[128 + i] = i < R ? l.vs0 : l.vs1;
-                    }
+                // 16 bytes a lane at a time: issued by the whole warp at once, where a bulk copy takes about 90
+                // clocks, and a tile has 8 or 16
+                const uint8_t *src = static_cast<const uint8_t *>(w ? a.v : a.k);
+                constexpr int PC = D / 16, RW = 32 / PC;  // pieces of a row, rows at a time
+                const int rr = lane / PC, ch = lane % PC;
+                const uint32_t dst = smem_u32(pipe.smem + L::raw) + slot * (L::kSlot / 2) + rr * D + ch * 16;
+#pragma unroll
+                for (int i0 = 0; i0 < 8; ++i0) {
+                    const int g = 8 * part + i0;
+                    const long long r0 = __shfl_sync(0xffffffffu, g & 1 ? l.row1 : l.row0, g >> 1);
+                    if (r0 < 0) continue;
+                    const uint8_t *from = src + (r0 + rr) * D + ch * 16;
+#pragma unroll
+                    for (int i = 0; i < 8; i += RW) cp_async16(dst + (g * 8 + i) * D, from + i * D);
                 }
-                __syncwarp();
-            }
-            if (lane == 0) mbar_arrive_expect_tx(&r_full[slot], bytes);
-            __syncwarp();
-            const CUtensorMap *map = w ? &tm_v : &tm_k;
-            if constexpr (Q8) {
-                uint8_t *dst = pipe.smem + L::raw + slot * (L::kSlot / 2) + lane * (16 * D);
-                if (l.row0 >= 0) tma_load_2d(dst, map, 0, l.row0, &r_full[slot]);
-                if (l.row1 >= 0) tma_load_2d(dst + 8 * D, map, 0, l.row1, &r_full[slot]);
-                if (w == 0 && !page_scales) {
-                    float *sk = reinterpret_cast<float *>(pipe.smem + L::scales) + sc_slot * 256 + lane * 16;
-                    if (l.row0 >= 0) {
-                        bulk_load(sk, a.k_scales + l.sc0, R * 4, &r_full[slot]);
-                        bulk_load(sk + 128, a.v_scales + l.sc0, R * 4, &r_full[slot]);
+                if (w == 0) {
+                    // with K: both scales of the half tile, 2 positions a lane (a page's one scale as often)
+                    const int from = 4 * part + (lane >> 3), h8 = lane >> 2 & 1;
+                    const uint32_t sk = smem_u32(pipe.smem + L::scales) + sc_slot * 1024 + (32 * part + lane) * 8;
+                    const long long row0 = __shfl_sync(0xffffffffu, l.row0, from), row1 = __shfl_sync(0xffffffffu, l.row1, from);
+                    const long long c0 = __shfl_sync(0xffffffffu, l.sc0, from), c1 = __shfl_sync(0xffffffffu, l.sc1, from);
+                    const long long so = (h8 ? c1 : c0) + (lane & 3) * 2 * a.scale_token_stride;
+                    if ((h8 ? row1 : row0) >= 0) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            cp_async4(sk + 4 * i, a.k_scales + so + i * a.scale_token_stride);
+                            cp_async4(sk + 512 + 4 * i, a.v_scales + so + i * a.scale_token_stride);
+                        }
                     }
-                    if (l.row1 >= 0) {
-                        bulk_load(sk + 8, a.k_scales + l.sc1, R * 4, &r_full[slot]);
-                        bulk_load(sk + 136, a.v_scales + l.sc1, R * 4, &r_full[slot]);
-                    }
+                    sc_slot = sc_slot + 1 == L::kScales ? 0 : sc_slot + 1;
                 }
-                if (w == 0) sc_slot = sc_slot + 1 == L::kScales ? 0 : sc_slot + 1;
+                cp_async_mbar_arrive_noinc(&r_full[slot]);
             } else {
+                const unsigned boxes = (l.row0 >= 0) + (l.row1 >= 0);
+                const uint32_t bytes = __reduce_add_sync(0xffffffffu, boxes) * R * 2 * D;
+                if (lane == 0) mbar_arrive_expect_tx(&r_full[slot], bytes);
+                __syncwarp();
+                const CUtensorMap *map = w ? &tm_v : &tm_k;
                 uint8_t *dst = pipe.smem + L::ring + slot * L::kSlot + lane * (16 * D * 2);
                 if (l.row0 >= 0) tma_load_4d(dst, map, 0, 0, 0, l.row0, &r_full[slot]);
                 if (l.row1 >= 0) tma_load_4d(dst + 8 * D * 2, map, 0, 0, 0, l.row1, &r_full[slot]);
@@ -745,65 +772,70 @@ __device__ __forceinline__ void tile_producer(const TileArgs &p, const TilePipe<
     }
     if (!ok && lane == 0) tile_give_up(abort);
     // every copy issued lands before the shared memory is released
-    if (lane == 0)
-        for (int n = Q8 ? L::kRaw : NS, k = max(0, copies - n); k < copies; ++k)
-            mbar_wait(Q8 ? &raw_full[k % n] : &full[k % n], (k / n) & 1);
+    if (Q8)
+        cp_async_wait_all();
+    else if (lane == 0)
+        for (int k = max(0, copies - NS); k < copies; ++k) mbar_wait(&full[k % NS], (k / NS) & 1);
     __syncwarp();
 }
 
-// Copies of the ring in order: 128 x D bytes to bf16 in the operand layout, 16 bytes a thread at a
-// time.  0x4300 | u is bf16 128 + u for u < 128, and 0x4300 | sign bit is 128 or 256: their
+// A copy's 128 x D bytes to bf16 in the operand layout, 16 bytes a thread at a time.
+// 0x4300 | u is bf16 128 + u for u < 128, and 0x4300 | sign bit is 128 or 256: their
 // difference is the signed byte, without the conversion pipe that the exponentials use.
-template <typename L, int D, int THREADS>
+template <int D, int THREADS>
+__device__ __forceinline__ void convert_tile(uint32_t src, uint32_t dst, int me) {
+    constexpr int C = D / 16;  // 16-byte pieces of a row
+#pragma unroll 4
+    for (int i = me; i < kTileTok * C; i += THREADS) {
+        const int tok = i / C, pc = i % C;
+        const uint4 w = lds_u4(src + i * 16);
+        uint32_t o[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t x = k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w;
+            o[2 * k] = byte_pair<0x4140>(x);
+            o[2 * k + 1] = byte_pair<0x4342>(x);
+        }
+        // the upper half of a row's threads stores its second chunk first: no two of eight
+        // lanes meet in a bank
+        const bool swap = pc >= C / 2;
+        const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+        sts_u4(dst + kv_chunk_off<D>(tok, 2 * pc + swap), swap ? hi : lo);
+        sts_u4(dst + kv_chunk_off<D>(tok, 2 * pc + !swap), swap ? lo : hi);
+    }
+    fence_proxy_async_smem();
+}
+
+// Converter warps: the ring's copies in order, or (K_ONLY) the K among them.
+template <typename L, int D, int THREADS, bool K_ONLY>
 __device__ __forceinline__ void tile_converter(const TilePipe<L> &pipe, int me) {
     constexpr int NS = L::kSlots;
     const int lane = me & 31;
-    uint64_t *const full = pipe.full, *const empty = pipe.empty, *const run_full = pipe.run_full, *const run_free = pipe.run_free;
-    uint64_t *const raw_full = pipe.raw_full, *const raw_free = pipe.raw_free;
-    RunDesc *const runs = pipe.runs;
-    volatile int *const abort = pipe.abort;
-    auto wait = [&](uint64_t *bar, uint32_t phase) { return pipe.wait(bar, phase); };
     int rs = 0, bs = 0;
     uint32_t rph = 0, bph = 1;
     bool ok = true;
 #pragma unroll 1
     for (int run = 0; ok; ++run) {
         const int at = run % L::kRuns;
-        if (!(ok = wait(&run_full[at], run / L::kRuns))) break;
-        const int n = runs[at].n;
+        if (!(ok = pipe.wait(&pipe.run_full[at], run / L::kRuns))) break;
+        const int n = pipe.runs[at].n;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&run_free[at]);
+        if (lane == 0) mbar_arrive(&pipe.run_free[at]);
         if (n == 0) break;
 #pragma unroll 1
         for (int c = 0; c < 2 * n; ++c) {
-            ok = wait(&raw_full[rs], rph) && wait(&empty[bs], bph);
-            if (!ok) break;
-            const uint32_t src = smem_u32(pipe.smem + L::raw) + rs * (L::kSlot / 2);
-            const uint32_t dst = smem_u32(pipe.smem + L::ring) + bs * L::kSlot;
-            constexpr int C = D / 16;  // 16-byte pieces of a row
-#pragma unroll 4
-            for (int i = me; i < kTileTok * C; i += THREADS) {
-                const int tok = i / C, pc = i % C;
-                const uint4 w = lds_u4(src + i * 16);
-                uint32_t o[8];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t x = k == 0 ? w.x : k == 1 ? w.y : k == 2 ? w.z : w.w;
-                    o[2 * k] = byte_pair<0x4140>(x);
-                    o[2 * k + 1] = byte_pair<0x4342>(x);
+            if (!K_ONLY || c == 0 || ((c & 1) && c != 2 * n - 1)) {
+                // K_ONLY: a bf16 slot's release first.  It says that the copy kSlots in front of this one
+                // has landed, so that the phase of raw_full waited for is this copy's (kRaw = kSlots).
+                ok = pipe.wait(&pipe.empty[bs], bph) && pipe.wait(&pipe.raw_full[rs], rph);
+                if (!ok) break;
+                convert_tile<D, THREADS>(smem_u32(pipe.smem + L::raw) + rs * (L::kSlot / 2),
+                                         smem_u32(pipe.smem + L::ring) + bs * L::kSlot, me);
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&pipe.full[bs]);
+                    mbar_arrive(&pipe.raw_free[rs]);
                 }
-                // the upper half of a row's threads stores its second chunk first: no two of eight
-                // lanes meet in a bank
-                const bool swap = pc >= C / 2;
-                const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
-                sts_u4(dst + kv_chunk_off<D>(tok, 2 * pc + swap), swap ? hi : lo);
-                sts_u4(dst + kv_chunk_off<D>(tok, 2 * pc + !swap), swap ? lo : hi);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&full[bs]);
-                mbar_arrive(&raw_free[rs]);
             }
             if (++rs == L::kRaw) {
                 rs = 0;
@@ -815,7 +847,7 @@ __device__ __forceinline__ void tile_converter(const TilePipe<L> &pipe, int me) 
             }
         }
     }
-    if (!ok && lane == 0) tile_give_up(abort);
+    if (!ok && lane == 0) tile_give_up(pipe.abort);
 }
 
 // FEAT: what is done to the scores besides scale and mask (kPlain, kBias: distance bias,
@@ -848,7 +880,7 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        pipe.init(Q8 ? 4 : 1, 2, Q8 ? 14 : 10);
+        pipe.init(Q8 ? 4 : 2, 2, Q8 ? 14 : 10);
         for (int t = 0; t < 2; ++t) {
             mbar_init(&s_full[t], 1);
             mbar_init(&p_full[t], 4);
@@ -878,12 +910,12 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
     auto wait = [&](uint64_t *bar, uint32_t phase) { return pipe.wait(bar, phase); };
 
     if (warp >= 8) {
-        if (warp == 9) {
-            // ===================================================================== producer
-            tile_producer<L, D, Q8>(p, pipe, tm_k, tm_v, lane);
+        if (warp == 9 || warp == 11) {
+            // ===================================================================== producers
+            tile_producer<L, D, Q8>(p, pipe, tm_k, tm_v, lane, warp == 11);
         } else if (Q8 && warp >= 12) {
             // ===================================================================== converters
-            if constexpr (Q8) tile_converter<L, D, 128>(pipe, tid - 384);
+            if constexpr (Q8) tile_converter<L, D, 128, false>(pipe, tid - 384);
         } else if (warp == 8 || warp == 10) {
             // ===================================================================== MMA issuers
             // Warp 8 issues group 0's MMAs, warp 10 group 1's: what one waits for does not hold the
