@@ -266,7 +266,8 @@ __global__ void __launch_bounds__(kRowsThreads + (Q8 ? kRowsConverters : 0), 1)
             const int n = d.n;
             // lane r < 16 looks after row r; the others of 16 rows see what the block sees
             RowInfo me{d.lo, d.hi, 0, 0.f};
-            long long out_row = 0;
+            const long long out0 = static_cast<long long>(d.tok0) * a.num_q_heads;
+            long long out_row = out0;
             if (lane < d.nrows) {
                 const int rho = d.row0 + lane, i = fast_div(rho, G, g_magic), head = d.h * G + (rho - i * G);
                 out_row = static_cast<long long>(d.tok0 + i) * a.num_q_heads + head;
@@ -363,17 +364,23 @@ __global__ void __launch_bounds__(kRowsThreads + (Q8 ? kRowsConverters : 0), 1)
                 const int4 fl = *reinterpret_cast<const int4 *>(flags);
                 if (fl.x | fl.y | fl.z | fl.w) {
                     // The references rise by an integer (where there was one), and the sums and O follow.
+                    const int r0 = lane & (N - 1);  // this lane's row of the 16
+                    float was = m[0];
+#pragma unroll
+                    for (int r = 1; r < N; ++r) was = r0 == r ? m[r] : was;
+                    float top = fl.x ? vmax[r0] : -INFINITY;
+                    top = fmaxf(top, fl.y ? vmax[N + r0] : -INFINITY);
+                    top = fmaxf(top, fl.z ? vmax[2 * N + r0] : -INFINITY);
+                    top = fmaxf(top, fl.w ? vmax[3 * N + r0] : -INFINITY);
+                    const bool move = top - was > kLazyMax<T>;
+                    const float by = move && was != -INFINITY ? ceilf(top - was) : 0.f;
+                    const float now = !move ? was : was == -INFINITY ? top : was + by;
+                    const float fall = fast_exp2(-by);
                     float alpha[N];
 #pragma unroll
                     for (int r = 0; r < N; ++r) {
-                        float top = fl.x ? vmax[r] : -INFINITY;
-                        top = fmaxf(top, fl.y ? vmax[N + r] : -INFINITY);
-                        top = fmaxf(top, fl.z ? vmax[2 * N + r] : -INFINITY);
-                        top = fmaxf(top, fl.w ? vmax[3 * N + r] : -INFINITY);
-                        const bool move = top - m[r] > kLazyMax<T>;
-                        const float by = move && m[r] != -INFINITY ? ceilf(top - m[r]) : 0.f;
-                        m[r] = !move ? m[r] : m[r] == -INFINITY ? top : m[r] + by;
-                        alpha[r] = fast_exp2(-by);
+                        m[r] = __shfl_sync(0xffffffffu, now, r);
+                        alpha[r] = __shfl_sync(0xffffffffu, fall, r);
                         l[r] *= alpha[r];
                     }
                     if (j != t) {  // the scores' commit covers the group's earlier value MMAs: O is at rest
@@ -462,26 +469,37 @@ __global__ void __launch_bounds__(kRowsThreads + (Q8 ? kRowsConverters : 0), 1)
                     ps[lane] = mm;
                     ps[kBlkRows + lane] = ll;
                 }
+                // each row's factors and place, in the room of the run's RowInfo
+                __syncwarp();
+                if (lane < N) info[lane] = RowInfo{ll == 0.f, static_cast<int>(out_row - out0), __float_as_int(fa), fb};
+                __syncwarp();
                 float oa[N], ob[N];
                 tmem_ld<N>(t_o, oa);
                 tmem_ld<N>(t_o + 16, ob);  // group 1's; not used where it had no tile
                 tmem_wait_ld();
 #pragma unroll
                 for (int r = 0; r < N; ++r) {
-                    const float wa = __shfl_sync(0xffffffffu, fa, r), wb = __shfl_sync(0xffffffffu, fb, r);
-                    const float s = __shfl_sync(0xffffffffu, ll, r);
-                    const long long to = __shfl_sync(0xffffffffu, out_row, r);
-                    if (r >= d.nrows) continue;
-                    const float o = two ? fmaf(oa[r], wa, ob[r] * wb) : oa[r] * wa;
-                    if (whole) {
-                        T *out = reinterpret_cast<T *>(a.out) + to * D + row;
-                        const float v = s == 0.f ? 0.f : o;
+                    const RowInfo w = info[r];
+                    oa[r] *= __int_as_float(w.pos);
+                    if (two) oa[r] = fmaf(ob[r], w.slope, oa[r]);
+                    if (whole && w.lo) oa[r] = 0.f;  // nothing seen
+                }
+                if (whole) {
+                    T *out = reinterpret_cast<T *>(a.out) + out0 * D + row;
+#pragma unroll
+                    for (int r = 0; r < N; ++r) {
+                        if (r >= d.nrows) break;
                         if constexpr (kBf16)
-                            *out = __float2bfloat16_rn(v);
+                            out[static_cast<long long>(info[r].hi) * D] = __float2bfloat16_rn(oa[r]);
                         else
-                            *out = __float2half_rn(v);
-                    } else {
-                        ps[2 * kBlkRows + r * D + row] = o;
+                            out[static_cast<long long>(info[r].hi) * D] = __float2half_rn(oa[r]);
+                    }
+                } else {
+                    float *out = ps + 2 * kBlkRows + row;
+#pragma unroll
+                    for (int r = 0; r < N; ++r) {
+                        if (r >= d.nrows) break;
+                        out[r * D] = oa[r];
                     }
                 }
                 tc_fence_before();

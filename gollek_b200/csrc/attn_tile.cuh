@@ -301,46 +301,50 @@ __device__ __forceinline__ int find_block(const TileArgs &p, int nb, long long x
 
 // The runs of a CTA in order; every lane of a warp holds the same state.
 struct RunIter {
-    long long x, xe, base, m;
-    int i, hkv;
+    long long x, xe, at, m;  // at: start of unit (block i, head h), m: its length
+    int i, h, hkv;
     TileBlk b;
 
     __device__ __forceinline__ void load(const TileArgs &p) {
-        const long long c0 = p.cost[i];
-        base = c0 * hkv;
-        m = p.cost[i + 1] - c0;
+        m = p.cost[i + 1] - p.cost[i];
         b = p.blks[i];
     }
-    // warp-collective: finds the block that holds the range's first unit
+    // warp-collective: finds the unit that holds the range's first tile
     __device__ __forceinline__ void begin(const TileArgs &p, int cta) {
         const PlanHead hd = *p.head;
         hkv = p.a.num_kv_heads;
         x = min(static_cast<long long>(cta) * hd.range, hd.total);
         xe = min(x + hd.range, hd.total);
-        i = 0;
         if (x >= xe) return;
         i = find_block(p, hd.nb, x);
         load(p);
+        const long long base = p.cost[i] * hkv;
+        h = static_cast<int>((x - base) / m);
+        at = base + h * m;
     }
     __device__ __forceinline__ bool next(const TileArgs &p, TileRun &r) {
-        while (x < xe) {
-            while (x >= base + m * hkv) {
-                ++i;
-                load(p);
-            }
-            const long long y = x - base;
-            r.h = static_cast<int>(y / m);
-            const long long v = y - r.h * m;
-            const long long len = min(m - v, xe - x);
-            x += len;
+        bool found = false;
+#pragma unroll 1
+        while (!found && x < xe) {
+            const long long v = x - at, len = min(m - v, xe - x);
             run_tiles(v, len, r.ta, r.tb);
-            if (r.ta < r.tb) {
-                r.b = b;
-                r.n = static_cast<int>(m) - kRunCostTiles;
-                return true;
+            found = r.ta < r.tb;
+            r.b = b;
+            r.h = h;
+            r.n = static_cast<int>(m) - kRunCostTiles;
+            x += len;
+            if (x == at + m) {
+                at = x;
+                ++h;
+#pragma unroll 1
+                while (x < xe && (h == hkv || m == 0)) {  // the next block; one without tiles has no units
+                    ++i;
+                    h = 0;
+                    load(p);
+                }
             }
         }
-        return false;
+        return found;
     }
 };
 
@@ -532,7 +536,7 @@ __device__ __forceinline__ uint32_t kv_chunk_off(int tok, int ch) {
     return static_cast<uint32_t>((tok >> 3) * (16 * D) + (ch >> 3) * 1024 + r8 * 128 + (((ch & 7) ^ r8) << 4));
 }
 
-// What lane g < 8 copies of the 16 positions 16 g .. of a tile: two halves of 8, in one page or
+// What lane g of 4 copies of the 16 positions 16 g .. of a tile: two halves of 8, in one page or
 // (pages of 8) in one each.  `entry`: the pages' table entries, looked up two tiles ahead;
 // resolved one tile ahead.
 struct PageEntry {
@@ -574,14 +578,14 @@ struct TilePipe {
         own = run_free + L::kRuns;
         abort = reinterpret_cast<volatile int *>(base + L::misc);
     }
-    // by one thread; `fillers` arrive on full, `readers` on empty, `users` read a descriptor
+    // by one thread; `fillers` warps arrive on full, `readers` on empty, `users` read a descriptor
     __device__ __forceinline__ void init(int fillers, int readers, int users) const {
         for (int i = 0; i < L::kSlots; ++i) {
             mbar_init(&full[i], fillers);
             mbar_init(&empty[i], readers);
         }
         for (int i = 0; i < L::kRaw; ++i) {
-            mbar_init(&raw_full[i], 64);  // the producers' lanes
+            mbar_init(&raw_full[i], 64);  // the two producers' lanes
             mbar_init(&raw_free[i], fillers);
         }
         for (int i = 0; i < L::kRuns; ++i) {
@@ -606,8 +610,10 @@ struct TilePipe {
     }
 };
 
-// Walks the runs, hands their descriptors out and copies their tiles; the page lookups go
-// two tiles ahead of the copies, across runs.
+// Two warps walk the runs and copy half of each tile, part 0 the first 64 positions; it also
+// hands the runs' descriptors out.  The page lookups go two tiles ahead of the copies, across
+// runs.  One warp alone, at some 90 clocks a box, and a lookup that waited for its table entry
+// were what bounded decode (229 -> 185 us for 64 sequences of 512 to 8192 tokens, 32 q and 8 kv heads).
 template <typename L, int D, bool Q8>
 __device__ __forceinline__ void tile_producer(const TileArgs &p, const TilePipe<L> &pipe, const CUtensorMap &tm_k,
                                               const CUtensorMap &tm_v, int lane, int part) {
@@ -677,10 +683,12 @@ __device__ __forceinline__ void tile_producer(const TileArgs &p, const TilePipe<
             s2.last = t == tb - 1;
             const int at = (r.b.lo / kTileTok + tb - 1 - (t - ta)) * kTileTok + lane * 16;
             s2.at.h = r.h;
+            // (straight-line, so that nothing waits for an entry before it is resolved)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const int p0 = at + 8 * k;  // a page of 16 positions or more is copied 16 at a time
-                if (lane >> 2 != part || (R == 16 ? at >= r.b.hi || at + 16 <= r.b.lo : p0 >= r.b.hi || p0 + 8 <= r.b.lo)) continue;
+                if (lane >> 2 != part || (R == 16 ? at >= r.b.hi || at + 16 <= r.b.lo : p0 >= r.b.hi || p0 + 8 <= r.b.lo))
+                    continue;
                 const int pg = fast_div(p0, a.block_size, bs_magic);
                 (k ? s2.at.off1 : s2.at.off0) = p0 - pg * a.block_size;
                 if (k == 0 || R == 8) (k ? s2.at.e1 : s2.at.e0) = __ldg(bt + pg);
@@ -700,9 +708,9 @@ __device__ __forceinline__ void tile_producer(const TileArgs &p, const TilePipe<
             }
             const long long first = e * p.page_rows + static_cast<long long>(s1.at.h) * a.block_size + off;
             if constexpr (Q8) {
-                const long long so = e * a.scale_page_stride + s1.at.h * a.scale_head_stride + off * a.scale_token_stride;
                 (k ? s1.loc.row1 : s1.loc.row0) = first;
-                (k ? s1.loc.sc1 : s1.loc.sc0) = so;
+                (k ? s1.loc.sc1 : s1.loc.sc0) =
+                    e * a.scale_page_stride + s1.at.h * a.scale_head_stride + off * a.scale_token_stride;
             } else if (k == 0 || R == 8) {
                 (k ? s1.loc.row1 : s1.loc.row0) = static_cast<int>(first >> 3);
             }
@@ -734,15 +742,16 @@ __device__ __forceinline__ void tile_producer(const TileArgs &p, const TilePipe<
                     for (int i = 0; i < 8; i += RW) cp_async16(dst + (g * 8 + i) * D, from + i * D);
                 }
                 if (w == 0) {
-                    // with K: both scales of the half tile, 2 positions a lane (a page's one scale as often)
-                    const int from = 4 * part + (lane >> 3), h8 = lane >> 2 & 1;
-                    const uint32_t sk = smem_u32(pipe.smem + L::scales) + sc_slot * 1024 + (32 * part + lane) * 8;
+                    // with K: both scales of its positions, NP a lane (a page's one scale as often)
+                    constexpr int NP = 2;
+                    const int p0 = 64 * part + lane * NP, from = p0 >> 4, h8 = p0 >> 3 & 1;
+                    const uint32_t sk = smem_u32(pipe.smem + L::scales) + sc_slot * 1024 + p0 * 4;
                     const long long row0 = __shfl_sync(0xffffffffu, l.row0, from), row1 = __shfl_sync(0xffffffffu, l.row1, from);
                     const long long c0 = __shfl_sync(0xffffffffu, l.sc0, from), c1 = __shfl_sync(0xffffffffu, l.sc1, from);
-                    const long long so = (h8 ? c1 : c0) + (lane & 3) * 2 * a.scale_token_stride;
+                    const long long so = (h8 ? c1 : c0) + (p0 & 7) * a.scale_token_stride;
                     if ((h8 ? row1 : row0) >= 0) {
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
+                        for (int i = 0; i < NP; ++i) {
                             cp_async4(sk + 4 * i, a.k_scales + so + i * a.scale_token_stride);
                             cp_async4(sk + 512 + 4 * i, a.v_scales + so + i * a.scale_token_stride);
                         }
@@ -785,7 +794,7 @@ __device__ __forceinline__ void tile_producer(const TileArgs &p, const TilePipe<
 template <int D, int THREADS>
 __device__ __forceinline__ void convert_tile(uint32_t src, uint32_t dst, int me) {
     constexpr int C = D / 16;  // 16-byte pieces of a row
-#pragma unroll 4
+#pragma unroll 2  // more is slower: its code pushes other code out of the instruction cache
     for (int i = me; i < kTileTok * C; i += THREADS) {
         const int tok = i / C, pc = i % C;
         const uint4 w = lds_u4(src + i * 16);
@@ -907,7 +916,8 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *sm_tmem;
-    auto wait = [&](uint64_t *bar, uint32_t phase) { return pipe.wait(bar, phase); };
+    const uint32_t abort_s = smem_u32(tile_smem + L::misc);
+    auto wait = [&](uint64_t *bar, uint32_t phase) { return tile_wait(smem_u32(bar), phase & 1, abort_s); };
 
     if (warp >= 8) {
         if (warp == 9 || warp == 11) {
