@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kRowsThreads + (Q8 ? kRowsConverters : 0), 1)
         mbar_init(drained, 1);
         fence_barrier_init();
     }
-    if (warp == 9 && lane == 0) {
+    if (!Q8 && warp == 9 && lane == 0) {
         prefetch_tensormap(&tm_k);
         prefetch_tensormap(&tm_v);
     }
@@ -271,8 +271,10 @@ __global__ void __launch_bounds__(kRowsThreads + (Q8 ? kRowsConverters : 0), 1)
             if (lane < d.nrows) {
                 const int rho = d.row0 + lane, i = fast_div(rho, G, g_magic), head = d.h * G + (rho - i * G);
                 out_row = static_cast<long long>(d.tok0 + i) * a.num_q_heads + head;
-                me.pos = d.pos0 + i;
-                row_range(a, d.tab, d.tok0 + i, me.pos, d.len, me.lo, me.hi);
+                if ((d.flags & 3) == kOwn) {
+                    me.pos = d.pos0 + i;
+                    row_range(a, d.tab, d.tok0 + i, me.pos, d.len, me.lo, me.hi);
+                }
                 if (a.slopes) me.slope = a.slopes[head] * kLog2e;
             }
             __syncwarp();  // the last run's rows are read
@@ -458,20 +460,27 @@ __global__ void __launch_bounds__(kRowsThreads + (Q8 ? kRowsConverters : 0), 1)
                     fb = mb == -INFINITY ? (lb == 0.f ? 0.f : 1.f) : fast_exp2(mb - mm);
                     ll = ll * fa + lb * fb;
                 }
-                const bool whole = d.flags & 4;
+                const bool whole = d.flags & 4, direct = whole && (d.flags & 3) == kOwn;
                 const float inv = ll == 0.f ? 0.f : 1.f / ll;  // a NaN stays one
-                if (whole) {
+                if (direct) {
                     fa *= inv;
                     fb *= inv;
                 }
-                float *ps = p.slots + (static_cast<size_t>(blockIdx.x) * 2 + (d.flags >> 3 & 1)) * (kBlkRows * (D + 2));
-                if (!whole && w4 == 0 && lane < d.nrows) {
-                    ps[lane] = mm;
-                    ps[kBlkRows + lane] = ll;
+                // a partial state goes to the CTA's slot, a whole unit's of a call with prefixes to its row's place
+                float *st_o = p.slots + (static_cast<size_t>(blockIdx.x) * 2 + (d.flags >> 3 & 1)) * (kBlkRows * (D + 2));
+                const long long own = static_cast<long long>(a.total_q) * a.num_q_heads;
+                if (w4 == 0 && lane < d.nrows) {
+                    if (!whole) {
+                        st_o[lane] = mm;
+                        st_o[kBlkRows + lane] = ll;
+                    } else if (!direct) {
+                        p.ml[own + out_row] = make_float2(mm, ll);
+                    }
                 }
+                st_o = whole ? p.acc + (own + out0) * D : st_o + 2 * kBlkRows;
                 // each row's factors and place, in the room of the run's RowInfo
                 __syncwarp();
-                if (lane < N) info[lane] = RowInfo{ll == 0.f, static_cast<int>(out_row - out0), __float_as_int(fa), fb};
+                if (lane < N) info[lane] = RowInfo{ll == 0.f, whole ? static_cast<int>(out_row - out0) : lane, __float_as_int(fa), fb};
                 __syncwarp();
                 float oa[N], ob[N];
                 tmem_ld<N>(t_o, oa);
@@ -482,9 +491,9 @@ __global__ void __launch_bounds__(kRowsThreads + (Q8 ? kRowsConverters : 0), 1)
                     const RowInfo w = info[r];
                     oa[r] *= __int_as_float(w.pos);
                     if (two) oa[r] = fmaf(ob[r], w.slope, oa[r]);
-                    if (whole && w.lo) oa[r] = 0.f;  // nothing seen
+                    if (direct && w.lo) oa[r] = 0.f;  // nothing seen
                 }
-                if (whole) {
+                if (direct) {
                     T *out = reinterpret_cast<T *>(a.out) + out0 * D + row;
 #pragma unroll
                     for (int r = 0; r < N; ++r) {
@@ -495,11 +504,11 @@ __global__ void __launch_bounds__(kRowsThreads + (Q8 ? kRowsConverters : 0), 1)
                             out[static_cast<long long>(info[r].hi) * D] = __float2half_rn(oa[r]);
                     }
                 } else {
-                    float *out = ps + 2 * kBlkRows + row;
+                    float *out = st_o + row;
 #pragma unroll
                     for (int r = 0; r < N; ++r) {
                         if (r >= d.nrows) break;
-                        out[r * D] = oa[r];
+                        out[static_cast<long long>(info[r].hi) * D] = oa[r];
                     }
                 }
                 tc_fence_before();

@@ -104,7 +104,7 @@ struct TileArgs {
     float *slots;     // [CTA][2]: ml [2][256], O [256][D]
     float2 *ml;       // shared: [2][rows]
     float *acc;       // shared: [2][rows][D]
-    int entities, grid, max_blocks;
+    int ent0, entities, grid, max_blocks;  // entities ent0 .. ent0 + entities - 1 of the call
     int blk_rows;     // rows a block may have
     long long page_rows;
 };
@@ -157,7 +157,13 @@ __device__ __forceinline__ int entity_tokens(const AttnArgs &a, int e) {
     return n;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(const TileArgs p) {
+// Two lines at most, one per CTA: a call whose entities go to two kernels has one for each.
+struct PlanArgs {
+    TileArgs line[2];
+};
+
+__global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(const __grid_constant__ PlanArgs both) {
+    const TileArgs &p = both.line[blockIdx.x];
     const AttnArgs &a = p.a;
     const int G = a.num_q_heads / a.num_kv_heads;
     const int tid = threadIdx.x;
@@ -170,13 +176,14 @@ __global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(const TileArgs 
         const int e = e0 + tid;
         long long blocks = 0;
         if (e < p.entities) {
+            const int ent = p.ent0 + e;
             if (a.num_groups == 0)
-                check_seq(a, e);
-            else if (e < a.num_groups)
-                check_group(a, e);
+                check_seq(a, ent);
+            else if (ent < a.num_groups)
+                check_group(a, ent);
             else
-                check_seq(a, e - a.num_groups);
-            blocks = (static_cast<long long>(entity_tokens(a, e)) * G + p.blk_rows - 1) / p.blk_rows;
+                check_seq(a, ent - a.num_groups);
+            blocks = (static_cast<long long>(entity_tokens(a, ent)) * G + p.blk_rows - 1) / p.blk_rows;
         }
         long long sum;
         const long long at = block_scan(blocks, sm_l, &sum);
@@ -202,7 +209,7 @@ __global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(const TileArgs 
                 else
                     hi = mid - 1;
             }
-            const int e = lo;
+            const int e = p.ent0 + lo;
             int first, n;
             if (a.num_groups == 0) {
                 seq_rows(a, e, first, n);
@@ -222,7 +229,7 @@ __global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(const TileArgs 
                 k.len = clamp_len(a, a.context_lens[k.tab], a.max_blocks);
             }
             k.tok0 = first;
-            k.row0 = (b - p.ents[e]) * p.blk_rows;
+            k.row0 = (b - p.ents[lo]) * p.blk_rows;
             k.nrows = static_cast<int>(min(static_cast<long long>(n) * G - k.row0, static_cast<long long>(p.blk_rows)));
             k.lo = 0;
             k.hi = k.len;
@@ -904,7 +911,7 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
         fence_barrier_init();
     }
     if (Q8 && tid < 128) reinterpret_cast<float *>(tile_smem + L::ones)[tid] = 1.f;
-    if (warp == 9 && lane == 0) {
+    if (!Q8 && warp == 9 && lane == 0) {
         prefetch_tensormap(&tm_k);
         prefetch_tensormap(&tm_v);
     }
@@ -1558,13 +1565,12 @@ __global__ void __launch_bounds__(kMergeThreads) tile_merge_kernel(const TileArg
 
 // Shared prefixes.  One warp per (sequence, q head): the prefix's state, then the own tokens'.
 template <typename T, int D>
-__global__ void __launch_bounds__(kMergeThreads) tile_merge_shared_kernel(const TileArgs p) {
-    const AttnArgs &a = p.a;
+__global__ void __launch_bounds__(kMergeThreads) tile_merge_shared_kernel(const __grid_constant__ PlanArgs both) {
+    const AttnArgs &a = both.line[0].a;
     const int lane = threadIdx.x & 31;
     const int G = a.num_q_heads / a.num_kv_heads;
     const long long rows = static_cast<long long>(a.num_seqs) * a.num_q_heads;
     pdl_wait();
-    const PlanHead hd = *p.head;
     const long long row = static_cast<long long>(blockIdx.x) * (kMergeThreads / 32) + (threadIdx.x >> 5);
     if (row >= rows) return;
     const int s = static_cast<int>(row / a.num_q_heads), head = static_cast<int>(row % a.num_q_heads);
@@ -1572,6 +1578,7 @@ __global__ void __launch_bounds__(kMergeThreads) tile_merge_shared_kernel(const 
     RowState<D / 32> st;
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
+        const TileArgs &p = both.line[part];  // the same twice where one kernel took both
         int e = a.num_groups + s;
         long long rho = g;
         if (part == 0) {
@@ -1579,11 +1586,12 @@ __global__ void __launch_bounds__(kMergeThreads) tile_merge_shared_kernel(const 
             if (e < 0) continue;
             rho += static_cast<long long>(s - a.group_starts[e]) * G;
         }
+        e -= p.ent0;
         const long long i = p.ents[e] + rho / kBlkRows;
         if (i >= p.ents[e + 1]) continue;  // only where group_starts is not usable
         const long long c0 = p.cost[i], m = p.cost[i + 1] - c0;
         if (m == 0) continue;
-        if (!add_pieces<D>(p, hd.range, c0 * a.num_kv_heads + h * m, m, static_cast<int>(rho % kBlkRows), lane, st)) {
+        if (!add_pieces<D>(p, p.head->range, c0 * a.num_kv_heads + h * m, m, static_cast<int>(rho % kBlkRows), lane, st)) {
             const long long at = part * rows + row;
             const float2 ml = p.ml[at];
             float o[D / 32];
@@ -1591,7 +1599,7 @@ __global__ void __launch_bounds__(kMergeThreads) tile_merge_shared_kernel(const 
             st.add(ml.x, ml.y, o);
         }
     }
-    write_row<T, D>(p, row, lane, st);
+    write_row<T, D>(both.line[0], row, lane, st);
 }
 
 }  // namespace gk

@@ -101,10 +101,53 @@ bool tile_takes(const AttnArgs &a) {
     return a.num_blocks == 0 || a.num_blocks * page_rows < (1LL << 31);
 }
 
-long long tile_entities(int num_groups, int num_seqs) { return static_cast<long long>(num_groups) + num_seqs; }
+// How the entities of a call are laid out: one cost line, or (shared prefixes) one for the
+// prefixes and one for the own tokens, each with its part of the workspace.
+struct CallPlan {
+    struct Line {
+        int ent0, entities, blk_rows;
+        TileWs ws;
+    } line[2];
+    int lines;
+    size_t total;
+};
 
-// Rows of all entities: each query token's heads of one group; shared: twice (prefix, own).
-long long tile_rows(int total_q, int G, bool shared) { return static_cast<long long>(total_q) * G * (shared ? 2 : 1); }
+// Blocks of few rows go to attn_rows_kernel (head_dim 128):
+// - varlen calls whose sequences have 16 rows at most on average (a longer one is cut into
+//   blocks of 16, each of which reads its pages): 237 -> 183 us for 64 sequences of one token;
+// - the own tokens of shared-prefix calls of up to 16 q heads per kv head, once they alone
+//   give the device kSplitUnits units of work; below, one more launch costs more than it saves.
+constexpr int kSplitUnits = 256;
+
+CallPlan plan_call(int num_groups, int num_seqs, int total_q, int hq, int hkv, int D) {
+    const int G = hq / hkv;
+    const long long rows = static_cast<long long>(total_q) * G, out_rows = static_cast<long long>(total_q) * hq;
+    const bool few = D == kFewD && G <= kFewRows;
+    CallPlan c{};
+    c.lines = 1;
+    auto &l = c.line[0];
+    if (num_groups == 0) {
+        l.entities = num_seqs;
+        l.blk_rows = few && rows <= static_cast<long long>(num_seqs) * kFewRows ? kFewRows : kBlkRows;
+        l.ws = tile_ws(num_seqs, rows, l.blk_rows, 0, D, false);
+    } else if (few && static_cast<long long>(num_seqs) * hkv >= kSplitUnits) {
+        auto &own = c.line[1];
+        c.lines = 2;
+        l.entities = num_groups;
+        l.blk_rows = kBlkRows;
+        l.ws = tile_ws(num_groups, rows, kBlkRows, out_rows, D, true);
+        own.ent0 = num_groups;
+        own.entities = num_seqs;
+        own.blk_rows = kFewRows;
+        own.ws = tile_ws(num_seqs, rows, kFewRows, 0, D, false);
+    } else {
+        l.entities = num_groups + num_seqs;
+        l.blk_rows = kBlkRows;
+        l.ws = tile_ws(static_cast<long long>(num_groups) + num_seqs, 2 * rows, kBlkRows, out_rows, D, true);
+    }
+    c.total = l.ws.total + c.line[1].ws.total;
+    return c;
+}
 
 // 4-D map over a pool of 16-bit rows: (64 columns, 8 rows, column slabs, 8-row blocks), so a
 // box of (64, 8, slabs, box_rows / 8) lands in the layout of kv_chunk_off.
@@ -122,36 +165,6 @@ int encode_tile_map(CUtensorMap *m, const void *base, int kv_dtype, int D, long 
                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(GOLLEK_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return GOLLEK_OK;
-}
-
-// 2-D map over a pool of int8 rows; a box is box_rows whole rows, behind one another.
-int encode_byte_map(CUtensorMap *m, const void *base, int D, long long rows, int box_rows) {
-    auto enc = encode_fn();
-    if (!enc) return fail(GOLLEK_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled unavailable");
-    cuuint64_t dims[2] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows)};
-    cuuint64_t strides[1] = {static_cast<cuuint64_t>(D)};
-    cuuint32_t box[2] = {static_cast<cuuint32_t>(D), static_cast<cuuint32_t>(box_rows)};
-    cuuint32_t estr[2] = {1, 1};
-    CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, estr,
-                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(GOLLEK_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-    return GOLLEK_OK;
-}
-
-// Whether a varlen call goes to the kernel for few rows: its sequences have 16 rows at most on
-// average (a longer one is cut into blocks of 16, each of which reads its pages).
-bool few_rows(int num_groups, int num_seqs, int total_q, int G, int D) {
-    return num_groups == 0 && D == kFewD && G <= kFewRows && static_cast<long long>(total_q) * G <= static_cast<long long>(num_seqs) * kFewRows;
-}
-
-// The workspace of a call; *blk_rows receives the rows of its blocks.
-TileWs attn_ws(int num_groups, int num_seqs, int total_q, int hq, int hkv, int D, int *blk_rows) {
-    const int G = hq / hkv;
-    const bool shared = num_groups > 0;
-    *blk_rows = few_rows(num_groups, num_seqs, total_q, G, D) ? kFewRows : kBlkRows;
-    return tile_ws(tile_entities(num_groups, num_seqs), tile_rows(total_q, G, shared), *blk_rows,
-                   static_cast<long long>(total_q) * hq, D, shared);
 }
 
 // A launch that may begin before the kernel in front of it has ended (that kernel's results are
@@ -172,32 +185,35 @@ int launch_dependent(const void *fn, dim3 grid, int threads, size_t smem, cudaSt
 }
 
 template <typename T, int D, bool Q8 = false>
-int launch_tile_as(TileArgs &p, const CUtensorMap &tmk, const CUtensorMap &tmv, cudaStream_t st) {
-    const AttnArgs &a = p.a;
-    uint32_t smem = TileSmem<D, Q8>::total;
+int launch_tile_as(const PlanArgs &both, int lines, const CUtensorMap &tmk, const CUtensorMap &tmv, cudaStream_t st) {
+    const AttnArgs &a = both.line[0].a;
     static_assert(TileSmem<D, Q8>::total <= 227 * 1024, "shared memory of the tile kernel");
-    const void *fn = a.soft_cap > 0.f ? reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kCap, Q8>)
-                     : a.slopes       ? reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kBias, Q8>)
-                                      : reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kPlain, Q8>);
-    int threads = Q8 ? kTileThreadsQ8 : kTileThreads;
-    if constexpr (D == kFewD) {
-        static_assert(RowsSmem<Q8>::total <= 227 * 1024, "shared memory of the kernel for few rows");
-        if (p.blk_rows == kFewRows) {
-            smem = RowsSmem<Q8>::total;
-            fn = reinterpret_cast<const void *>(&attn_rows_kernel<T, Q8>);
-            threads = kRowsThreads + (Q8 ? kRowsConverters : 0);
-        }
-    }
-    GK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute");
-    tile_plan_kernel<<<1, kPlanThreads, 0, st>>>(p);
+    tile_plan_kernel<<<lines, kPlanThreads, 0, st>>>(both);
     GK_CUDA(cudaGetLastError(), "tile_plan_kernel launch");
-    void *args[] = {const_cast<CUtensorMap *>(&tmk), const_cast<CUtensorMap *>(&tmv), &p};
-    int rc = launch_dependent(fn, dim3(p.grid), threads, smem, st, args, "attn_tile_kernel launch");
-    if (rc) return rc;
-    void *margs[] = {&p};
+    for (int i = 0; i < lines; ++i) {
+        const TileArgs &p = both.line[i];
+        uint32_t smem = TileSmem<D, Q8>::total;
+        int threads = Q8 ? kTileThreadsQ8 : kTileThreads;
+        const void *fn = a.soft_cap > 0.f ? reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kCap, Q8>)
+                         : a.slopes       ? reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kBias, Q8>)
+                                          : reinterpret_cast<const void *>(&attn_tile_kernel<T, D, kPlain, Q8>);
+        if constexpr (D == kFewD) {
+            static_assert(RowsSmem<Q8>::total <= 227 * 1024, "shared memory of the kernel for few rows");
+            if (p.blk_rows == kFewRows) {
+                smem = RowsSmem<Q8>::total;
+                fn = reinterpret_cast<const void *>(&attn_rows_kernel<T, Q8>);
+                threads = kRowsThreads + (Q8 ? kRowsConverters : 0);
+            }
+        }
+        GK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "cudaFuncSetAttribute");
+        void *args[] = {const_cast<CUtensorMap *>(&tmk), const_cast<CUtensorMap *>(&tmv), const_cast<TileArgs *>(&p)};
+        int rc = launch_dependent(fn, dim3(p.grid), threads, smem, st, args, "attention kernel launch");
+        if (rc) return rc;
+    }
+    void *margs[] = {const_cast<PlanArgs *>(&both)}, *margs1[] = {const_cast<TileArgs *>(&both.line[0])};
     if (a.num_groups == 0)
-        return launch_dependent(reinterpret_cast<const void *>(&tile_merge_kernel<T, D>), dim3(p.grid, kMergeSplit),
-                                kMergeThreads, 0, st, margs, "tile_merge_kernel launch");
+        return launch_dependent(reinterpret_cast<const void *>(&tile_merge_kernel<T, D>), dim3(both.line[0].grid, kMergeSplit),
+                                kMergeThreads, 0, st, margs1, "tile_merge_kernel launch");
     const long long rows = static_cast<long long>(a.num_seqs) * a.num_q_heads;
     return launch_dependent(reinterpret_cast<const void *>(&tile_merge_shared_kernel<T, D>),
                             dim3(static_cast<unsigned>((rows + kMergeThreads / 32 - 1) / (kMergeThreads / 32))), kMergeThreads,
@@ -205,49 +221,57 @@ int launch_tile_as(TileArgs &p, const CUtensorMap &tmk, const CUtensorMap &tmv, 
 }
 
 int launch_tile(AttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
-    TileArgs p{};
-    p.entities = a.num_groups + a.num_seqs;
-    const TileWs w = attn_ws(a.num_groups, a.num_seqs, a.total_q, a.num_q_heads, a.num_kv_heads, a.head_dim, &p.blk_rows);
-    if (w.max_blocks > (1LL << 22)) return fail(GOLLEK_ERR_UNSUPPORTED, "too many query rows for one call");
+    const CallPlan c = plan_call(a.num_groups, a.num_seqs, a.total_q, a.num_q_heads, a.num_kv_heads, a.head_dim);
+    if (std::max(c.line[0].ws.max_blocks, c.line[1].ws.max_blocks) > (1LL << 22))
+        return fail(GOLLEK_ERR_UNSUPPORTED, "too many query rows for one call");
     int dev = 0;
     GK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
     if (!ws) {
-        int rc = library_workspace(dev, stream, w.total, &ws, &ws_bytes);
+        int rc = library_workspace(dev, stream, c.total, &ws, &ws_bytes);
         if (rc) return rc;
     }
-    if (ws_bytes < w.total)
-        return fail(GOLLEK_ERR_WORKSPACE, "workspace of %zu bytes < %zu needed", ws_bytes, w.total);
+    if (ws_bytes < c.total)
+        return fail(GOLLEK_ERR_WORKSPACE, "workspace of %zu bytes < %zu needed", ws_bytes, c.total);
     if (reinterpret_cast<uintptr_t>(ws) & 255) return fail(GOLLEK_ERR_INVALID_ARGUMENT, "workspace not 256-byte aligned");
-    uint8_t *base = static_cast<uint8_t *>(ws);
-    p.a = a;
-    p.head = reinterpret_cast<PlanHead *>(base);
-    p.blks = reinterpret_cast<TileBlk *>(base + w.blks);
-    p.cost = reinterpret_cast<long long *>(base + w.cost);
-    p.ents = reinterpret_cast<int *>(base + w.ents);
-    p.slots = reinterpret_cast<float *>(base + w.slots);
-    p.ml = reinterpret_cast<float2 *>(base + w.ml);
-    p.acc = reinterpret_cast<float *>(base + w.acc);
-    p.max_blocks = static_cast<int>(w.max_blocks);
-    p.page_rows = a.page_stride / a.head_dim;
-    p.grid = std::min(std::max(1, sm_count(dev)), kMaxTileCtas);
-    const long long rows = a.num_blocks > 0 ? a.num_blocks * p.page_rows : (1LL << 31) - 8;
-    const int box = std::min(a.block_size, 16);
-    CUtensorMap tmk, tmv;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a.kv_dtype == GOLLEK_DTYPE_I8) {
-        int rc = encode_byte_map(&tmk, a.k, a.head_dim, rows, box);
-        if (!rc) rc = encode_byte_map(&tmv, a.v, a.head_dim, rows, box);
-        if (rc) return rc;
-        return a.head_dim == 128 ? launch_tile_as<__nv_bfloat16, 128, true>(p, tmk, tmv, st)
-                                 : launch_tile_as<__nv_bfloat16, 64, true>(p, tmk, tmv, st);
+    PlanArgs both{};
+    for (int i = 0; i < 2; ++i) {
+        const int from = std::min(i, c.lines - 1);  // one line stands twice
+        const auto &l = c.line[from];
+        const TileWs &w = l.ws;
+        uint8_t *base = static_cast<uint8_t *>(ws) + (from ? c.line[0].ws.total : 0);
+        TileArgs &p = both.line[i];
+        p.a = a;
+        p.head = reinterpret_cast<PlanHead *>(base);
+        p.blks = reinterpret_cast<TileBlk *>(base + w.blks);
+        p.cost = reinterpret_cast<long long *>(base + w.cost);
+        p.ents = reinterpret_cast<int *>(base + w.ents);
+        p.slots = reinterpret_cast<float *>(base + w.slots);
+        // the rows' states are the call's, whatever line they come from
+        p.ml = reinterpret_cast<float2 *>(static_cast<uint8_t *>(ws) + c.line[0].ws.ml);
+        p.acc = reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + c.line[0].ws.acc);
+        p.ent0 = l.ent0;
+        p.entities = l.entities;
+        p.blk_rows = l.blk_rows;
+        p.max_blocks = static_cast<int>(w.max_blocks);
+        p.page_rows = a.page_stride / a.head_dim;
+        p.grid = std::min(std::max(1, sm_count(dev)), kMaxTileCtas);
     }
+    CUtensorMap tmk{}, tmv{};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a.kv_dtype == GOLLEK_DTYPE_I8)  // copied without tensor maps
+        return a.head_dim == 128 ? launch_tile_as<__nv_bfloat16, 128, true>(both, c.lines, tmk, tmv, st)
+                                 : launch_tile_as<__nv_bfloat16, 64, true>(both, c.lines, tmk, tmv, st);
+    const long long rows = a.num_blocks > 0 ? a.num_blocks * both.line[0].page_rows : (1LL << 31) - 8;
+    const int box = std::min(a.block_size, 16);
     int rc = encode_tile_map(&tmk, a.k, a.kv_dtype, a.head_dim, rows, box);
     if (!rc) rc = encode_tile_map(&tmv, a.v, a.kv_dtype, a.head_dim, rows, box);
     if (rc) return rc;
     const bool bf16 = a.kv_dtype == GOLLEK_DTYPE_BF16;
     if (a.head_dim == 128)
-        return bf16 ? launch_tile_as<__nv_bfloat16, 128>(p, tmk, tmv, st) : launch_tile_as<__half, 128>(p, tmk, tmv, st);
-    return bf16 ? launch_tile_as<__nv_bfloat16, 64>(p, tmk, tmv, st) : launch_tile_as<__half, 64>(p, tmk, tmv, st);
+        return bf16 ? launch_tile_as<__nv_bfloat16, 128>(both, c.lines, tmk, tmv, st)
+                    : launch_tile_as<__half, 128>(both, c.lines, tmk, tmv, st);
+    return bf16 ? launch_tile_as<__nv_bfloat16, 64>(both, c.lines, tmk, tmv, st)
+                : launch_tile_as<__half, 64>(both, c.lines, tmk, tmv, st);
 }
 
 int launch_attn(AttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
@@ -257,8 +281,7 @@ int launch_attn(AttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
 
 size_t attn_workspace(int num_groups, int num_seqs, int total_q, int hq, int hkv, int D) {
     if (num_seqs <= 0 || total_q <= 0 || num_groups < 0 || hkv <= 0 || hq <= 0 || hq % hkv || D <= 0) return 0;
-    int blk_rows;
-    return attn_ws(num_groups, num_seqs, total_q, hq, hkv, D, &blk_rows).total;
+    return plan_call(num_groups, num_seqs, total_q, hq, hkv, D).total;
 }
 
 template <int KV>
