@@ -92,6 +92,8 @@ class GollekError(RuntimeError):
 def load(path: str | None = None, build_if_missing: bool = True):
     """Loads (building first if the sources are newer) and returns the CDLL."""
     global _lib
+    if _lib is not None and path is None:
+        return _lib
     with _lock:
         if _lib is not None and path is None:
             return _lib

@@ -1,33 +1,42 @@
 // attn_tile.cuh -- ragged and shared-prefix paged attention on the 5th-generation tensor
-// cores, for bf16 or f16 caches with head_dim 64 or 128 and queries of the same type.
+// cores, for bf16 or f16 caches with queries of the same type and int8 caches with bf16
+// queries, head_dim 64 or 128: the plan, the kernel for blocks of many rows, the merge.
+// attn_rows.cuh has the kernel for blocks of few.
 //
 // A block is up to 256 rows -- (query token, q head) pairs of one kv head -- over the
-// positions [lo, hi) that any of them attends, in tiles of 128 positions:
+// positions [lo, hi) that any of them attends, in tiles of 128 positions, the last first:
 //
 //   S[128 rows x 128 pos] = Q . K^T        P = 2^(x - m), rounded to the cache's type
 //   O[128 rows x D]      += P . V          l += sum P (fp32, unrounded)
 //
-// One thread owns one row, so its maximum m and sum l never leave its registers.  S and O
+// One thread owns one row, so its reference m and sum l never leave its registers.  S and O
 // live in tensor memory; P overwrites S there and feeds the value MMA as its A operand, so
 // probabilities never touch shared memory.  P is rounded to 16 bits because both operands
 // of that MMA have one type: a half step of P, averaged over the positions, is of the size
-// of the output's own rounding.  m is a lazy maximum: it moves (and O is rescaled) only
-// when a score passes it by more than 2^kLazyMax, which keeps P below 2^8.
+// of the output's own rounding.  An int8 cache's scales multiply S (K's) and P (V's), never
+// the integers, which would be one rounding more.  m is a lazy maximum: it moves, by a whole
+// number, only when a score passes it by more than 2^kLazyMax; l, O and the columns of P
+// that stand already are then scaled by a power of two.
 //
 // Two row groups of 128 threads keep the tensor core busy while the other computes its
 // probabilities:
 //   blocks of more than 128 rows: group t owns rows 128 t .., every tile serves both;
-//   smaller blocks (decode, a chunk's tail): both groups own the same rows, group t the
-//     tiles t, t + 2, ..., each with its own m, l and O, merged at the end of the run.
+//   smaller blocks (a chunk's tail): both groups own the same rows, group t the tiles t,
+//     t + 2, ..., each with its own m, l and O, merged at the end of the run.
 //
 // Work: the plan kernel lays all tiles of all (block, kv head) units in one line, each unit
-// behind kRunCost tiles' worth of start-up, and cuts it into one equal range per CTA (one
-// CTA per SM).  A unit cut by a range end leaves partial (m, l, O) states, which the merge
-// kernel joins in a fixed order: no atomics, the same bits every time.
+// behind kRunCostTiles tiles' worth of start-up, and cuts it into one equal range per CTA
+// (one CTA per SM).  A unit cut by a range end leaves partial (m, l, O) states, which the
+// merge kernel joins in a fixed order: no atomics, the same bits every time.  Plan and merge
+// take about 6 us each, most of it a launch's latency.
 //
-// Bound by HBM where blocks are small (decode: each page is read once per kv head), by the
-// tensor and exponent pipes for long prompts (both take about as long as the other: 128 x
-// 128 x 128 MACs twice per tile against 16384 exponentials).
+// Bound, for long prompts, by the row groups' pass over S: 128 columns take a group about
+// 1000 clocks of tensor-memory reads and as long again for the exponentials, where the two
+// products take 512 each; two prompts of 2,000 tokens at 8,000 tokens of context (32 q, 8 kv
+// heads of 128, distance bias) take 545 us, 0.87 PFLOP/s.  What moved it: scores read once
+// (572 -> 532 us), groups that take turns at the exponentials (756 -> 522 us with one MMA
+// issuer each and less code).  Code size counts: at 100 KB the roles evicted each other's
+// instructions all the time, which the `unroll 1` loops and opaque() keep down to 60 KB.
 #pragma once
 
 #include <climits>

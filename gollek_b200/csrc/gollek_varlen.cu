@@ -79,17 +79,12 @@ int launch_generic(AttnArgs &a, cudaStream_t st) {
     return GOLLEK_OK;
 }
 
-// Whether the tile kernel takes the call: 16-bit pool and q of one type, or int8 pool and
-// bf16 q (one scale per page and head, or the scales of a page's tokens behind one another);
-// head_dim 64 or 128, pages of 8 or a multiple of 16 tokens in whole 8-row groups, 16-byte
+// Whether the tile kernels take the call: 16-bit pool and q of one type, or int8 pool and
+// bf16 q; head_dim 64 or 128, pages of 8 or a multiple of 16 tokens in whole 8-row groups, 16-byte
 // aligned tensors.
 bool tile_takes(const AttnArgs &a) {
     if (a.kv_dtype == GOLLEK_DTYPE_I8) {
         if (a.q_dtype != GOLLEK_DTYPE_BF16) return false;
-        if (a.scale_token_stride != 0 &&
-            (a.scale_token_stride != 1 || ((a.scale_page_stride | a.scale_head_stride) & 3) || !aligned16(a.k_scales) ||
-             !aligned16(a.v_scales)))
-            return false;
     } else if (a.q_dtype != a.kv_dtype || (a.kv_dtype != GOLLEK_DTYPE_BF16 && a.kv_dtype != GOLLEK_DTYPE_F16)) {
         return false;
     }

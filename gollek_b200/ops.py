@@ -216,15 +216,16 @@ class _on:
 
     def __enter__(self):
         self.guard = None
+        if self.given is None and torch._C._cuda_getDevice() == self.device.index:
+            return torch._C._cuda_getCurrentRawStream(self.device.index)
         if self.given is not None:
             s = self.given
             if not hasattr(s, "cuda_stream"):
                 s = torch.cuda.ExternalStream(int(s), device=self.device)
             self.guard = torch.cuda.stream(s)
-        elif torch.cuda.current_device() != self.device.index:
+        else:
             self.guard = torch.cuda.device(self.device)
-        if self.guard is not None:
-            self.guard.__enter__()
+        self.guard.__enter__()
         return torch.cuda.current_stream(self.device).cuda_stream
 
     def __exit__(self, *exc):
@@ -310,7 +311,7 @@ def paged_attention_shared_prefix(q, k_cache, v_cache, prefix_tables, prefix_len
                                   out=None, workspace=None, stream=None):
     """Decode attention of groups that share prefixes (gollek_paged_attention_shared_prefix):
     q [S, Hq, D] fp32/bf16/f16; sequences group_starts[g] .. group_starts[g+1] - 1 attend the
-    prefix_lens[g] tokens of prefix_tables[g], read once for the group, and then their own
+    prefix_lens[g] tokens of prefix_tables[g], read once for 256 of the group's rows, and their own
     context_lens[s] tokens."""
     dev = _first("q", q, 3)
     S, Hq, D = q.shape

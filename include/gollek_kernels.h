@@ -244,15 +244,19 @@ GOLLEK_API int gollek_paged_attention_v2_noalloc(
  *   token_starts  [total_queries] or NULL: first position a query may attend (packed
  *                 documents: the first position of the query's own document).
  *   sliding_window > 0 needs causal (GOLLEK_ERR_UNSUPPORTED otherwise).
- *   workspace     >= gollek_paged_attention_varlen_workspace_size(...) bytes, its contents
- *                 do not matter; not shared by calls that may overlap on the device (two
+ *   workspace     >= gollek_paged_attention_varlen_workspace_size(...) bytes, 256-byte
+ *                 aligned, its contents do not matter; not shared by calls that may overlap on the device (two
  *                 streams, two captured graphs).  NULL = library-owned scratch per (device,
  *                 stream), which such calls and graphs would share: pass a workspace there.
  * Pool, scales, tables and num_blocks as in gollek_paged_attention_v2; any head_dim up to
- * 256, any GQA group.  K and V at positions that no query attends may hold anything; a NaN
- * or infinity at a position that some query of a sequence attends may also reach outputs of
- * that sequence's other queries.  Asynchronous on `stream`.  Scores, softmax statistics and
- * sums are fp32.
+ * 256, any GQA group.  K and V may hold anything before the first and behind the last
+ * position that a query of their sequence attends; a NaN or infinity in between may also
+ * reach outputs of queries that do not attend it.  Asynchronous on `stream`.  Scores, softmax
+ * statistics and sums are fp32; the tensor-core kernels round probabilities to 16 bits.
+ *   Tensor-core kernels: bf16 or f16 pools with q of the same type, or int8 pools with bf16 q;
+ * head_dim 64 or 128; block_size 8 or a multiple of 16; page_stride a multiple of
+ * 8 * head_dim; 16-byte aligned tensors.  Every other call runs a generic kernel, which is
+ * several times slower.
  */
 GOLLEK_API int gollek_paged_attention_varlen(
     void *out, const void *q, const void *k_cache, const void *v_cache, const float *k_scales,
@@ -271,8 +275,8 @@ GOLLEK_API size_t gollek_paged_attention_varlen_workspace_size(int num_seqs, int
 /*
  * Decode attention of a batch whose sequences share prefixes: sequences group_starts[g] ..
  * group_starts[g+1] - 1 all attend the prefix_lens[g] tokens of group g's table and then
- * their own context_lens[s] tokens, one softmax over both; the prefix is read once for the
- * group.  The pages of a prefix are those that the prompt cache shares between requests
+ * their own context_lens[s] tokens, one softmax over both; the prefix is read once for each
+ * 256 rows (sequence, q head) of a kv head, not once per sequence.  The pages of a prefix are those that the prompt cache shares between requests
  * (optimization/gollek-plugin-prompt-cache/src/main/java/tech/kayys/gollek/cache/PagedKVCacheManagerExtension.java:45-180).
  *
  *   q, out         [num_seqs, num_q_heads, head_dim] of q_dtype (F32, BF16 or F16).

@@ -173,6 +173,51 @@ def test_long_contexts_split_over_the_gpu(cuda_device, ctx, new, kind, qkind):
     check_varlen(cuda_device, case, qkind, slopes=SLOPES(8) / 64)
 
 
+@pytest.mark.parametrize("kind,qkind", [("bf16", "bf16"), ("f16", "f16"), ("i8", "bf16")])
+@pytest.mark.parametrize("what", ["bias", "cap", "window", "prefix", "docs", "all", "full_bias", "plain"])
+def test_few_rows(cuda_device, kind, qkind, what):
+    """Batches of a few queries each (blocks of 16 rows), one sequence with many among them, one with none."""
+    ctx = [200, 333, 129, 40, 700, 1, 128, 0, 127, 256, 1025, 64] + [31 * i % 190 + 1 for i in range(28)]
+    new = [5, 1, 30, 1, 2, 1, 4, 0, 1, 3, 1, 1] + [1] * 28
+    rng = np.random.default_rng(70)
+    kw = {}
+    if what in ("bias", "all", "full_bias"):
+        kw["slopes"] = SLOPES(8)
+    if what in ("cap", "all"):
+        kw["cap"] = 2.0
+    if what in ("window", "all"):
+        kw["window"] = 37
+    if what in ("prefix", "all"):
+        kw["prefix"] = np.arange(40, dtype=np.int32) * 11
+    if what in ("docs", "all"):
+        kw["starts"] = np.concatenate([np.maximum(0, c - n + np.arange(n) - rng.integers(-2, 60, n))
+                                       for c, n in zip(ctx, new)]).astype(np.int32)
+    if what == "full_bias":
+        kw["causal"] = False
+    case = varlen_case(ctx, new, 8, 2, 128, 16, kind, qkind, 71)
+    check_varlen(cuda_device, case, qkind, **kw)
+
+
+@pytest.mark.parametrize("hq,hkv,bs,scales", [(4, 4, 16, "token"), (32, 8, 8, "token"), (16, 2, 48, "page"),
+                                              (16, 1, 64, "token"), (24, 2, 8, "page")])
+@pytest.mark.parametrize("kind", ["bf16", "i8"])
+def test_few_rows_in_turn(cuda_device, hq, hkv, bs, scales, kind):
+    """Runs of one tile and of many behind one another, cut anywhere by the ends of the SMs' shares."""
+    rng = np.random.default_rng(72)
+    for rep in range(2):
+        n = 70
+        ctx = np.where(rng.random(n) < 0.5, rng.integers(1, 140, n), rng.integers(128, 2500, n))
+        case = varlen_case(ctx, [1] * n, hq, hkv, 128, bs, kind, "bf16", 73 + rep, scales=scales)
+        check_varlen(cuda_device, case, "bf16", slopes=SLOPES(hq) / 32 if rep else None)
+
+
+@pytest.mark.parametrize("kind,qkind", [("bf16", "bf16"), ("f16", "f16"), ("i8", "bf16")])
+def test_few_rows_large_scores(cuda_device, kind, qkind):
+    """Maxima that keep rising from tile to tile: the references of all warps of a group move together."""
+    q, pool, tables, cu, ctx = varlen_case([1500, 700, 2000, 129], [1] * 4, 8, 2, 128, 16, kind, qkind, 74)
+    check_varlen(cuda_device, (rounded(q * 12, qkind), pool, tables, cu, ctx), qkind)
+
+
 @pytest.mark.parametrize("hq,hkv,window,cap", [(32, 8, 1024, 30.0), (8, 8, 0, 0.0), (12, 4, 200, 0.0), (64, 2, 0, 4.0)])
 def test_large_and_small_blocks_in_turn(cuda_device, hq, hkv, window, cap):
     """Blocks of more and of fewer than 128 rows, of many tiles and of one, behind one another in every order: what the
@@ -286,6 +331,19 @@ def test_shared_prefix_many_sequences(cuda_device, seqs, plen, hq, hkv):
     rng = np.random.default_rng(22)
     case = shared_case([plen], [0, seqs], rng.integers(0, 300, seqs), hq, hkv, 128, 16, "bf16", "bf16", 22)
     check_shared(cuda_device, case, "bf16")
+
+
+@pytest.mark.parametrize("kind,qkind", [("bf16", "bf16"), ("f16", "f16"), ("i8", "bf16")])
+@pytest.mark.parametrize("hq,hkv,seqs", [(16, 4, 64), (32, 2, 130), (8, 8, 40), (34, 2, 130)])
+def test_shared_prefix_own_tokens_apart(cuda_device, kind, qkind, hq, hkv, seqs):
+    """Batches whose own tokens alone fill the device (16 rows at most per sequence and kv head: a kernel of their
+    own; 17: the same kernel for all), in groups of every size and outside them."""
+    rng = np.random.default_rng(24)
+    ctx = np.where(rng.random(seqs) < 0.2, 0, rng.integers(1, 500, seqs))
+    case = shared_case([0, 900, 130, 1], [1, 5, seqs // 2, seqs // 2, seqs - 3], ctx, hq, hkv, 128, 16, kind, qkind, 25)
+    got = check_shared(cuda_device, case, qkind, cap=0.0 if kind == "f16" else 5.0)
+    if ctx[0] == 0:
+        assert (got[0] == 0).all()
 
 
 def test_shared_prefix_equals_the_prefix_in_every_table(cuda_device):
