@@ -177,6 +177,8 @@ __global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(const __grid_co
     const int G = a.num_q_heads / a.num_kv_heads;
     const int tid = threadIdx.x;
     __shared__ long long sm_l[32];
+    __shared__ int2 sm_rows[kPlanThreads];  // token_starts: first query token and tokens of a block
+    __shared__ int sm_least[kPlanThreads];
     pdl_launch();
 
     // first block of every entity; sizes that do not fit their tables are reported once
@@ -253,19 +255,20 @@ __global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(const __grid_co
                 if (a.window > 0) k.lo = max(k.lo, pos0 - a.window + 1);
             }
         }
-        if (docs) {  // one warp per block: the smallest first position of its queries
-            const int lane = tid & 31;
-            for (int u = 0; u < 32; ++u) {
-                const int nrows = __shfl_sync(0xffffffffu, k.nrows, u);
-                const int row0 = __shfl_sync(0xffffffffu, k.row0, u), tok0 = __shfl_sync(0xffffffffu, k.tok0, u);
-                if (nrows <= 0) continue;
-                const int i0 = row0 / G, i1 = (row0 + nrows - 1) / G;
+        if (docs) {  // the smallest first position of each block's queries: a warp per block, all warps in turn
+            sm_rows[tid] = make_int2(k.nrows > 0 ? k.tok0 + k.row0 / G : 0, k.nrows > 0 ? (k.row0 + k.nrows - 1) / G - k.row0 / G + 1 : 0);
+            __syncthreads();
+            const int lane = tid & 31, here = static_cast<int>(min(nb - b0, static_cast<long long>(kPlanThreads)));
+#pragma unroll 4
+            for (int u = tid >> 5; u < here; u += kPlanThreads / 32) {
+                const int2 r = sm_rows[u];
                 int least = INT_MAX;
-                for (int i = i0 + lane; i <= i1; i += 32) least = min(least, a.token_starts[tok0 + i]);
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
-                if (lane == u) k.lo = max(k.lo, least);
+                for (int i = lane; i < r.y; i += 32) least = min(least, a.token_starts[r.x + i]);
+                least = __reduce_min_sync(0xffffffffu, least);
+                if (lane == 0) sm_least[u] = least;
             }
+            __syncthreads();
+            if (k.nrows > 0) k.lo = max(k.lo, sm_least[tid]);
         }
         long long c = 0;
         if (b < nb) {

@@ -2,6 +2,7 @@
 // cache read-back: argument checks, kernel selection and their C ABI (gollek_kernels.h).
 #include <algorithm>
 
+#include "attn_block.cuh"
 #include "attn_rows.cuh"
 #include "attn_tile.cuh"
 #include "host.cuh"
@@ -68,8 +69,32 @@ const void *generic_fn(int G) {
     return reinterpret_cast<const void *>(&attn_generic_kernel<J, 4>);
 }
 
+template <int DP>
+int launch_block(AttnArgs &a, cudaStream_t st) {
+    const void *fn = a.kv_dtype == GOLLEK_DTYPE_F32    ? reinterpret_cast<const void *>(&attn_block_kernel<DP, GOLLEK_DTYPE_F32>)
+                     : a.kv_dtype == GOLLEK_DTYPE_BF16 ? reinterpret_cast<const void *>(&attn_block_kernel<DP, GOLLEK_DTYPE_BF16>)
+                     : a.kv_dtype == GOLLEK_DTYPE_F16  ? reinterpret_cast<const void *>(&attn_block_kernel<DP, GOLLEK_DTYPE_F16>)
+                     : a.kv_dtype == GOLLEK_DTYPE_I8   ? reinterpret_cast<const void *>(&attn_block_kernel<DP, GOLLEK_DTYPE_I8>)
+                                                       : reinterpret_cast<const void *>(&attn_block_kernel<DP, GOLLEK_DTYPE_I4>);
+    GK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kAbSmem<DP>)), "cudaFuncSetAttribute");
+    int qt = kAbRows / (a.num_q_heads / a.num_kv_heads);
+    void *args[] = {&a, &qt};
+    const long long blocks = a.total_q / qt + static_cast<long long>(a.num_seqs);
+    GK_CUDA(cudaLaunchKernel(fn, dim3(static_cast<unsigned>(blocks), a.num_kv_heads), dim3(kAbThreads), args, kAbSmem<DP>, st),
+            "attn_block_kernel launch");
+    return GOLLEK_OK;
+}
+
+// Calls that the tensor-core kernels do not take.  Varlen calls of kBlockRows rows and more a
+// sequence on average go to the blocked kernel, which reads a cache row once for 64 of them (8
+// fp32 sequences of 400 to 1500 tokens, 4 rows a query token: 16 rows 297 us there and 191 in
+// the other, 32 rows 301 and 363, 384 rows 788 and 3232).
+constexpr int kBlockRows = 32;
+
 int launch_generic(AttnArgs &a, cudaStream_t st) {
     const int G = a.num_q_heads / a.num_kv_heads;
+    if (a.num_groups == 0 && G <= kAbRows && static_cast<long long>(a.total_q) * G >= static_cast<long long>(a.num_seqs) * kBlockRows)
+        return a.head_dim <= 64 ? launch_block<64>(a, st) : a.head_dim <= 128 ? launch_block<128>(a, st) : launch_block<256>(a, st);
     const int J = a.head_dim <= 64 ? 2 : a.head_dim <= 128 ? 4 : 8;
     const void *fn = J == 2 ? generic_fn<2>(G) : J == 4 ? generic_fn<4>(G) : generic_fn<8>(G);
     const int GC = G == 1 ? 1 : G == 2 ? 2 : (G <= 4 || J == 8) ? 4 : 8;

@@ -126,6 +126,16 @@ def test_masks_and_bias(cuda_device, kind, qkind, what):
     check_varlen(cuda_device, case, qkind, **kw)
 
 
+@pytest.mark.parametrize("kind,qkind", [("f32", "f32"), ("i4", "bf16"), ("i8", "f32"), ("bf16", "f32"), ("f16", "bf16")])
+@pytest.mark.parametrize("hq,hkv,d,bs", [(5, 1, 96, 16), (6, 6, 10, 7), (4, 2, 256, 8), (20, 4, 128, 24), (64, 1, 34, 16),
+                                         (65, 1, 16, 16)])
+def test_ragged_prompts_of_odd_shapes(cuda_device, kind, qkind, hq, hkv, d, bs):
+    """Prompts outside the tensor-core kernels: blocks of 64 rows that end anywhere in a sequence, 64 heads and more."""
+    case = varlen_case([90, 0, 33, 1, 70, 41], [33, 0, 33, 1, 12, 40], hq, hkv, d, bs, kind, qkind, 75, gap=2)
+    check_varlen(cuda_device, case, qkind, slopes=SLOPES(hq), window=50, cap=3.0)
+    check_varlen(cuda_device, case, qkind, prefix=np.array([80, 0, 5, 1, 70, 9], np.int32))
+
+
 def test_rows_with_nothing_to_see_are_zero(cuda_device):
     q, pool, tables, cu, ctx = varlen_case([70, 20], [70, 20], 8, 2, 128, 16, "bf16", "bf16", 4)
     starts = np.concatenate([np.arange(70) + 1, np.full(20, 10 ** 9)]).astype(np.int32)
@@ -209,6 +219,29 @@ def test_few_rows_in_turn(cuda_device, hq, hkv, bs, scales, kind):
         ctx = np.where(rng.random(n) < 0.5, rng.integers(1, 140, n), rng.integers(128, 2500, n))
         case = varlen_case(ctx, [1] * n, hq, hkv, 128, bs, kind, "bf16", 73 + rep, scales=scales)
         check_varlen(cuda_device, case, "bf16", slopes=SLOPES(hq) / 32 if rep else None)
+
+
+@pytest.mark.parametrize("hq,hkv", [(10, 2), (12, 4), (7, 1)])
+@pytest.mark.parametrize("kind", ["bf16", "i8"])
+def test_few_rows_cut_inside_a_token(cuda_device, hq, hkv, kind):
+    """Groups that do not divide 16: blocks end between the heads of one query token."""
+    new = [1, 2, 3, 5, 9, 1, 1, 2, 1, 1] + [1] * 20
+    ctx = [13 * i + n for i, n in enumerate(new)]
+    case = varlen_case(ctx, new, hq, hkv, 128, 16, kind, "bf16", 76)
+    check_varlen(cuda_device, case, "bf16", slopes=SLOPES(hq), window=200)
+
+
+def test_documents_of_more_blocks_than_plan_threads(cuda_device):
+    """token_starts over more than 1,024 blocks, the last ones of a few rows."""
+    rng = np.random.default_rng(77)
+    n = 1100
+    new = rng.integers(1, 5, n)
+    ctx = new + rng.integers(0, 40, n)
+    starts = np.concatenate([rng.integers(0, c, k) for c, k in zip(ctx, new)]).astype(np.int32)
+    case = varlen_case(ctx, new, 16, 2, 128, 16, "bf16", "bf16", 78)
+    check_varlen(cuda_device, case, "bf16", starts=starts)
+    case = varlen_case(ctx, new, 16, 2, 64, 16, "bf16", "bf16", 78)
+    check_varlen(cuda_device, case, "bf16", starts=starts)
 
 
 @pytest.mark.parametrize("kind,qkind", [("bf16", "bf16"), ("f16", "f16"), ("i8", "bf16")])
