@@ -472,17 +472,17 @@ __global__ void __launch_bounds__(kRowsThreads + (Q8 ? kRowsConverters : 0), 1)
                     fb *= inv;
                 }
                 // a partial state goes to the CTA's slot, a whole unit's of a call with prefixes to its row's place
-                float *st_o = p.slots + (static_cast<size_t>(blockIdx.x) * 2 + (d.flags >> 3 & 1)) * (kBlkRows * (D + 2));
+                float *st_o = p.slots + (static_cast<size_t>(blockIdx.x) * 2 + (d.flags >> 3 & 1)) * (N * (D + 2));
                 const long long own = static_cast<long long>(a.total_q) * a.num_q_heads;
                 if (w4 == 0 && lane < d.nrows) {
                     if (!whole) {
                         st_o[lane] = mm;
-                        st_o[kBlkRows + lane] = ll;
+                        st_o[N + lane] = ll;
                     } else if (!direct) {
                         p.ml[own + out_row] = make_float2(mm, ll);
                     }
                 }
-                st_o = whole ? p.acc + (own + out0) * D : st_o + 2 * kBlkRows;
+                st_o = whole ? p.acc + (own + out0) * D : st_o + 2 * N;
                 // each row's factors and place, in the room of the run's RowInfo
                 __syncwarp();
                 if (lane < N) info[lane] = RowInfo{ll == 0.f, whole ? static_cast<int>(out_row - out0) : lane, __float_as_int(fa), fb};

@@ -95,7 +95,7 @@ inline TileWs tile_ws(long long entities, long long rows, int blk_rows, long lon
     w.ents = o;
     o = up256(o + (entities + 1) * 4);
     w.slots = o;
-    o = up256(o + static_cast<size_t>(kMaxTileCtas) * 2 * kBlkRows * (D + 2) * 4);
+    o = up256(o + static_cast<size_t>(kMaxTileCtas) * 2 * blk_rows * (D + 2) * 4);
     w.ml = o;
     if (shared) o = up256(o + out_rows * 4 * 4);  // (m, l) of the prefix and of the own tokens, per row
     w.acc = o;
@@ -110,11 +110,12 @@ struct TileArgs {
     TileBlk *blks;
     long long *cost;  // [max_blocks + 1] start of each block's cost, per kv head
     int *ents;        // [entities + 1] first block of each entity
-    float *slots;     // [CTA][2]: ml [2][256], O [256][D]
+    float *slots;     // [CTA][2]: ml [2][blk_rows], O [blk_rows][D]
     float2 *ml;       // shared: [2][rows]
     float *acc;       // shared: [2][rows][D]
     int ent0, entities, grid, max_blocks;  // entities ent0 .. ent0 + entities - 1 of the call
     int blk_rows;     // rows a block may have
+    int rows_min, rows_max;  // entities of rows_min .. rows_max rows are this line's, the rest another's
     long long page_rows;
 };
 
@@ -194,7 +195,8 @@ __global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(const __grid_co
                 check_group(a, ent);
             else
                 check_seq(a, ent - a.num_groups);
-            blocks = (static_cast<long long>(entity_tokens(a, ent)) * G + p.blk_rows - 1) / p.blk_rows;
+            const long long rows = static_cast<long long>(entity_tokens(a, ent)) * G;
+            if (rows >= p.rows_min && rows <= p.rows_max) blocks = (rows + p.blk_rows - 1) / p.blk_rows;
         }
         long long sum;
         const long long at = block_scan(blocks, sm_l, &sum);
@@ -1513,10 +1515,10 @@ __device__ __forceinline__ bool add_pieces(const TileArgs &p, long long range, l
             run_tiles(v0, v1 - v0, ta, tb);
             if (ta >= tb) continue;
             if (ta == 0 && tb == n) return false;
-            const float *slot = p.slots + (static_cast<size_t>(b + k) * 2 + (ta == 0 ? 1 : 0)) * (kBlkRows * (D + 2));
+            const float *slot = p.slots + (static_cast<size_t>(b + k) * 2 + (ta == 0 ? 1 : 0)) * (p.blk_rows * (D + 2));
             pm[k] = __ldcg(slot + ri);
-            pl[k] = __ldcg(slot + kBlkRows + ri);
-            load_cols<C>(slot + 2 * kBlkRows + ri * D, lane, po[k]);
+            pl[k] = __ldcg(slot + p.blk_rows + ri);
+            load_cols<C>(slot + 2 * p.blk_rows + ri * D, lane, po[k]);
         }
 #pragma unroll
         for (int k = 0; k < B; ++k) st.add(pm[k], pl[k], po[k]);
@@ -1541,10 +1543,11 @@ __device__ __forceinline__ void write_row(const TileArgs &p, long long row, int 
 constexpr int kMergeThreads = 256;
 constexpr int kMergeSplit = 8;
 
-// Varlen.  CTA (c, y): rows y * 8 + warp, ... of the unit that starts in range c and goes on
+// Varlen.  CTA (c, y, line): rows y * 8 + warp, ... of the unit that starts in range c and goes on
 // behind it; and zeros for the rows of blocks that attend nothing.
 template <typename T, int D>
-__global__ void __launch_bounds__(kMergeThreads) tile_merge_kernel(const TileArgs p) {
+__global__ void __launch_bounds__(kMergeThreads) tile_merge_kernel(const __grid_constant__ PlanArgs both) {
+    const TileArgs &p = both.line[blockIdx.z];
     const AttnArgs &a = p.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = a.num_q_heads / a.num_kv_heads;

@@ -121,51 +121,58 @@ bool tile_takes(const AttnArgs &a) {
     return a.num_blocks == 0 || a.num_blocks * page_rows < (1LL << 31);
 }
 
-// How the entities of a call are laid out: one cost line, or (shared prefixes) one for the
-// prefixes and one for the own tokens, each with its part of the workspace.
+// How the entities of a call are laid out: one cost line for each kernel that takes some of
+// them, each with its part of the workspace.
 struct CallPlan {
     struct Line {
-        int ent0, entities, blk_rows;
+        int ent0, entities, blk_rows, rows_min, rows_max;
         TileWs ws;
+        size_t at;  // of ws
     } line[2];
     int lines;
     size_t total;
 };
 
-// Blocks of few rows go to attn_rows_kernel (head_dim 128):
-// - varlen calls whose sequences have 16 rows at most on average (a longer one is cut into
-//   blocks of 16, each of which reads its pages): 237 -> 183 us for 64 sequences of one token;
-// - the own tokens of shared-prefix calls of up to 16 q heads per kv head, once they alone
-//   give the device kSplitUnits units of work; below, one more launch costs more than it saves.
+// attn_rows_kernel (head_dim 128, up to 16 q heads per kv head) takes entities of 16 rows at
+// most: 237 -> 183 us for 64 sequences of one token.  What a call gives it, and what the kernel
+// for many rows, is chosen from the sizes alone:
+// - varlen, no more query tokens than sequences: all, whatever their rows (a longer entity is
+//   cut into blocks of 16, each of which reads its pages);
+// - otherwise, once the sequences give the device kSplitUnits units of work: varlen, the entities
+//   of few rows, the rest going to the kernel for many (60 decode steps beside 4 chunks of 200
+//   tokens 392 -> 281 us, beside 4 of 1000 645 -> 533, 64 sequences of 8 tokens 222.5 -> 223.4);
+//   shared prefixes, the own tokens (64 sequences behind 4,096 tokens 82 -> 67 us).  Below, the
+//   launch costs more than it saves (8 sequences behind 500 tokens 19.6 us, 26.5 in two).
+// The layout of the workspace does not depend on the choice, so that what is enough for a call
+// is enough for smaller ones.
 constexpr int kSplitUnits = 256;
 
 CallPlan plan_call(int num_groups, int num_seqs, int total_q, int hq, int hkv, int D) {
     const int G = hq / hkv;
+    const bool shared = num_groups > 0;
     const long long rows = static_cast<long long>(total_q) * G, out_rows = static_cast<long long>(total_q) * hq;
-    const bool few = D == kFewD && G <= kFewRows;
     CallPlan c{};
+    const CallPlan::Line many{0, num_groups + num_seqs, kBlkRows, 0, INT_MAX,
+                              tile_ws(static_cast<long long>(num_groups) + num_seqs, shared ? 2 * rows : rows, kBlkRows, out_rows, D, shared), 0};
+    c.line[0] = many;
     c.lines = 1;
-    auto &l = c.line[0];
-    if (num_groups == 0) {
-        l.entities = num_seqs;
-        l.blk_rows = few && rows <= static_cast<long long>(num_seqs) * kFewRows ? kFewRows : kBlkRows;
-        l.ws = tile_ws(num_seqs, rows, l.blk_rows, 0, D, false);
-    } else if (few && static_cast<long long>(num_seqs) * hkv >= kSplitUnits) {
-        auto &own = c.line[1];
+    c.total = many.ws.total;
+    if (D != kFewD || G > kFewRows) return c;
+    const CallPlan::Line few{0, num_seqs, kFewRows, 0, INT_MAX, tile_ws(num_seqs, rows, kFewRows, 0, D, false), c.total};
+    c.total += few.ws.total;
+    if (!shared && total_q <= num_seqs) {
+        c.line[0] = few;
+    } else if (static_cast<long long>(num_seqs) * hkv >= kSplitUnits) {
         c.lines = 2;
-        l.entities = num_groups;
-        l.blk_rows = kBlkRows;
-        l.ws = tile_ws(num_groups, rows, kBlkRows, out_rows, D, true);
-        own.ent0 = num_groups;
-        own.entities = num_seqs;
-        own.blk_rows = kFewRows;
-        own.ws = tile_ws(num_seqs, rows, kFewRows, 0, D, false);
-    } else {
-        l.entities = num_groups + num_seqs;
-        l.blk_rows = kBlkRows;
-        l.ws = tile_ws(static_cast<long long>(num_groups) + num_seqs, 2 * rows, kBlkRows, out_rows, D, true);
+        c.line[1] = few;
+        if (shared) {
+            c.line[0].entities = num_groups;
+            c.line[1].ent0 = num_groups;
+        } else {
+            c.line[0].rows_min = kFewRows + 1;
+            c.line[1].rows_max = kFewRows;
+        }
     }
-    c.total = l.ws.total + c.line[1].ws.total;
     return c;
 }
 
@@ -230,10 +237,10 @@ int launch_tile_as(const PlanArgs &both, int lines, const CUtensorMap &tmk, cons
         int rc = launch_dependent(fn, dim3(p.grid), threads, smem, st, args, "attention kernel launch");
         if (rc) return rc;
     }
-    void *margs[] = {const_cast<PlanArgs *>(&both)}, *margs1[] = {const_cast<TileArgs *>(&both.line[0])};
+    void *margs[] = {const_cast<PlanArgs *>(&both)};
     if (a.num_groups == 0)
-        return launch_dependent(reinterpret_cast<const void *>(&tile_merge_kernel<T, D>), dim3(both.line[0].grid, kMergeSplit),
-                                kMergeThreads, 0, st, margs1, "tile_merge_kernel launch");
+        return launch_dependent(reinterpret_cast<const void *>(&tile_merge_kernel<T, D>), dim3(both.line[0].grid, kMergeSplit, lines),
+                                kMergeThreads, 0, st, margs, "tile_merge_kernel launch");
     const long long rows = static_cast<long long>(a.num_seqs) * a.num_q_heads;
     return launch_dependent(reinterpret_cast<const void *>(&tile_merge_shared_kernel<T, D>),
                             dim3(static_cast<unsigned>((rows + kMergeThreads / 32 - 1) / (kMergeThreads / 32))), kMergeThreads,
@@ -258,7 +265,7 @@ int launch_tile(AttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
         const int from = std::min(i, c.lines - 1);  // one line stands twice
         const auto &l = c.line[from];
         const TileWs &w = l.ws;
-        uint8_t *base = static_cast<uint8_t *>(ws) + (from ? c.line[0].ws.total : 0);
+        uint8_t *base = static_cast<uint8_t *>(ws) + l.at;
         TileArgs &p = both.line[i];
         p.a = a;
         p.head = reinterpret_cast<PlanHead *>(base);
@@ -272,6 +279,8 @@ int launch_tile(AttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
         p.ent0 = l.ent0;
         p.entities = l.entities;
         p.blk_rows = l.blk_rows;
+        p.rows_min = l.rows_min;
+        p.rows_max = l.rows_max;
         p.max_blocks = static_cast<int>(w.max_blocks);
         p.page_rows = a.page_stride / a.head_dim;
         p.grid = std::min(std::max(1, sm_count(dev)), kMaxTileCtas);

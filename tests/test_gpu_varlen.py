@@ -186,13 +186,13 @@ def test_long_contexts_split_over_the_gpu(cuda_device, ctx, new, kind, qkind):
 @pytest.mark.parametrize("kind,qkind", [("bf16", "bf16"), ("f16", "f16"), ("i8", "bf16")])
 @pytest.mark.parametrize("what", ["bias", "cap", "window", "prefix", "docs", "all", "full_bias", "plain"])
 def test_few_rows(cuda_device, kind, qkind, what):
-    """Batches of a few queries each (blocks of 16 rows), one sequence with many among them, one with none."""
+    """Batches of a few queries each (at most 16 rows), one sequence with many among them, one with none."""
     ctx = [200, 333, 129, 40, 700, 1, 128, 0, 127, 256, 1025, 64] + [31 * i % 190 + 1 for i in range(28)]
     new = [5, 1, 30, 1, 2, 1, 4, 0, 1, 3, 1, 1] + [1] * 28
     rng = np.random.default_rng(70)
     kw = {}
     if what in ("bias", "all", "full_bias"):
-        kw["slopes"] = SLOPES(8)
+        kw["slopes"] = SLOPES(32)
     if what in ("cap", "all"):
         kw["cap"] = 2.0
     if what in ("window", "all"):
@@ -204,8 +204,18 @@ def test_few_rows(cuda_device, kind, qkind, what):
                                        for c, n in zip(ctx, new)]).astype(np.int32)
     if what == "full_bias":
         kw["causal"] = False
-    case = varlen_case(ctx, new, 8, 2, 128, 16, kind, qkind, 71)
+    case = varlen_case(ctx, new, 32, 8, 128, 16, kind, qkind, 71)
     check_varlen(cuda_device, case, qkind, **kw)
+
+
+@pytest.mark.parametrize("kind,qkind", [("bf16", "bf16"), ("i8", "bf16")])
+def test_many_rows_in_blocks_of_few(cuda_device, kind, qkind):
+    """No more tokens than sequences, but most of them in one: its rows go in blocks of 16."""
+    new = [1, 30, 0, 3, 1] + [0] * 33
+    ctx = [400, 1300, 50, 3, 129] + [7] * 33
+    case = varlen_case(ctx, new, 10, 2, 128, 16, kind, qkind, 81)
+    check_varlen(cuda_device, case, qkind, slopes=SLOPES(10), cap=2.0, prefix=np.array([0, 1290, 0, 0, 0] + [0] * 33, np.int32))
+    check_varlen(cuda_device, case, qkind, window=300)
 
 
 @pytest.mark.parametrize("hq,hkv,bs,scales", [(4, 4, 16, "token"), (32, 8, 8, "token"), (16, 2, 48, "page"),
@@ -221,7 +231,7 @@ def test_few_rows_in_turn(cuda_device, hq, hkv, bs, scales, kind):
         check_varlen(cuda_device, case, "bf16", slopes=SLOPES(hq) / 32 if rep else None)
 
 
-@pytest.mark.parametrize("hq,hkv", [(10, 2), (12, 4), (7, 1)])
+@pytest.mark.parametrize("hq,hkv", [(10, 2), (12, 4), (7, 1), (45, 9)])
 @pytest.mark.parametrize("kind", ["bf16", "i8"])
 def test_few_rows_cut_inside_a_token(cuda_device, hq, hkv, kind):
     """Groups that do not divide 16: blocks end between the heads of one query token."""
@@ -229,6 +239,22 @@ def test_few_rows_cut_inside_a_token(cuda_device, hq, hkv, kind):
     ctx = [13 * i + n for i, n in enumerate(new)]
     case = varlen_case(ctx, new, hq, hkv, 128, 16, kind, "bf16", 76)
     check_varlen(cuda_device, case, "bf16", slopes=SLOPES(hq), window=200)
+
+
+@pytest.mark.parametrize("kind,qkind", [("bf16", "bf16"), ("f16", "f16"), ("i8", "bf16")])
+@pytest.mark.parametrize("what", ["plain", "bias", "cap", "window", "docs"])
+def test_few_rows_beside_many(cuda_device, kind, qkind, what):
+    """Decode steps, short drafts and prompt chunks in one call: each goes to the kernel for its rows, and a call
+    has parts that both cut over the ends of their shares."""
+    rng = np.random.default_rng(79)
+    new = np.array([1, 1, 200, 1, 4, 0, 1, 5, 1, 33, 1, 1, 3, 1, 90] + [1] * 25)
+    ctx = new + rng.integers(0, 900, len(new))
+    kw = {"slopes": SLOPES(32)} if what == "bias" else {"cap": 3.0} if what == "cap" else {"window": 70} if what == "window" else {}
+    if what == "docs":
+        kw["starts"] = np.concatenate([np.maximum(0, c - n + np.arange(n) - rng.integers(-2, 400, n))
+                                       for c, n in zip(ctx, new)]).astype(np.int32)
+    case = varlen_case(ctx, new, 32, 8, 128, 16, kind, qkind, 80, window=kw.get("window", 0))
+    check_varlen(cuda_device, case, qkind, **kw)
 
 
 def test_documents_of_more_blocks_than_plan_threads(cuda_device):

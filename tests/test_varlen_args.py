@@ -131,3 +131,18 @@ def test_reference_known_answers():
     assert np.allclose(out[0, 0], (np.array([4, 5]) / 4 + np.array([6, 7]) / 2 + np.array([0, 1])) / 1.75)
     out = R.shared_prefix(q[:1], pool, np.array([[1]]), [2], [0, 1], np.array([[0]]), [1], 1.0)
     assert np.allclose(out[0, 0], [10 / 3, 13 / 3])
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (8, 8, 64), (64, 2, 128), (20, 4, 96)])
+def test_a_workspace_for_more_is_enough_for_less(hq, hkv, d):
+    """Callers keep the workspace of their largest batch, whichever kernels smaller ones go to."""
+    from gollek_b200 import ops
+    seqs, tokens = [1, 2, 31, 32, 33, 64, 300], [1, 2, 64, 65, 500, 1024, 5000, 40000]
+    size = {(s, t): ops.varlen_workspace_size(s, t, hq, hkv, d) for s in seqs for t in tokens}
+    for (s, t), n in size.items():
+        assert n > 0
+        assert all(n <= size[s2, t2] for s2 in seqs for t2 in tokens if s2 >= s and t2 >= t)
+    size = {(g, s): ops.shared_prefix_workspace_size(g, s, hq, hkv, d) for g in (1, 2, 40) for s in seqs}
+    for (g, s), n in size.items():
+        assert n > 0
+        assert all(n <= size[g2, s2] for g2 in (1, 2, 40) for s2 in seqs if g2 >= g and s2 >= s)
