@@ -15,8 +15,9 @@
 // Bound by HBM for 16-bit caches, each page being read once per kv head: a decode step of 64
 // sequences of 512 to 8192 tokens (32 q, 8 kv heads of 128) takes 183 us, 6.2 TB/s (237 us
 // in attn_tile.cuh's kernel, whose blocks of 128 rows are empty but for 4).  For int8 caches
-// by the instructions that turn bytes into bf16 (some 8,000 a tile and SM, issued in 57% of
-// the slots): 48 such sequences take 191 us, 2.4 TB/s (286 us there).  K is converted by warps of its own, V by the group whose
+// by the instructions that turn bytes into bf16 (of 8,700 a tile, issued in 57% of the slots,
+// before their address arithmetic went): 48 such sequences take 191 us, 2.4 TB/s (286 us
+// there).  K is converted by warps of its own, V by the group whose
 // tile it is, which would wait for its scores' MMA meanwhile.
 #pragma once
 
