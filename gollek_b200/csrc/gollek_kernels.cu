@@ -81,9 +81,9 @@ PFN_cuMemGetAddressRange_v3020 address_range_fn() {
 
 std::mutex g_mu;
 std::map<int, int> g_sm_count;
-// (device, stream, thread) -> scratch.  The thread is part of the key only for the
+// (device, stream, thread, kind) -> scratch.  The thread is part of the key only for the
 // per-thread default stream, whose handle is the same constant on every thread.
-std::map<std::tuple<int, void *, size_t>, std::pair<void *, size_t>> g_ws;
+std::map<std::tuple<int, void *, size_t, Scratch>, std::pair<void *, size_t>> g_ws;
 
 int sm_count(int dev) {
     std::lock_guard<std::mutex> lk(g_mu);
@@ -95,14 +95,14 @@ int sm_count(int dev) {
     return n;
 }
 
-// Library-owned split-K scratch for (device, stream), zero-filled when (re)allocated;
+// Library-owned scratch of one kind for (device, stream), zero-filled when (re)allocated;
 // *cap_out receives its size.
-int library_workspace(int dev, void *stream, size_t bytes, void **out, size_t *cap_out) {
+int library_workspace(int dev, void *stream, Scratch kind, size_t bytes, void **out, size_t *cap_out) {
     const size_t tkey = stream == static_cast<void *>(cudaStreamPerThread)
                             ? std::hash<std::thread::id>()(std::this_thread::get_id())
                             : 0;
     std::lock_guard<std::mutex> lk(g_mu);
-    auto &slot = g_ws[std::make_tuple(dev, stream, tkey)];
+    auto &slot = g_ws[std::make_tuple(dev, stream, tkey, kind)];
     if (slot.second < bytes) {
         if (slot.first) {
             cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
@@ -110,9 +110,9 @@ int library_workspace(int dev, void *stream, size_t bytes, void **out, size_t *c
             slot = {nullptr, 0};
         }
         void *p = nullptr;
-        GK_CUDA(cudaMalloc(&p, bytes), "cudaMalloc(split-K workspace)");
+        GK_CUDA(cudaMalloc(&p, bytes), "cudaMalloc(library scratch)");
         GK_CUDA(cudaMemsetAsync(p, 0, bytes, static_cast<cudaStream_t>(stream)),
-                "cudaMemsetAsync(split-K workspace)");
+                "cudaMemsetAsync(library scratch)");
         slot = {p, bytes};
     }
     *out = slot.first;
@@ -398,7 +398,7 @@ int v2_workspace(const V2 &p, int dev, void **ws, size_t *cap) {
             return fail(GOLLEK_ERR_WORKSPACE, "workspace of %zu bytes < %zu needed", p.workspace_bytes, need);
         return GOLLEK_OK;
     }
-    return library_workspace(dev, p.stream, need, ws, cap);
+    return library_workspace(dev, p.stream, Scratch::kSplitK, need, ws, cap);
 }
 
 // 2-D tensor maps over the K and V pools: rows of head_dim elements, boxes of 128 bytes
@@ -846,7 +846,7 @@ int check_v2(const V2 &p) {
 int rezero_library_counters(int dev) {
     std::lock_guard<std::mutex> lk(g_mu);
     for (auto &kv : g_ws) {
-        if (std::get<0>(kv.first) != dev || !kv.second.first) continue;
+        if (std::get<0>(kv.first) != dev || std::get<3>(kv.first) != Scratch::kSplitK || !kv.second.first) continue;
         GK_CUDA(cudaMemset(kv.second.first, 0, ws_counter_region(kv.second.second)),
                 "cudaMemset(split-K counters after a timeout)");
     }
@@ -1103,7 +1103,7 @@ int gollek_paged_attention_prefill(void *out, const void *q, const void *k_cache
         if (workspace_bytes < need)
             return fail(GOLLEK_ERR_WORKSPACE, "workspace of %zu bytes < %zu needed", workspace_bytes, need);
     } else {
-        rc = library_workspace(dev, stream, need, &ws, &cap);
+        rc = library_workspace(dev, stream, Scratch::kSplitK, need, &ws, &cap);
         if (rc) return rc;
     }
     if (ws_counter_region(cap) + ws_partials_bytes(n, num_q_heads, num_kv_heads, head_dim) + lens_bytes > cap)

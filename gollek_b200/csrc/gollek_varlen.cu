@@ -254,7 +254,7 @@ int launch_tile(AttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
     int dev = 0;
     GK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
     if (!ws) {
-        int rc = library_workspace(dev, stream, c.total, &ws, &ws_bytes);
+        int rc = library_workspace(dev, stream, Scratch::kPlan, c.total, &ws, &ws_bytes);
         if (rc) return rc;
     }
     if (ws_bytes < c.total)

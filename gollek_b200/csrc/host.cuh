@@ -38,7 +38,10 @@ struct DeviceGuard {
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn();
 int sm_count(int dev);
-int library_workspace(int dev, void *stream, size_t bytes, void **out, size_t *cap_out = nullptr);
+// The library's scratch: kSplitK begins with arrival counters that are zero between calls; kPlan
+// holds whatever the last ragged or shared-prefix call left there.  Never one for the other.
+enum class Scratch { kSplitK, kPlan };
+int library_workspace(int dev, void *stream, Scratch kind, size_t bytes, void **out, size_t *cap_out = nullptr);
 int dtype_bytes(int dt);
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -245,9 +245,12 @@ GOLLEK_API int gollek_paged_attention_v2_noalloc(
  *                 documents: the first position of the query's own document).
  *   sliding_window > 0 needs causal (GOLLEK_ERR_UNSUPPORTED otherwise).
  *   workspace     >= gollek_paged_attention_varlen_workspace_size(...) bytes, 256-byte
- *                 aligned, its contents do not matter; not shared by calls that may overlap on the device (two
- *                 streams, two captured graphs).  NULL = library-owned scratch per (device,
- *                 stream), which such calls and graphs would share: pass a workspace there.
+ *                 aligned; its contents do not matter, and the call leaves anything there: zero
+ *                 a workspace again before gollek_paged_attention_v2 or _prefill may have it.
+ *                 Not shared by calls that may overlap on the device (two streams, two captured
+ *                 graphs).  NULL = library-owned scratch per (device, stream), apart from that of
+ *                 gollek_paged_attention_v2, which such calls and graphs would share: pass a
+ *                 workspace there.
  * Pool, scales, tables and num_blocks as in gollek_paged_attention_v2; any head_dim up to
  * 256, any GQA group.  K and V may hold anything before the first and behind the last
  * position that a query of their sequence attends; a NaN or infinity in between may also
