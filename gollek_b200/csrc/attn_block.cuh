@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kAbThreads) attn_block_kernel(const AttnArgs a
         }
     }
     __syncthreads();
-    const int first = span[0], last = span[1];
+    const int last = span[1], first = min(span[0], last);  // an empty span where no row sees anything
     // lane u < 4: the page of the warp's position u, looked up a tile ahead
     int next = lane < 4 && first + 4 * warp + lane < last ? bt[(first + 4 * warp + lane) / BS] : 0;
     for (int p0 = first; p0 < last; p0 += kAbTok) {
