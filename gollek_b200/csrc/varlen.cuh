@@ -132,7 +132,8 @@ __device__ __forceinline__ int group_of_seq(const AttnArgs &a, int s) {
     return (s >= s0 && s - s0 < n) ? lo : -1;
 }
 
-// Positions [lo, hi) that query token t, at position pos of sequence s (length len), attends.
+// Positions [lo, hi) that query token t, at position pos of sequence s (length len), attends; [0, 0)
+// where there are none, so that a caller's token_starts never enters a sum of positions.
 __device__ __forceinline__ void row_range(const AttnArgs &a, int s, int t, int pos, int len, int &lo, int &hi) {
     hi = len;
     if (a.causal) {
@@ -142,6 +143,7 @@ __device__ __forceinline__ void row_range(const AttnArgs &a, int s, int t, int p
     lo = 0;
     if (a.window > 0) lo = max(lo, pos - a.window + 1);
     if (a.token_starts) lo = max(lo, a.token_starts[t]);
+    if (lo >= hi) lo = hi = 0;
 }
 
 // ------------------------------------------------------------------ generic kernel
