@@ -254,6 +254,12 @@ int launch_tile(AttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
     int dev = 0;
     GK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
     if (!ws) {
+        // A graph would keep the library's scratch, which a larger call frees, and share it with other
+        // graphs and calls.
+        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+        GK_CUDA(cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capturing), "cudaStreamIsCapturing");
+        if (capturing != cudaStreamCaptureStatusNone)
+            return fail(GOLLEK_ERR_WORKSPACE, "a call that is being captured needs a workspace of its own");
         int rc = library_workspace(dev, stream, Scratch::kPlan, c.total, &ws, &ws_bytes);
         if (rc) return rc;
     }

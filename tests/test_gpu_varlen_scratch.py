@@ -99,3 +99,32 @@ def test_null_workspaces_of_all_entry_points_on_one_stream(cuda_device):
             same = torch.equal(out, alone[n]) if n in ("varlen", "shared") else torch.allclose(
                 out.float(), alone[n].float(), atol=2e-3, rtol=0)
             assert same, f"{n} in the order {order}"
+
+
+def test_a_captured_call_needs_its_own_workspace(cuda_device):
+    """NULL is refused under capture, where the library's scratch could be freed or shared behind the graph; the
+    capture goes on, and a graph with a workspace gives the eager call's rows."""
+    from gollek_b200 import _lib
+    calls = Calls(cuda_device)
+    want = [calls.varlen(0), calls.shared(0)]  # the default stream's scratch is large enough from here on
+    torch.cuda.synchronize()
+    graph, s = torch.cuda.CUDAGraph(), torch.cuda.Stream(cuda_device)
+    with torch.cuda.stream(s):
+        eager = [calls.varlen(s.cuda_stream), calls.shared(s.cuda_stream)]
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(eager, want))
+    n = _lib.load().gollek_paged_attention_varlen_workspace_size(4, 700, HQ, HKV, D)
+    ws, out = torch.empty(n, dtype=torch.uint8, device=cuda_device), torch.zeros_like(calls.qp)
+    with torch.cuda.graph(graph, stream=s):
+        for call in (calls.varlen, calls.shared):
+            with pytest.raises(_lib.GollekError) as e:
+                call(s.cuda_stream)
+            assert e.value.code == _lib.ERR_WORKSPACE and "captured" in str(e.value)
+        _lib.check(_lib.load().gollek_paged_attention_varlen(
+            out.data_ptr(), calls.qp.data_ptr(), *calls.pool(), calls.t.data_ptr(), calls.cu.data_ptr(), calls.c.data_ptr(),
+            None, None, None, 4, 700, HQ, HKV, D, BS, calls.t.shape[1], calls.nb, 0, _lib.BF16, _lib.BF16, 0, 0, 0,
+            1 / math.sqrt(D), 0.0, 0, 1, ws.data_ptr(), n, s.cuda_stream))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want[0])
+    del graph
