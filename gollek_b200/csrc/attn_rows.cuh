@@ -338,7 +338,26 @@ __global__ void __launch_bounds__(kRowsThreads + (Q8 ? kRowsConverters : 0), 1)
                     f *= 1.f / a.soft_cap;
 #pragma unroll
                     for (int r = 0; r < N; ++r) x[r] *= f;
-                    unit_cap(x);
+                    // each score in its own way: a position's 16 rows do not depend on one another, nor on the
+                    // warp's other positions; the vote only leaves out the second way where none needs it
+                    float big = 0.f;
+#pragma unroll
+                    for (int r = 0; r < N; ++r) big = fmaxf(big, fabsf(x[r]));
+                    if (__any_sync(0xffffffffu, big > 0.5f)) {
+#pragma unroll
+                        for (int r = 0; r < N; r += 2) {
+                            const float2 q = tanh_small(make_float2(x[r], x[r + 1]));
+                            x[r] = fabsf(x[r]) > 0.5f ? tanh_large(x[r]) : q.x;
+                            x[r + 1] = fabsf(x[r + 1]) > 0.5f ? tanh_large(x[r + 1]) : q.y;
+                        }
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < N; r += 2) {
+                            const float2 q = tanh_small(make_float2(x[r], x[r + 1]));
+                            x[r] = q.x;
+                            x[r + 1] = q.y;
+                        }
+                    }
                     f = a.soft_cap * kLog2e;
                 }
 #pragma unroll

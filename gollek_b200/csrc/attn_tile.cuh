@@ -516,30 +516,44 @@ __device__ __forceinline__ uint32_t scale_pair(uint32_t x, uint32_t by) {
     return d;
 }
 
-// w = tanh(w), warp-collective: on the FMA pipe where |w| <= 1/2 in the whole warp (the usual
-// case: caps are several times the scores), an odd polynomial of relative error below 2^-22;
-// else 1 - 2 / (1 + e^2w), two exponent-pipe operations.
+// tanh(y) of two values: an odd polynomial on the FMA pipe for |y| <= 1/2, the usual case (caps are
+// several times the scores), relative error 2^-25.9 (the minimax polynomial of tanh(y) / y in y^2
+// under the relative error, by Remez exchange) ...
+__device__ __forceinline__ float2 tanh_small(float2 y) {
+    const float2 y2 = mul2(y, y);
+    float2 q = fma2(y2, pair(0.01724149100482f), pair(-0.05304549261928f));
+    q = fma2(q, y2, pair(0.13325878977776f));
+    q = fma2(q, y2, pair(-0.33333143591881f));
+    return fma2(mul2(q, y2), y, y);
+}
+// ... and 1 - 2 / (1 + e^2y), two exponent-pipe operations, beyond.
+__device__ __forceinline__ float tanh_large(float y) {
+    return fmaf(-2.f, __fdividef(1.f, 1.f + fast_exp2(y * (2.f * kLog2e))), 1.f);
+}
+// w = tanh(w) of a row's N scores of a tile (what the others become does not matter), in the way
+// that the largest of those in `seen` needs: its bits depend on what the row attends alone.  Warp-
+// collective.
 template <int N>
-__device__ __forceinline__ void unit_cap(float (&w)[N]) {
+__device__ __forceinline__ void unit_cap(float (&w)[N], unsigned seen) {
+    if (opaque(__any_sync(0xffffffffu, seen != ~0u))) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = seen >> i & 1 ? w[i] : 0.f;
+    }
     float big = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) big = fmaxf(big, fabsf(w[i]));
-    if (__any_sync(0xffffffffu, !(big <= 0.5f))) {
+    if (big > 0.5f) {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            w[i] = fmaf(-2.f, __fdividef(1.f, 1.f + fast_exp2(w[i] * (2.f * kLog2e))), 1.f);
+        for (int i = 0; i < N; ++i) w[i] = tanh_large(w[i]);
     } else {
 #pragma unroll
         for (int i = 0; i < N; i += 2) {
-            const float2 y = make_float2(w[i], w[i + 1]), y2 = mul2(y, y);
-            float2 q = fma2(y2, pair(0.01724149100482f), pair(-0.05304549261928f));
-            q = fma2(q, y2, pair(0.13325878977776f));
-            q = fma2(q, y2, pair(-0.33333143591881f));
-            q = fma2(mul2(q, y2), y, y);
+            const float2 q = tanh_small(make_float2(w[i], w[i + 1]));
             w[i] = q.x;
             w[i + 1] = q.y;
         }
     }
+    __syncwarp();
 }
 
 // One lane of the converged warp, always the same.
@@ -1150,15 +1164,15 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
                         w[i] *= s4.x, w[i + 1] *= s4.y, w[i + 2] *= s4.z, w[i + 3] *= s4.w;
                     }
                 }
-                if constexpr (FEAT == kCap) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) w[i] *= cap1;
-                    unit_cap(w);
-                }
-                const float f = FEAT == kCap ? cap2 : a.q_scale;
                 const int l0 = jlo - k, h0 = jhi - k;
                 unsigned seen = h0 >= 32 ? ~0u : h0 <= 0 ? 0u : (1u << h0) - 1;
                 if (l0 > 0) seen = l0 >= 32 ? 0u : seen & (~0u << l0);
+                if constexpr (FEAT == kCap) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) w[i] *= cap1;
+                    unit_cap(w, seen);
+                }
+                const float f = FEAT == kCap ? cap2 : a.q_scale;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
                     float x = w[i] * f;
