@@ -10,7 +10,7 @@
 // One thread owns one position of a tile (an int8 position's scales are one load each) and
 // one column of the output.  P goes back through 4 KB of shared memory.  The reference m of a
 // row belongs to all 128 threads of a group, so they vote, tile by tile, whether any of
-// their scores passes it by 2^kLazyMax; only then is a maximum taken.
+// their scores passes it by kLazyMax; only then is a maximum taken.
 //
 // Bound by HBM for 16-bit caches, each page being read once per kv head: a decode step of 64
 // sequences of 512 to 8192 tokens (32 q, 8 kv heads of 128) takes 183 us, 6.2 TB/s (237 us
@@ -400,8 +400,8 @@ __global__ void __launch_bounds__(kRowsThreads + (Q8 ? kRowsConverters : 0), 1)
                     top = fmaxf(top, fl.z ? vmax[2 * N + r0] : -INFINITY);
                     top = fmaxf(top, fl.w ? vmax[3 * N + r0] : -INFINITY);
                     const bool move = top - was > kLazyMax<T>;
-                    const float by = move && was != -INFINITY ? ceilf(top - was) : 0.f;
-                    const float now = !move ? was : was == -INFINITY ? top : was + by;
+                    const float by = move && was != -INFINITY ? ceilf(top - was) - kBelowMax<T> : 0.f;
+                    const float now = !move ? was : was == -INFINITY ? top - kBelowMax<T> : was + by;
                     const float fall = fast_exp2(-by);
                     float alpha[N];
 #pragma unroll

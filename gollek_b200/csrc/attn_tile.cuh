@@ -15,8 +15,8 @@
 // of that MMA have one type: a half step of P, averaged over the positions, is of the size
 // of the output's own rounding.  An int8 cache's scales multiply S (K's) and P (V's), never
 // the integers, which would be one rounding more.  m is a lazy maximum: it moves, by a whole
-// number, only when a score passes it by more than 2^kLazyMax; l, O and the columns of P
-// that stand already are then scaled by a power of two.
+// number, only when a score passes it by more than kLazyMax; l, O and the columns of P that
+// stand already are then scaled by a power of two (exact but for f16's smallest numbers).
 //
 // Two row groups of 128 threads keep the tensor core busy while the other computes its
 // probabilities:
@@ -52,10 +52,15 @@ constexpr int kRunCostTiles = 2;      // start-up of a run (q, pipeline fill, ou
 constexpr int kMaxTileCtas = 160;
 constexpr int kTileThreads = 384;     // 8 row warps, 2 MMA issuers, 2 producers
 constexpr int kTileThreadsQ8 = 512;   // int8 caches: a fourth warpgroup converts
-// Scores may pass their row's reference by this much (log2 units) before it moves: P stays far
-// below the largest number of its type, and sums of it below fp32's.
+// Scores may pass their row's reference by this much (log2 units) before it moves: P stays
+// below the largest number of its type, and sums of it far below fp32's.
 template <typename T>
-constexpr float kLazyMax = std::is_same<T, __half>::value ? 12.f : 64.f;
+constexpr float kLazyMax = std::is_same<T, __half>::value ? 15.f : 64.f;
+// The reference is set this far below a maximum.  f16's smallest step is 2^-24: with P of 1 at the
+// maximum, probabilities of 2^-25 and less would be lost, and thousands of them beside one large score
+// are a share that shows.
+template <typename T>
+constexpr float kBelowMax = std::is_same<T, __half>::value ? 8.f : 0.f;
 
 // A block: rows row0 .. row0 + nrows - 1 (row r: query token tok0 + r / G, q head h G + r % G)
 // over positions [lo, hi) of table row `tab`, whose length is len.
@@ -502,17 +507,6 @@ __device__ __forceinline__ uint32_t byte_pair(uint32_t w) {
     const uint32_t x = __byte_perm(w, 0x43434343u, SEL);
     uint32_t a = x & 0xFF7FFF7Fu, b = x & 0xFF80FF80u, d;
     asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-    return d;
-}
-
-// A packed pair times a packed pair.
-template <typename T>
-__device__ __forceinline__ uint32_t scale_pair(uint32_t x, uint32_t by) {
-    uint32_t d;
-    if constexpr (std::is_same<T, __half>::value)
-        asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(by));
-    else
-        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(by));
     return d;
 }
 
@@ -1189,13 +1183,12 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
         // already and O (fresh: the group has none in this run yet; what stands there may be another
         // run's that group 0 is still reading).
         auto raise = [&](bool move, float top, float2 &acc, int stored, bool fresh) {
-            const float by = !move || m == -INFINITY ? 0.f : ceilf(top), alpha = fast_exp2(-by);
-            m = !move ? m : m == -INFINITY ? top : m + by;
+            const float by = !move || m == -INFINITY ? 0.f : ceilf(top) - kBelowMax<T>, alpha = fast_exp2(-by);
+            m = !move ? m : m == -INFINITY ? top - kBelowMax<T> : m + by;
             if (!__any_sync(0xffffffffu, by != 0.f)) return;
             l *= alpha;
             acc.x *= alpha;
             acc.y *= alpha;
-            const uint32_t a2 = pack2<T>(alpha, alpha);
             tmem_wait_ld();
             tmem_wait_st();
 #pragma unroll 1
@@ -1208,8 +1201,11 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
                 tmem_wait_ld();
                 uint32_t w[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    w[i] = is_o ? __float_as_uint(o[i] * alpha) : scale_pair<T>(__float_as_uint(o[i]), a2);
+                for (int i = 0; i < 8; ++i) {
+                    // (in fp32, whose range the factor needs; f16 pairs below 2^-14 are rounded once more)
+                    const float2 x = unpack2<T>(__float_as_uint(o[i]));
+                    w[i] = is_o ? __float_as_uint(o[i] * alpha) : pack2<T>(x.x * alpha, x.y * alpha);
+                }
                 tmem_st8(at, w);
             }
             tmem_wait_st();

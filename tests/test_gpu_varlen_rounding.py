@@ -11,6 +11,41 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 
+# ------------------------------------------------------------------------ small probabilities
+
+@pytest.mark.parametrize("d,new", [(128, 1), (64, 1), (64, 200), (128, 40)])
+@pytest.mark.parametrize("sink", [3990, 3700, 3685, 2000, 3])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_a_long_tail_behind_one_large_score(cuda_device, kind, d, new, sink):
+    """One position takes all but 2^-13.5 of the weight, and its value is 0: the output is the tail's, 4,000 positions
+    of weight 2^-25.5 each.
+
+    Tolerance: every tail probability is rounded to the cache's type, by half a step of the value (h) where the type has
+    its full precision there, else (f16) by half of 2^-24 in a scale where the largest probability is 2^7 or more: 2^-32
+    of it, twice if the column is scaled after it was stored.  The scores' own error: 18 products' sizes at 2^-24, 25.5
+    binary orders at 2^-23, exp2 2^-21: below 2^-16.  Then half a step of the output."""
+    hkv, grp, n, seqs, bs = 8, 2, 4000, 8, 16
+    rng = np.random.default_rng(91)
+    pages = n // bs
+    table = rng.permutation(pages + 2)[:pages].astype(np.int32)
+    k = np.zeros((pages + 2, hkv, bs, d))
+    v = np.full((pages + 2, hkv, bs, d), 1000.0)
+    at = table[sink // bs], slice(None), sink % bs
+    k[at + (0,)] = 25.5 * np.log(2) * np.sqrt(d)
+    v[at] = 0.0
+    pool = R.Pool(kind, k, v)
+    q = np.zeros((seqs * new, hkv * grp, d))
+    q[..., 0] = 1.0
+    tables = np.repeat(table[None], seqs, axis=0)
+    cu = (np.arange(seqs + 1) * new).astype(np.int32)
+    ctx = np.full(seqs, n, np.int32)
+    got = run_varlen(cuda_device, q, pool, tables, cu, ctx, kind, causal=False).double().cpu().numpy()
+    want = R.varlen(q[:1], pool, tables[:1], np.array([0, 1]), ctx[:1], 1 / np.sqrt(d), causal=False)[0, 0]
+    assert want[0] > 0.05
+    tol = (2 * R.HALF_STEP[kind] + 2.0 ** -15) * want + (2 * n * 2.0 ** -32 * 1000 if kind == "f16" else 0)
+    assert (np.abs(got - want) <= tol).all(), f"{got.min()} .. {got.max()}, not {want[0]}"
+
+
 # ------------------------------------------------------------------------ same bits
 
 def unseen_filled(k, v, tables, ctx, bs, value):
