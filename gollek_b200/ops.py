@@ -220,6 +220,8 @@ class _on:
             return torch._C._cuda_getCurrentRawStream(self.device.index)
         if self.given is not None:
             s = self.given
+            if getattr(s, "device", self.device) != self.device:
+                raise ValueError(f"stream is on {s.device}, not {self.device}")
             if not hasattr(s, "cuda_stream"):
                 s = torch.cuda.ExternalStream(int(s), device=self.device)
             self.guard = torch.cuda.stream(s)
