@@ -85,12 +85,12 @@ __global__ void __launch_bounds__(kRowsThreads + (Q8 ? kRowsConverters : 0), 1)
     uint64_t *vote = q_free + 2;   // [2] the group's warps have looked at their scores
     uint64_t *sums_full = vote + 2; // [2] the group's (m, l) of a run written
     uint64_t *drained = sums_full + 2;
-    uint32_t *sm_tmem = reinterpret_cast<uint32_t *>(tile_smem + L::misc + 4);
+    uint32_t *sm_tmem = reinterpret_cast<uint32_t *>(tile_smem + L::misc + 8);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         constexpr int conv = kRowsConverters / 32;
-        pipe.init(Q8 ? conv : 2, 1, 9 + (Q8 ? conv : 0));
+        pipe.init(Q8 ? conv : 2, 1, 9 + (Q8 ? conv : 0), p.wait_tries);
         for (int t = 0; t < 2; ++t) {
             mbar_init(&s_full[t], 1);
             mbar_init(&p_full[t], 4);

@@ -122,6 +122,10 @@ struct TileArgs {
     int blk_rows;     // rows a block may have
     int rows_min, rows_max;  // entities of rows_min .. rows_max rows are this line's, the rest another's
     long long page_rows;
+    // Tests of the waits that give up (host: test_hooks): tests a wait may take, and the tiles
+    // behind which CTA 0's producers stop (-1: none).
+    unsigned wait_tries;
+    int stop_at;
 };
 
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -413,19 +417,21 @@ struct __align__(16) RunDesc {
 
 // Bounded wait of a whole warp: each lane tests on its own, one vote at the end (the
 // result is warp-uniform); gives up once another warp did.  The warp that gives up first
-// raises the status (tile_give_up) at the end of its role.  One copy of the code for all
-// waits: see opaque() on why size matters here.
+// raises the status (tile_give_up) at the end of its role.  The number of tests allowed
+// stands behind the abort flag.  One copy of the code for all waits: see opaque() on why size
+// matters here.
 __device__ __noinline__ bool tile_wait(uint32_t bar, uint32_t parity, uint32_t abort) {
     bool ok = false;
+    uint32_t tries = 1;
 #pragma unroll 1
-    for (unsigned i = 0; !ok && i < kSuspendTries; ++i) {
+    for (unsigned i = 0; !ok && i < tries; ++i) {
         uint32_t done, gone;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%2], %3, %5;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%3], %4, %6;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t"
-            "ld.volatile.shared.u32 %1, [%4];\n\t}"
-            : "=r"(done), "=r"(gone)
+            "ld.volatile.shared.v2.u32 {%1, %2}, [%5];\n\t}"
+            : "=&r"(done), "=&r"(gone), "=&r"(tries)
             : "r"(bar), "r"(parity), "r"(abort), "r"(kSuspendNs)
             : "memory");
         ok = done != 0;
@@ -608,7 +614,7 @@ struct TilePipe {
         abort = reinterpret_cast<volatile int *>(base + L::misc);
     }
     // by one thread; `fillers` warps arrive on full, `readers` on empty, `users` read a descriptor
-    __device__ __forceinline__ void init(int fillers, int readers, int users) const {
+    __device__ __forceinline__ void init(int fillers, int readers, int users, unsigned tries) const {
         for (int i = 0; i < L::kSlots; ++i) {
             mbar_init(&full[i], fillers);
             mbar_init(&empty[i], readers);
@@ -621,7 +627,8 @@ struct TilePipe {
             mbar_init(&run_full[i], 1);
             mbar_init(&run_free[i], users);
         }
-        *abort = 0;
+        abort[0] = 0;
+        abort[1] = tries;  // ([2]: the tensor memory's address)
     }
     // by a whole warp; the call is left to waits that have something to wait for (it takes some
     // 350 clocks)
@@ -705,12 +712,16 @@ __device__ __forceinline__ void tile_producer(const TileArgs &p, const TilePipe<
                                      : a.block_tables + static_cast<long long>(r.b.tab) * a.max_blocks;
             t = ta = r.ta;
             tb = more ? r.tb : r.ta;
+            if (p.stop_at >= 0 && blockIdx.x == 0) {
+                tb = min(tb, ta + p.stop_at);
+                more = false;
+            }
         }
         if (t < tb) {
             s2.live = true;
             s2.first = t == ta;
-            s2.last = t == tb - 1;
-            const int at = (r.b.lo / kTileTok + tb - 1 - (t - ta)) * kTileTok + lane * 16;
+            s2.last = t == r.tb - 1;
+            const int at = (r.b.lo / kTileTok + r.tb - 1 - (t - ta)) * kTileTok + lane * 16;
             s2.at.h = r.h;
             // (straight-line, so that nothing waits for an entry before it is resolved)
 #pragma unroll
@@ -916,11 +927,11 @@ __global__ void __launch_bounds__(Q8 ? kTileThreadsQ8 : kTileThreads, 1)
     uint64_t *drained = q_free + 2;            // [2] an issuer's MMAs done
     uint64_t *turn = drained + 2;              // [2][4] group t's warp may use the exponent pipe
     uint64_t *ml_full = turn + 8;              // group 1's (m, l) handed over
-    uint32_t *sm_tmem = reinterpret_cast<uint32_t *>(tile_smem + L::misc + 4);
+    uint32_t *sm_tmem = reinterpret_cast<uint32_t *>(tile_smem + L::misc + 8);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        pipe.init(Q8 ? 4 : 2, 2, Q8 ? 14 : 10);
+        pipe.init(Q8 ? 4 : 2, 2, Q8 ? 14 : 10, p.wait_tries);
         for (int t = 0; t < 2; ++t) {
             mbar_init(&s_full[t], 1);
             mbar_init(&p_full[t], 4);

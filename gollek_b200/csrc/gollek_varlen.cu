@@ -1,6 +1,7 @@
 // gollek_varlen.cu -- host side of ragged and shared-prefix paged attention and of the
 // cache read-back: argument checks, kernel selection and their C ABI (gollek_kernels.h).
 #include <algorithm>
+#include <cstdlib>
 
 #include "attn_block.cuh"
 #include "attn_rows.cuh"
@@ -247,6 +248,15 @@ int launch_tile_as(const PlanArgs &both, int lines, const CUtensorMap &tmk, cons
                             0, st, margs, "tile_merge_shared_kernel launch");
 }
 
+// Hooks of the failure-detection tests (unset in normal use), those of the split-K kernels: a short
+// bound for the waits (a test suspends for up to 20 us: 64 of the others'), and the tiles of CTA 0's
+// first run behind which its producers issue no copies any more.
+void test_hooks(TileArgs &p) {
+    const char *limit = std::getenv("GOLLEK_TEST_WAIT_LIMIT"), *skip = std::getenv("GOLLEK_TEST_SKIP_GROUP");
+    p.wait_tries = limit ? std::max(1u, static_cast<unsigned>(std::strtoul(limit, nullptr, 10)) >> 6) : kSuspendTries;
+    p.stop_at = skip ? std::atoi(skip) : -1;
+}
+
 int launch_tile(AttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
     const CallPlan c = plan_call(a.num_groups, a.num_seqs, a.total_q, a.num_q_heads, a.num_kv_heads, a.head_dim);
     if (std::max(c.line[0].ws.max_blocks, c.line[1].ws.max_blocks) > (1LL << 22))
@@ -289,6 +299,7 @@ int launch_tile(AttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
         p.rows_max = l.rows_max;
         p.max_blocks = static_cast<int>(w.max_blocks);
         p.page_rows = a.page_stride / a.head_dim;
+        test_hooks(p);
         p.grid = std::min(std::max(1, sm_count(dev)), kMaxTileCtas);
     }
     CUtensorMap tmk{}, tmv{};

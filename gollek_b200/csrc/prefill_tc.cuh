@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const Schedule sch = schedule_prologue(a, sm_prefix, sm_cprefix, sm_len, sm_rstart, &sm_misc[1],
                                            reinterpret_cast<int *>(smem + L.p));
 
-    // tries of a suspending wait (GOLLEK_TEST_WAIT_LIMIT shortens them, as for every wait)
+    // tries of a suspending wait (GOLLEK_TEST_WAIT_LIMIT shortens them)
     const unsigned it_tries = a.wait_limit ? max(1u, a.wait_limit >> 6) : kSuspendTries;
 
     // Sequences with nothing to attend to: zeros, written by CTA s % grid (threads 0-63).
