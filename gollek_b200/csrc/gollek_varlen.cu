@@ -137,16 +137,18 @@ struct CallPlan {
 // attn_rows_kernel (head_dim 128, up to 16 q heads per kv head) takes entities of 16 rows at
 // most: 237 -> 183 us for 64 sequences of one token.  What a call gives it, and what the kernel
 // for many rows, is chosen from the sizes alone:
-// - varlen, no more query tokens than sequences: all, whatever their rows (a longer entity is
-//   cut into blocks of 16, each of which reads its pages);
-// - otherwise, once the sequences give the device kSplitUnits units of work: varlen, the entities
-//   of few rows, the rest going to the kernel for many (60 decode steps beside 4 chunks of 200
-//   tokens 392 -> 281 us, beside 4 of 1000 645 -> 533, 64 sequences of 8 tokens 222.5 -> 223.4);
-//   shared prefixes, the own tokens (64 sequences behind 4,096 tokens 82 -> 67 us).  Below, the
-//   launch costs more than it saves (8 sequences behind 500 tokens 19.6 us, 26.5 in two).
+// - varlen, no more query tokens than sequences: all, whatever their rows (64 decode steps at 1,024
+//   tokens 71 us, with both kernels launched 79).  A longer entity is cut into blocks of 16, each of which
+//   reads its pages: a chunk of 512 tokens at 4,096 among 511 idle slots takes 313 us, in both 82.
+// - otherwise, once the sequences give the device enough units of work (sequences times kv heads):
+//   varlen, from kSplitVarlen units, the entities of few rows, the rest going to the kernel for many
+//   (decode steps at 1,024 tokens beside 2 chunks of 300 at 2,048: 128 units 87.5 us in one kernel
+//   and 89.2 in two, 192: 97.2 and 97.3, 256: 107.6 and 104.4, 512: 151.6 and 125.0);
+//   shared prefixes, from kSplitShared, the own tokens (sequences of 300 tokens behind 4,096: 192
+//   units 42.0 and 51.2, 256: 45.6 and 54.3, 384: 62.0 and 62.4, 512: 77.2 and 70.0).
 // The layout of the workspace does not depend on the choice, so that what is enough for a call
 // is enough for smaller ones.
-constexpr int kSplitUnits = 256;
+constexpr int kSplitVarlen = 256, kSplitShared = 384;
 
 CallPlan plan_call(int num_groups, int num_seqs, int total_q, int hq, int hkv, int D) {
     const int G = hq / hkv;
@@ -163,7 +165,7 @@ CallPlan plan_call(int num_groups, int num_seqs, int total_q, int hq, int hkv, i
     c.total += few.ws.total;
     if (!shared && total_q <= num_seqs) {
         c.line[0] = few;
-    } else if (static_cast<long long>(num_seqs) * hkv >= kSplitUnits) {
+    } else if (static_cast<long long>(num_seqs) * hkv >= (shared ? kSplitShared : kSplitVarlen)) {
         c.lines = 2;
         c.line[1] = few;
         if (shared) {

@@ -77,7 +77,7 @@ def test_counts_of_many_sequences_in_turn(cuda_device, kind, hq, hkv, bs, d):
 @pytest.mark.parametrize("kind,qkind", KINDS)
 @pytest.mark.parametrize("seqs,plens,starts,hq,hkv,d", [
     (70, [2100], [0, 70], 8, 2, 128), (43, [130, 50, 0, 1700], [2, 9, 9, 14, 40], 8, 2, 128), (9, [5000], [0, 9], 6, 2, 64),
-    (64, [900, 16], [0, 30, 64], 16, 4, 128)])
+    (64, [900, 16], [0, 30, 64], 16, 4, 128), (130, [900, 16, 0], [3, 60, 100, 128], 16, 4, 128)])
 def test_counts_behind_shared_prefixes(cuda_device, kind, qkind, seqs, plens, starts, hq, hkv, d):
     rng = np.random.default_rng(106)
     ctx = np.where(rng.random(seqs) < 0.2, 0, rng.integers(1, 500, seqs)).astype(np.int32)
@@ -115,7 +115,8 @@ def test_norms_over_long_contexts(cuda_device, ctx, new, kind, qkind, what):
 
 
 @pytest.mark.parametrize("kind,qkind", [("bf16", "bf16"), ("f16", "f16"), ("i8", "bf16"), ("f32", "f32")])
-@pytest.mark.parametrize("seqs,plen,hq,hkv,d", [(1, 5000, 8, 2, 128), (70, 2100, 8, 2, 128), (33, 640, 8, 2, 64)])
+@pytest.mark.parametrize("seqs,plen,hq,hkv,d", [(1, 5000, 8, 2, 128), (70, 2100, 8, 2, 128), (33, 640, 8, 2, 64),
+                                                 (50, 1500, 16, 8, 128), (130, 700, 32, 4, 128)])
 def test_norms_behind_a_shared_prefix(cuda_device, kind, qkind, seqs, plen, hq, hkv, d):
     rng = np.random.default_rng(111)
     case = shared_case([plen], [0, seqs], rng.integers(0, 300, seqs), hq, hkv, d, 16, kind, qkind, 112)

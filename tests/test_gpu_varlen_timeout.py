@@ -45,7 +45,7 @@ def test_a_wait_gives_up_then_the_next_call_is_right(cuda_device, monkeypatch, k
 def test_a_wait_behind_a_shared_prefix_gives_up(cuda_device, monkeypatch):
     """Two kernels in a row (the prefix's and the own tokens'): both stop, both leave."""
     from gollek_b200 import _lib, ops
-    case = shared_case([30000], [0, 64], [400] * 64, 16, 4, 128, 16, "bf16", "bf16", 131)
+    case = shared_case([30000], [0, 64], [400] * 64, 32, 8, 128, 16, "bf16", "bf16", 131)
     ops.device_status(cuda_device.index or 0)
     want = run_shared(cuda_device, case, "bf16")
     monkeypatch.setenv("GOLLEK_TEST_WAIT_LIMIT", "20000")
