@@ -313,8 +313,9 @@ def paged_attention_shared_prefix(q, k_cache, v_cache, prefix_tables, prefix_len
                                   out=None, workspace=None, stream=None):
     """Decode attention of groups that share prefixes (gollek_paged_attention_shared_prefix):
     q [S, Hq, D] fp32/bf16/f16; sequences group_starts[g] .. group_starts[g+1] - 1 attend the
-    prefix_lens[g] tokens of prefix_tables[g], read once for 256 of the group's rows, and their own
-    context_lens[s] tokens."""
+    prefix_lens[g] tokens of prefix_tables[g] and their own context_lens[s] tokens.  The tensor-core
+    kernels read a prefix once for 256 of its group's rows, the generic kernel (fp32 and int4
+    caches, q of another type, other head_dims) once per sequence."""
     dev = _first("q", q, 3)
     S, Hq, D = q.shape
     if q.dtype not in _FLOAT:

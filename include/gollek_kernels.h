@@ -278,8 +278,10 @@ GOLLEK_API size_t gollek_paged_attention_varlen_workspace_size(int num_seqs, int
 /*
  * Decode attention of a batch whose sequences share prefixes: sequences group_starts[g] ..
  * group_starts[g+1] - 1 all attend the prefix_lens[g] tokens of group g's table and then
- * their own context_lens[s] tokens, one softmax over both; the prefix is read once for each
- * 256 rows (sequence, q head) of a kv head, not once per sequence.  The pages of a prefix are those that the prompt cache shares between requests
+ * their own context_lens[s] tokens, one softmax over both.  The tensor-core kernels (see
+ * gollek_paged_attention_varlen for the calls they take) read the prefix once for each 256 rows
+ * (sequence, q head) of a kv head; every other call reads it once per sequence.  The pages of a
+ * prefix are those that the prompt cache shares between requests
  * (optimization/gollek-plugin-prompt-cache/src/main/java/tech/kayys/gollek/cache/PagedKVCacheManagerExtension.java:45-180).
  *
  *   q, out         [num_seqs, num_q_heads, head_dim] of q_dtype (F32, BF16 or F16).
