@@ -2,6 +2,7 @@
 // cache read-back: argument checks, kernel selection and their C ABI (gollek_kernels.h).
 #include <algorithm>
 #include <cstdlib>
+#include <mutex>
 
 #include "attn_block.cuh"
 #include "attn_rows.cuh"
@@ -259,13 +260,20 @@ void test_hooks(TileArgs &p) {
     p.stop_at = skip ? std::atoi(skip) : -1;
 }
 
+// Held by a call that uses the library's scratch until its launches are in the stream: the plan, the
+// attention and the merge of two host threads' calls on one stream would otherwise mix, one's
+// kernels working from the other's plan.
+std::mutex g_plan_mu;
+
 int launch_tile(AttnArgs &a, void *ws, size_t ws_bytes, void *stream) {
     const CallPlan c = plan_call(a.num_groups, a.num_seqs, a.total_q, a.num_q_heads, a.num_kv_heads, a.head_dim);
     if (std::max(c.line[0].ws.max_blocks, c.line[1].ws.max_blocks) > (1LL << 22))
         return fail(GOLLEK_ERR_UNSUPPORTED, "too many query rows for one call");
     int dev = 0;
     GK_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
+    std::unique_lock<std::mutex> whole_call(g_plan_mu, std::defer_lock);
     if (!ws) {
+        whole_call.lock();
         // A graph would keep the library's scratch, which a larger call frees, and share it with other
         // graphs and calls.
         cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;

@@ -247,10 +247,12 @@ GOLLEK_API int gollek_paged_attention_v2_noalloc(
  *   workspace     >= gollek_paged_attention_varlen_workspace_size(...) bytes, 256-byte
  *                 aligned; its contents do not matter, and the call leaves anything there: zero
  *                 a workspace again before gollek_paged_attention_v2 or _prefill may have it.
- *                 Not shared by calls that may overlap on the device (two streams, two captured
- *                 graphs).  NULL = library-owned scratch per (device, stream), apart from that of
- *                 gollek_paged_attention_v2; refused (GOLLEK_ERR_WORKSPACE) while `stream` is
- *                 being captured, if the call needs scratch.
+ *                 One call at a time has it, from its entry to the end of its work on the device
+ *                 (not two streams, two captured graphs or two host threads at once).  NULL =
+ *                 library-owned scratch per (device, stream), apart from that of
+ *                 gollek_paged_attention_v2 and safe from any thread; refused
+ *                 (GOLLEK_ERR_WORKSPACE) while `stream` is being captured, if the call needs
+ *                 scratch.
  * Pool, scales, tables and num_blocks as in gollek_paged_attention_v2; any head_dim up to
  * 256, any GQA group.  K and V may hold anything before the first and behind the last
  * position that a query of their sequence attends; a NaN or infinity in between may also

@@ -128,3 +128,32 @@ def test_a_captured_call_needs_its_own_workspace(cuda_device):
     torch.cuda.synchronize()
     assert torch.equal(out, want[0])
     del graph
+
+
+def test_two_host_threads_on_one_stream(cuda_device):
+    """Calls with NULL workspaces from two threads: each call's kernels follow one another in the stream."""
+    import threading
+    calls = Calls(cuda_device)
+    s = torch.cuda.Stream(cuda_device)
+    want, wrong = {}, []
+    with torch.cuda.stream(s):
+        for n in ("varlen", "shared"):
+            want[n] = getattr(calls, n)(s.cuda_stream)
+    s.synchronize()
+
+    def work(name):
+        try:
+            with torch.cuda.stream(s):
+                for _ in range(100):
+                    if not torch.equal(getattr(calls, name)(s.cuda_stream), want[name]):
+                        wrong.append(name)
+        except Exception as e:  # noqa: BLE001 -- reported by the main thread
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in ("varlen", "shared", "varlen")]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong, wrong[:3]
