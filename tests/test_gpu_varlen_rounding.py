@@ -57,9 +57,10 @@ def unseen_filled(k, v, tables, ctx, bs, value):
 
 @pytest.mark.parametrize("kind,qkind", [("bf16", "bf16"), ("f16", "f16"), ("i8", "bf16")])
 @pytest.mark.parametrize("ctx,new", [([300, 45, 129, 1000, 8] * 8, [1] * 40), ([300, 45, 203, 1000], [90, 30, 203, 7])])
-def test_capped_bits_do_not_depend_on_what_nobody_attends(cuda_device, kind, qkind, ctx, new):
-    """With a soft-cap, whatever slots behind a sequence hold, and whatever calls ran before."""
-    d, bs, hq, hkv, cap = 128, 16, 8, 2, 30.0
+@pytest.mark.parametrize("cap", [30.0, 0.0])
+def test_bits_do_not_depend_on_what_nobody_attends(cuda_device, kind, qkind, ctx, new, cap):
+    """Whatever slots behind a sequence hold, and whatever calls ran before."""
+    d, bs, hq, hkv = 128, 16, 8, 2
     ctx = np.array(ctx, np.int32)
     rng = np.random.default_rng(92)
     q, pool, tables, cu, ctx = varlen_case(ctx, new, hq, hkv, d, bs, "f32", qkind, 93, plant=False)
